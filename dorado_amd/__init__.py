@@ -5,6 +5,7 @@ Layout:
   csrc/      hand-written gfx950 HIP kernels + the C-ABI shared library (include/mibc.h)
   config.py  host mirror of dorado/config (BasecallModelConfig, BatchParams)
   capi.py    ctypes binding of the C-ABI (the only way Python reaches the kernels)
+  ops.py     transformer-layer operators on torch tensors (RMS norm, rotary positions, masked attention)
   host/      C++ mirror of basecall::ModelRunnerBase / CudaCaller / BasecallerNode (libmibc_host.so)
   hostapi.py ctypes binding of the host layer
   dist.py    one-process-per-GPU plumbing (replicas only, no data-path collective)

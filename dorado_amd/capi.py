@@ -51,6 +51,7 @@ EXPORTS = [
     "mibc_forward_i16", "mibc_call_device_i16", "mibc_call_i16", "mibc_scaler_stats", "mibc_scale_reads",
     "mibc_svb16_decode", "mibc_forward_var", "mibc_call_device_var", "mibc_call_var",
     "mibc_call_async", "mibc_call_wait", "mibc_call_poll", "mibc_call_var_async",
+    "mibc_rms_norm", "mibc_rope", "mibc_rope_frequencies", "mibc_attention", "mibc_attention_workspace",
 ]
 
 SCALE_QUANTILE = 0

@@ -1,0 +1,25 @@
+// dorado_amd/csrc/ops_attention.h — what the host half (ops_attention.hip) hands to the kernels (ops_attention_kernels.hip, compiled
+// once per head size).
+#pragma once
+#include "ops.h"
+
+struct AttArgs {
+    mibc_attention_args a;
+    int group;        // query heads per key head
+    int rows;         // q_tokens * group: row r = (token r / group, head r % group) of a (batch, key head) pair
+    int pairs;        // batch * kv_heads
+    int tiles;        // row tiles per pair
+    int splits;       // parts the keys of a tile are split into, joined by the second launch if > 1
+    int order;        // workgroup -> (pair, tile, split): 0 pairs innermost, 1 tiles innermost (one pair stays on one XCD)
+    float scale2;     // scale * log2(e)
+    float cap_in, cap_out;   // scores / cap in, cap out: 2 * scale / cap * log2(e), cap * log2(e); 0: no cap
+    float *part_o;    // [pairs * rows][splits][D] f32
+    float *part_l;    // [pairs * rows][splits] log2 of the sum
+};
+
+// variant: 0 row tiles of 256, 1 of 128, 2 of 64, 3 at most 16 rows per pair (single tokens)
+#define MIBC_ATT_DECLARE(D) int mibc_att_launch_##D(hipStream_t s, const AttArgs &p, int variant, unsigned grid);
+MIBC_ATT_DECLARE(32)
+MIBC_ATT_DECLARE(64)
+MIBC_ATT_DECLARE(96)
+MIBC_ATT_DECLARE(128)

@@ -1,0 +1,127 @@
+// dorado_amd/csrc/ops_attention.hip — host half of mibc_attention: checks, choice of the kernel and of the split over the keys.
+#include "ops_attention.h"
+
+#include <math.h>
+
+static int att_check(const mibc_attention_args &a) {
+    if (a.type != MIBC_TYPE_F16 && a.type != MIBC_TYPE_BF16) return op_refuse(MIBC_NOT_SUPPORTED, "attention: type must be f16 or bf16");
+    if (a.head_dim != 32 && a.head_dim != 64 && a.head_dim != 96 && a.head_dim != 128)
+        return op_refuse(MIBC_NOT_SUPPORTED, "attention: head_dim must be 32, 64, 96 or 128");
+    if (a.batch < 0 || a.q_tokens < 0 || a.k_tokens < 0 || a.heads < 1 || a.kv_heads < 1)
+        return op_refuse(MIBC_ERR_ARG, "attention: negative size, or no heads");
+    if (a.heads % a.kv_heads != 0) return op_refuse(MIBC_ERR_ARG, "attention: heads must be a multiple of kv_heads");
+    if (!(a.scale > 0.0f) || !(a.scale <= 1e30f)) return op_refuse(MIBC_ERR_ARG, "attention: scale must be positive and finite");
+    if (!(a.softcap >= 0.0f) || !(a.softcap <= 1e30f)) return op_refuse(MIBC_ERR_ARG, "attention: softcap must be 0 (none) or positive and finite");
+    if (a.reserved != 0) return op_refuse(MIBC_ERR_ARG, "attention: reserved must be 0");
+    const int64_t big = (int64_t)1 << 30;
+    if (a.q_tokens > big || a.k_tokens > big || (int64_t)a.q_tokens * (a.heads / a.kv_heads) > big ||
+        (int64_t)a.batch * a.kv_heads > big || (a.q_start != MIBC_ATTN_END && (a.q_start > big || a.q_start < -big)))
+        return op_refuse(MIBC_NOT_SUPPORTED, "attention: more than 2^30 tokens, rows or heads");
+    if (a.doc_offsets != nullptr) {
+        if (a.batch != 1 || a.q_tokens != a.k_tokens || a.k_len != nullptr || a.q_start != MIBC_ATTN_END)
+            return op_refuse(MIBC_ERR_ARG, "attention: documents need batch 1, q_tokens == k_tokens, no k_len and no q_start");
+        if (a.n_docs < 0 || a.n_docs > big) return op_refuse(MIBC_ERR_ARG, "attention: n_docs");
+    } else if (a.n_docs != 0) {
+        return op_refuse(MIBC_ERR_ARG, "attention: n_docs without doc_offsets");
+    }
+    if (a.batch == 0 || a.q_tokens == 0) return MIBC_OK;
+    if (a.q == nullptr || a.out == nullptr || (a.k_tokens > 0 && (a.k == nullptr || a.v == nullptr)))
+        return op_refuse(MIBC_ERR_ARG, "attention: null pointer");
+    const int64_t qs[3] = {a.batch, a.q_tokens, a.heads}, ks[3] = {a.batch, a.k_tokens, a.kv_heads};
+    for (int d = 0; d < 3; ++d) {
+        if (a.q_stride[d] < 0 || a.k_stride[d] < 0 || a.v_stride[d] < 0) return op_refuse(MIBC_ERR_ARG, "attention: negative stride");
+        if (qs[d] > 1 && a.out_stride[d] < a.head_dim) return op_refuse(MIBC_ERR_ARG, "attention: output heads overlap");
+        if ((qs[d] > 1 && (a.q_stride[d] % 8 != 0 || a.out_stride[d] % 8 != 0)) || (ks[d] > 1 && (a.k_stride[d] % 8 != 0 || a.v_stride[d] % 8 != 0)))
+            return op_refuse(MIBC_NOT_SUPPORTED, "attention: strides must be multiples of 8 elements");
+    }
+    // a tile's rows are reached through 32-bit offsets from its first one
+    if (a.k_tokens > 1 && (a.k_stride[1] > (1 << 24) || a.v_stride[1] > (1 << 24)))
+        return op_refuse(MIBC_NOT_SUPPORTED, "attention: key and value tokens at most 2^24 elements apart");
+    if (!op_aligned(a.q, 16) || !op_aligned(a.out, 16) || !op_aligned(a.k, 16) || !op_aligned(a.v, 16))
+        return op_refuse(MIBC_NOT_SUPPORTED, "attention: pointers must be aligned to 16 bytes");
+    if (!op_aligned(a.lse, 4) || !op_aligned(a.k_len, 4) || !op_aligned(a.prefix, 4) || !op_aligned(a.doc_offsets, 4) || !op_aligned(a.slopes, 4))
+        return op_refuse(MIBC_ERR_ARG, "attention: pointer not aligned to its type");
+    return MIBC_OK;
+}
+
+struct AttPlan {
+    int variant, tiles, splits;
+};
+static AttPlan att_plan(const mibc_attention_args &a) {
+    const int64_t rows = (int64_t)a.q_tokens * (a.heads / a.kv_heads), pairs = (int64_t)a.batch * a.kv_heads;
+    AttPlan p;
+    p.variant = rows > 128 ? 0 : rows > 64 ? 1 : 2;
+    const int tile = p.variant == 0 ? 256 : p.variant == 1 ? 128 : 64;
+    p.tiles = (int)((rows + tile - 1) / tile);
+    // keys a row can see at most, in tiles of 64
+    int64_t keys = a.k_tokens;
+    if (a.window_back >= 0 && a.window_ahead >= 0 && a.prefix == nullptr) {
+        const int64_t w = (int64_t)a.window_back + a.window_ahead + 1 + tile;
+        keys = keys < w ? keys : w;
+    }
+    const int64_t ktiles = (keys + 63) / 64, groups = p.tiles * pairs;
+    int64_t splits = groups >= 512 ? 1 : 512 / groups;
+    if (splits > ktiles / 4) splits = ktiles / 4;     // a part is worth its share of the join from four tiles on
+    p.splits = splits < 1 ? 1 : (int)splits;
+    return p;
+}
+
+static uint64_t att_room(const mibc_attention_args &a, const AttPlan &p) {
+    return p.splits == 1 ? 0 : (uint64_t)a.batch * a.heads * a.q_tokens * p.splits * (a.head_dim + 1) * 4;
+}
+static int att_check_plan(const mibc_attention_args &a, const AttPlan &p) {
+    if ((int64_t)a.batch * a.kv_heads * p.tiles * p.splits > 0x7fffffff) return op_refuse(MIBC_NOT_SUPPORTED, "attention: too many row tiles");
+    const uint64_t need = att_room(a, p);
+    if (need == 0) return MIBC_OK;
+    if (a.workspace == nullptr || a.workspace_bytes < need)
+        return op_refuse(MIBC_ERR_ARG, "attention: workspace smaller than mibc_attention_workspace says");
+    if (!op_aligned(a.workspace, 16)) return op_refuse(MIBC_ERR_ARG, "attention: workspace must be aligned to 16 bytes");
+    return MIBC_OK;
+}
+
+extern "C" uint64_t mibc_attention_workspace(const mibc_attention_args *a) {
+    if (a == nullptr || att_check(*a) != MIBC_OK || a->batch == 0 || a->q_tokens == 0) return 0;
+    return att_room(*a, att_plan(*a));
+}
+
+// launch on a stream of the current device (the engine's own path); checks included
+int mibc_launch_attention(hipStream_t s, const mibc_attention_args &a) {
+    if (const int rc = att_check(a)) return rc;
+    if (a.batch == 0 || a.q_tokens == 0) return MIBC_OK;
+    const AttPlan plan = att_plan(a);
+    if (const int rc = att_check_plan(a, plan)) return rc;
+    AttArgs p{};
+    p.a = a;
+    p.group = a.heads / a.kv_heads;
+    p.rows = a.q_tokens * p.group;
+    p.pairs = a.batch * a.kv_heads;
+    p.tiles = plan.tiles;
+    p.splits = plan.splits;
+    p.scale2 = a.scale * 1.4426950408889634f;
+    if (a.softcap > 0.0f) {
+        p.cap_in = 2.0f * a.scale / a.softcap * 1.4426950408889634f;
+        p.cap_out = a.softcap * 1.4426950408889634f;
+    }
+    if (plan.splits > 1) {
+        p.part_o = (float *)a.workspace;
+        p.part_l = p.part_o + (uint64_t)p.pairs * p.rows * p.splits * a.head_dim;
+    }
+    const int64_t grid = (int64_t)p.pairs * p.tiles * p.splits;
+    p.order = (a.window_ahead != 0 && p.pairs % 8 == 0) ? 1 : 0;
+    switch (a.head_dim) {
+        case 32: return mibc_att_launch_32(s, p, plan.variant, (unsigned)grid);
+        case 64: return mibc_att_launch_64(s, p, plan.variant, (unsigned)grid);
+        case 96: return mibc_att_launch_96(s, p, plan.variant, (unsigned)grid);
+        default: return mibc_att_launch_128(s, p, plan.variant, (unsigned)grid);
+    }
+}
+
+extern "C" int mibc_attention(int device, void *stream, const mibc_attention_args *a) {
+    if (a == nullptr) return op_refuse(MIBC_ERR_ARG, "attention: null arguments");
+    if (const int rc = att_check(*a)) return rc;
+    if (a->batch == 0 || a->q_tokens == 0) return MIBC_OK;
+    if (const int rc = att_check_plan(*a, att_plan(*a))) return rc;
+    OpDevice d(device);
+    if (d.rc != hipSuccess) return op_hip(d.rc, "attention: device");
+    return mibc_launch_attention((hipStream_t)stream, *a);
+}

@@ -1,0 +1,502 @@
+// dorado_amd/csrc/ops_attention_kernels.hip — the kernels of mibc_attention for one head size (ATT_D, set by the Makefile).
+#include "ops_attention.h"
+
+#ifndef ATT_D
+#error "compile with -DATT_D=<head size>"
+#endif
+
+typedef bf16_t bf16x8_t __attribute__((ext_vector_type(8)));
+typedef short short4_att __attribute__((ext_vector_type(4)));
+#define LDSP(T) __attribute__((address_space(3))) T *
+typedef __attribute__((address_space(3))) void *att_lds_vptr;
+typedef const __attribute__((address_space(1))) char *att_gptr;
+
+template <typename T>
+struct AttType;
+template <>
+struct AttType<half_t> {
+    typedef half8_t vec8;
+    static constexpr unsigned EXPONENT = 0x7c00, MANTISSA = 0x03ff, ONE = 0x3c00;
+    static __device__ __forceinline__ float16_t mfma32(vec8 a, vec8 b, float16_t c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
+    static __device__ __forceinline__ float4_t mfma16(vec8 a, vec8 b, float4_t c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
+};
+template <>
+struct AttType<bf16_t> {
+    typedef bf16x8_t vec8;
+    static constexpr unsigned EXPONENT = 0x7f80, MANTISSA = 0x007f, ONE = 0x3f80;
+    static __device__ __forceinline__ float16_t mfma32(vec8 a, vec8 b, float16_t c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
+    static __device__ __forceinline__ float4_t mfma16(vec8 a, vec8 b, float4_t c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
+};
+
+__device__ __forceinline__ void att_dma16(att_gptr g, unsigned lds_addr) {
+    __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void *)g, (att_lds_vptr)(size_t)lds_addr, 16, 0, 0);
+}
+template <typename V8>
+__device__ __forceinline__ V8 att_lds16(unsigned addr) {
+    return *(LDSP(const V8))(size_t)addr;
+}
+// 4 rows x 16 columns per 16 lanes: lane l hands in the address of row l / 4, columns 4 (l & 3) .. + 3, and gets column l of the 4 rows
+__device__ __forceinline__ uintx2 att_lds_tr(unsigned addr) {
+    return __builtin_bit_cast(uintx2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((LDSP(short4_att))(size_t)addr));
+}
+__device__ __forceinline__ float att_exp2(float x) { return __builtin_amdgcn_exp2f(x); }
+// over the two half waves
+__device__ __forceinline__ float att_half_max(float x) {
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+__device__ __forceinline__ float att_half_add(float x) {
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+__device__ __forceinline__ int att_wave_min(int x) {
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) x = min(x, __shfl_xor(x, o, 64));
+    return __builtin_amdgcn_readfirstlane(x);
+}
+__device__ __forceinline__ int att_wave_max(int x) { return -att_wave_min(-x); }
+
+// What a row sees: [lo, hi) and, where a prefix does not join on to it, [plo, phi).  An empty interval is [0, 0).
+struct AttRow {
+    int lo, hi, plo, phi, pos;
+};
+__device__ __forceinline__ AttRow att_row(const mibc_attention_args &a, int b, int t) {
+    int64_t k0 = 0, k1, pos;
+    int pre = 0;
+    if (a.doc_offsets != nullptr) {
+        // the last border that is <= t; borders out of order end in some document, whose keys are clamped all the same
+        int first = 0, n = a.n_docs + 1;     // borders [0, first) are <= t
+        while (n > 0) {
+            const int half = n >> 1;
+            if (a.doc_offsets[first + half] <= t) {
+                first += half + 1;
+                n -= half + 1;
+            } else {
+                n = half;
+            }
+        }
+        const int d = first - 1;
+        pos = t;
+        k1 = 0;
+        if (d >= 0 && d < a.n_docs) {
+            k0 = max(a.doc_offsets[d], 0);
+            k1 = min(a.doc_offsets[d + 1], a.k_tokens);
+            if (a.prefix != nullptr) pre = a.prefix[d];
+        }
+    } else {
+        k1 = a.k_len != nullptr ? min(max(a.k_len[b], 0), a.k_tokens) : a.k_tokens;
+        pos = (a.q_start == MIBC_ATTN_END ? k1 - a.q_tokens : (int64_t)a.q_start) + t;
+        if (a.prefix != nullptr) pre = a.prefix[b];
+    }
+    int64_t lo = a.window_back < 0 ? k0 : max(k0, pos - a.window_back);
+    int64_t hi = a.window_ahead < 0 ? k1 : min(k1, pos + a.window_ahead + 1);
+    int64_t ph = min(k1, k0 + max(pre, 0));
+    AttRow r;
+    r.pos = (int)pos;
+    r.lo = r.hi = r.plo = r.phi = 0;
+    if (lo < hi) {
+        if (ph >= lo) {
+            r.lo = (int)(ph > k0 ? k0 : lo);
+            r.hi = (int)max(hi, ph);
+        } else {
+            r.lo = (int)lo;
+            r.hi = (int)hi;
+            if (ph > k0) {
+                r.plo = (int)k0;
+                r.phi = (int)ph;
+            }
+        }
+    } else if (ph > k0) {
+        r.lo = (int)k0;
+        r.hi = (int)ph;
+    }
+    return r;
+}
+#define ATT_FAR 0x7fffffff
+
+// ------------------------------------------------------------------------------------------------------------------
+// Row tiles of 32 NW rows: one wave per 32 rows, all waves over the same tiles of 64 keys in LDS (two stages, filled by direct
+// global -> LDS loads while the tile before is worked on).
+//   S^T[key][row] = K Q^T   on 32x32x16: lane (row = lane & 31, half = lane >> 5) holds keys 8 g + 4 half + 0..3 of each 32
+//   O^T[dim][row] = V^T P^T  takes P^T from those very registers: the 16 k-slots of a step are enumerated as the keys a lane holds,
+//   and V^T comes out of the row-major V tile through transposing LDS reads (ds_read_b64_tr_b16).
+// A row's maximum and sum are one lane pair's: no exchange but one half-wave swap per tile.
+template <int D>
+__device__ __forceinline__ int att_k_slot(int row, int chunk) {   // 16-byte column of the K tile in LDS
+    return D == 128 ? chunk ^ (row & 15) : D == 64 ? chunk ^ ((row >> 1) & 7) : chunk ^ ((row >> 2) & 3);
+}
+template <int D>
+__device__ __forceinline__ int att_v_slot(int row, int chunk) {
+    return D == 128 ? chunk ^ ((row & 3) << 2) : D == 64 ? chunk ^ (((row >> 1) & 1) << 2) : chunk;
+}
+
+template <typename T, int D, int NW, bool GEN>
+__global__ __launch_bounds__(NW * 64, 2) void attention_kernel(AttArgs p) {
+    typedef AttType<T> X;
+    typedef typename X::vec8 vec8;
+    constexpr int NT = NW * 64;
+    constexpr int PITCH = D * 2;
+    constexpr int TILE = 64 * PITCH;
+    constexpr int CH = TILE / 16;               // 16-byte pieces of a tile
+    constexpr int NLD = (CH + NT - 1) / NT;
+    extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
+    __shared__ int range[NW][4];
+    const unsigned lds = (unsigned)(size_t)(LDSP(unsigned char))smem;
+    const mibc_attention_args &a = p.a;
+    const int tid = threadIdx.x, lane = tid & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int half = lane >> 5;
+
+    // workgroup -> (split, tile, pair)
+    unsigned id = blockIdx.x;
+    int pair, tile, split;
+    if (p.order == 0) {
+        pair = id % p.pairs;
+        id /= p.pairs;
+        split = id % p.splits;
+        tile = p.tiles - 1 - (int)(id / p.splits);      // causal: the long tiles start first
+    } else {
+        const int xcd = id & 7;
+        id >>= 3;
+        split = id % p.splits;
+        id /= p.splits;
+        tile = id % p.tiles;
+        pair = (int)(id / p.tiles) * 8 + xcd;
+    }
+    const int b = pair / a.kv_heads, kvh = pair - b * a.kv_heads;
+
+    const int row = tile * (32 * NW) + wave * 32 + (lane & 31);
+    const bool valid = row < p.rows;
+    const int rr = valid ? row : p.rows - 1;
+    const int t = rr / p.group, head = kvh * p.group + (rr - t * p.group);
+    const AttRow see = att_row(a, b, t);
+    const bool some = see.lo < see.hi, apart = see.plo < see.phi;
+    // the wave's rows together: outside [lo_min, hi_max) no row sees a key, inside [lo_max, hi_min) every row sees it
+    const int lo_min = att_wave_min(some ? see.lo : ATT_FAR), hi_max = att_wave_max(some ? see.hi : 0);
+    const int lo_max = att_wave_max(some ? see.lo : ATT_FAR), hi_min = att_wave_min(some ? see.hi : 0);
+    const int plo_min = att_wave_min(apart ? see.plo : ATT_FAR), phi_max = att_wave_max(apart ? see.phi : 0);
+    if (lane == 0) {
+        range[wave][0] = lo_min;
+        range[wave][1] = hi_max;
+        range[wave][2] = plo_min;
+        range[wave][3] = phi_max;
+    }
+    vec8 qf[D / 16];
+    {
+        const T *q = (const T *)a.q + b * a.q_stride[0] + t * a.q_stride[1] + head * a.q_stride[2] + 8 * half;
+#pragma unroll
+        for (int ks = 0; ks < D / 16; ++ks) qf[ks] = *(const vec8 *)(q + 16 * ks);
+    }
+    __syncthreads();
+    int w0 = ATT_FAR, w1 = 0, p0 = ATT_FAR, p1 = 0;
+#pragma unroll
+    for (int i = 0; i < NW; ++i) {
+        w0 = min(w0, range[i][0]);
+        w1 = max(w1, range[i][1]);
+        p0 = min(p0, range[i][2]);
+        p1 = max(p1, range[i][3]);
+    }
+    w0 = __builtin_amdgcn_readfirstlane(w0);
+    w1 = __builtin_amdgcn_readfirstlane(w1);
+    p0 = __builtin_amdgcn_readfirstlane(p0);
+    p1 = __builtin_amdgcn_readfirstlane(p1);
+    // tiles of the prefix, then of the window; one range where their tiles would overlap
+    int np = p0 < p1 ? (p1 - p0 + 63) >> 6 : 0;
+    if (np > 0 && p0 + 64 * np > w0) {
+        w0 = min(w0, p0);
+        w1 = max(w1, p1);
+        np = 0;
+    }
+    const int ntiles = np + (w0 < w1 ? (w1 - w0 + 63) >> 6 : 0);
+    const int it0 = (int)((int64_t)ntiles * split / p.splits), it1 = (int)((int64_t)ntiles * (split + 1) / p.splits);
+
+    // pieces of a tile this thread moves: LDS order is linear in the thread, the swizzle permutes what is fetched
+    const att_gptr kb = (att_gptr)a.k + (b * a.k_stride[0] + kvh * a.k_stride[2]) * 2;
+    const att_gptr vb = (att_gptr)a.v + (b * a.v_stride[0] + kvh * a.v_stride[2]) * 2;
+    const unsigned krow = (unsigned)a.k_stride[1] * 2, vrow = (unsigned)a.v_stride[1] * 2;
+    unsigned koff[NLD], voff[NLD];
+#pragma unroll
+    for (int i = 0; i < NLD; ++i) {
+        const int c = i * NT + tid, r = c / (D / 8), s = c % (D / 8);
+        koff[i] = r * krow + att_k_slot<D>(r, s) * 16;
+        voff[i] = r * vrow + att_v_slot<D>(r, s) * 16;
+    }
+    auto first_key = [&](int it) { return it < np ? p0 + 64 * it : w0 + 64 * (it - np); };
+    auto fetch = [&](int it, int stage) {
+        const int j0 = first_key(it), left = (it < np ? p1 : w1) - j0;
+        const att_gptr kt = kb + (int64_t)j0 * krow, vt = vb + (int64_t)j0 * vrow;
+        const unsigned to = lds + stage * (2 * TILE) + wave * 1024;
+        if (left >= 64) {
+#pragma unroll
+            for (int i = 0; i < NLD; ++i)
+                if (i * NT + wave * 64 < CH) {
+                    att_dma16(kt + koff[i], to + i * (NT * 16));
+                    att_dma16(vt + voff[i], to + i * (NT * 16) + TILE);
+                }
+        } else {   // rows behind the last key repeat it: nobody sees them
+#pragma unroll
+            for (int i = 0; i < NLD; ++i)
+                if (i * NT + wave * 64 < CH) {
+                    const int c = i * NT + tid, r = c / (D / 8), s = c % (D / 8), rc = min(r, left - 1);
+                    att_dma16(kt + (rc * krow + att_k_slot<D>(r, s) * 16), to + i * (NT * 16));
+                    att_dma16(vt + (rc * vrow + att_v_slot<D>(r, s) * 16), to + i * (NT * 16) + TILE);
+                }
+        }
+    };
+
+    // fragment addresses of this lane
+    unsigned kaddr[D / 16], vaddr[D / 32];
+#pragma unroll
+    for (int ks = 0; ks < D / 16; ++ks) kaddr[ks] = lds + (lane & 31) * PITCH + att_k_slot<D>(lane & 31, 2 * ks + half) * 16;
+#pragma unroll
+    for (int db = 0; db < D / 32; ++db) {
+        const int r = 4 * half + ((lane >> 2) & 3);
+        vaddr[db] = lds + TILE + r * PITCH + att_v_slot<D>(r, 4 * db + 2 * ((lane >> 4) & 1) + ((lane >> 1) & 1)) * 16 + (lane & 1) * 8;
+    }
+    const float slope2 = (GEN && a.slopes != nullptr) ? a.slopes[head] * 1.4426950408889634f : 0.0f;
+    const bool cap = GEN && p.cap_out > 0.0f;
+    const float step = GEN ? 1.0f : p.scale2;     // what a score is multiplied with in the exponent
+
+    float16_t o[D / 32];
+    float m, l;
+    auto pass = [&](auto safe_) {
+        constexpr bool SAFE = decltype(safe_)::value;
+#pragma unroll
+        for (int db = 0; db < D / 32; ++db) o[db] = (float16_t)(0.0f);
+        m = -INFINITY;
+        l = 0.0f;
+        if (it0 < it1) fetch(it0, 0);
+        for (int it = it0; it < it1; ++it) {
+            const int stage = (it - it0) & 1;
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+            __builtin_amdgcn_s_barrier();
+            if (it + 1 < it1) fetch(it + 1, stage ^ 1);
+            const int j0 = first_key(it);
+            if ((j0 >= hi_max || j0 + 64 <= lo_min) && (j0 >= phi_max || j0 + 64 <= plo_min)) continue;   // no row of the wave
+            const bool full = !SAFE && j0 >= lo_max && j0 + 64 <= hi_min;
+            const unsigned at = stage * (2 * TILE);
+
+            float16_t s[2];
+            s[0] = (float16_t)(0.0f);
+            s[1] = (float16_t)(0.0f);
+#pragma unroll
+            for (int ks = 0; ks < D / 16; ++ks)
+#pragma unroll
+                for (int i = 0; i < 2; ++i)
+                    s[i] = X::mfma32(att_lds16<vec8>(kaddr[ks] + at + i * (32 * PITCH)), qf[ks], s[i]);
+            if (GEN) {
+#pragma unroll
+                for (int i = 0; i < 2; ++i)
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) {
+                        float x = s[i][r];
+                        if (cap) {   // tanh(y) = 1 - 2 / (1 + e^2y)
+                            x = fmaf(-2.0f * p.cap_out, __builtin_amdgcn_rcpf(1.0f + att_exp2(x * p.cap_in)), p.cap_out);
+                        } else {
+                            x *= p.scale2;
+                        }
+                        const int j = j0 + 32 * i + (r & 3) + 8 * (r >> 2) + 4 * half;
+                        s[i][r] = fmaf(-slope2, fabsf((float)(see.pos - j)), x);
+                    }
+            }
+            unsigned seen = 0xffffffffu;     // bit 16 i + r
+            if (!full) {
+                seen = 0;
+#pragma unroll
+                for (int i = 0; i < 2; ++i)
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) {
+                        const int j = j0 + 32 * i + (r & 3) + 8 * (r >> 2) + 4 * half;
+                        const bool v = (unsigned)(j - see.lo) < (unsigned)(see.hi - see.lo) || (unsigned)(j - see.plo) < (unsigned)(see.phi - see.plo);
+                        s[i][r] = v ? s[i][r] : -INFINITY;
+                        if (SAFE) seen |= v ? 1u << (16 * i + r) : 0u;
+                    }
+            }
+            float top = -INFINITY;
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) top = fmaxf(top, s[i][r]);
+            top = att_half_max(top) * step;
+            // the maximum is only moved when it grew by more than 2^8: probabilities stay below 256, exact in f32 sums
+            if (__any(top > m + 8.0f)) {
+                const float mn = fmaxf(m, top);
+                const float f = m == -INFINITY ? 0.0f : att_exp2(m - mn);
+                m = mn;
+                l *= f;
+#pragma unroll
+                for (int db = 0; db < D / 32; ++db)
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) o[db][r] *= f;
+            }
+            const float base = m == -INFINITY ? 0.0f : m;
+            float add = 0.0f;
+            vec8 pf[4];
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                uintx4 pk[2];
+#pragma unroll
+                for (int r = 0; r < 16; r += 2) {
+                    const float x = att_exp2(fmaf(s[i][r], step, -base)), y = att_exp2(fmaf(s[i][r + 1], step, -base));
+                    add += x + y;
+                    pk[r >> 3][(r & 7) >> 1] = op_pack2(x, y, T());
+                }
+                pf[2 * i] = __builtin_bit_cast(vec8, pk[0]);
+                pf[2 * i + 1] = __builtin_bit_cast(vec8, pk[1]);
+            }
+            l += add;
+#pragma unroll
+            for (int db = 0; db < D / 32; ++db)
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    const uintx2 x = att_lds_tr(vaddr[db] + at + k * (16 * PITCH)), y = att_lds_tr(vaddr[db] + at + k * (16 * PITCH) + 8 * PITCH);
+                    uintx4 v = {x[0], x[1], y[0], y[1]};
+                    if (SAFE) {
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            if ((v[e] & X::EXPONENT) == X::EXPONENT) v[e] &= 0xffff0000u;
+                            if (((v[e] >> 16) & X::EXPONENT) == X::EXPONENT) v[e] &= 0x0000ffffu;
+                        }
+                    }
+                    o[db] = X::mfma32(__builtin_bit_cast(vec8, v), pf[k], o[db]);
+                }
+            if (SAFE) {
+                // values that are not finite reach the rows that see their key, and no other: 0 * NaN stays out of the product
+                // above, and the places of NaN (kind 0), infinity (1) and -infinity (2) are multiplied with the mask instead
+                vec8 vis[4];
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    uintx4 w;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        w[e] = ((seen >> (8 * k + 2 * e)) & 1 ? X::ONE : 0u) | ((seen >> (8 * k + 2 * e + 1)) & 1 ? X::ONE << 16 : 0u);
+                    vis[k] = __builtin_bit_cast(vec8, w);
+                }
+#pragma unroll 1
+                for (int kind = 0; kind < 3; ++kind)
+#pragma unroll
+                    for (int db = 0; db < D / 32; ++db) {
+                        float16_t hit = (float16_t)(0.0f);
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) {
+                            const uintx2 x = att_lds_tr(vaddr[db] + at + k * (16 * PITCH)), y = att_lds_tr(vaddr[db] + at + k * (16 * PITCH) + 8 * PITCH);
+                            uintx4 v = {x[0], x[1], y[0], y[1]};
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) {
+                                unsigned w = 0;
+#pragma unroll
+                                for (int z = 0; z < 2; ++z) {
+                                    const unsigned u = v[e] >> (16 * z);
+                                    const bool odd = (u & X::EXPONENT) == X::EXPONENT;
+                                    const int is = (u & X::MANTISSA) ? 0 : (u & 0x8000u) ? 2 : 1;
+                                    w |= odd && is == kind ? X::ONE << (16 * z) : 0u;
+                                }
+                                v[e] = w;
+                            }
+                            hit = X::mfma32(__builtin_bit_cast(vec8, v), vis[k], hit);
+                        }
+                        const float what = kind == 0 ? NAN : kind == 1 ? INFINITY : -INFINITY;
+#pragma unroll
+                        for (int r = 0; r < 16; ++r)
+                            if (hit[r] > 0.0f) o[db][r] += what;
+                    }
+            }
+        }
+    };
+    pass(std::false_type());
+    bool odd = false;
+#pragma unroll
+    for (int db = 0; db < D / 32; ++db)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) odd = odd || o[db][r] != o[db][r];
+    // a NaN: from a value or key that the row sees, or 0 * (a value that it does not see); the second pass tells them apart
+    if (__syncthreads_or(odd)) pass(std::true_type());
+
+    l = att_half_add(l);
+    const float base = m == -INFINITY ? 0.0f : m;
+    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+    if (!valid) return;
+    if (p.splits > 1) {
+        const int64_t at = ((int64_t)pair * p.rows + row) * p.splits + split;
+        float *po = p.part_o + at * D + 4 * half;
+#pragma unroll
+        for (int db = 0; db < D / 32; ++db)
+#pragma unroll
+            for (int g = 0; g < 4; ++g)
+                *(floatx4 *)(po + 32 * db + 8 * g) = (floatx4){o[db][4 * g] * inv, o[db][4 * g + 1] * inv, o[db][4 * g + 2] * inv, o[db][4 * g + 3] * inv};
+        if (half == 0) p.part_l[at] = l == 0.0f ? -INFINITY : base + log2f(l);
+        return;
+    }
+    T *out = (T *)a.out + b * a.out_stride[0] + t * a.out_stride[1] + head * a.out_stride[2] + 4 * half;
+#pragma unroll
+    for (int db = 0; db < D / 32; ++db)
+#pragma unroll
+        for (int g = 0; g < 4; ++g)
+            *(uintx2 *)(out + 32 * db + 8 * g) = (uintx2){op_pack2(o[db][4 * g] * inv, o[db][4 * g + 1] * inv, T()),
+                                                          op_pack2(o[db][4 * g + 2] * inv, o[db][4 * g + 3] * inv, T())};
+    if (a.lse != nullptr && half == 0)
+        a.lse[((int64_t)b * a.heads + head) * a.q_tokens + t] = l == 0.0f ? -INFINITY : base * 0.6931471805599453f + logf(l);
+}
+
+// ------------------------------------------------------------------------------------------------------------------
+// Joins the parts of a row: one wave per row.
+template <typename T, int D>
+__global__ __launch_bounds__(256) void attention_join_kernel(AttArgs p) {
+    const mibc_attention_args &a = p.a;
+    const int lane = threadIdx.x & 63;
+    const int64_t r = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+    if (r >= (int64_t)p.pairs * p.rows) return;
+    const int pair = (int)(r / p.rows), row = (int)(r - (int64_t)pair * p.rows);
+    const int b = pair / a.kv_heads, kvh = pair - b * a.kv_heads;
+    const int t = row / p.group, head = kvh * p.group + (row - t * p.group);
+    const float *pl = p.part_l + r * p.splits;
+    const float *po = p.part_o + r * p.splits * D;
+    float m = -INFINITY;
+    for (int s = 0; s < p.splits; ++s) m = fmaxf(m, pl[s]);
+    const float base = m == -INFINITY ? 0.0f : m;
+    float sum = 0.0f, y[(D + 63) / 64];
+#pragma unroll
+    for (int i = 0; i < (D + 63) / 64; ++i) y[i] = 0.0f;
+    for (int s = 0; s < p.splits; ++s) {
+        const float w = att_exp2(pl[s] - base);
+        if (w == 0.0f) continue;
+        sum += w;
+#pragma unroll
+        for (int i = 0; i < (D + 63) / 64; ++i)
+            if (lane + 64 * i < D) y[i] = fmaf(w, po[(int64_t)s * D + lane + 64 * i], y[i]);
+    }
+    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+    T *out = (T *)a.out + b * a.out_stride[0] + t * a.out_stride[1] + head * a.out_stride[2];
+#pragma unroll
+    for (int i = 0; i < (D + 63) / 64; ++i)
+        if (lane + 64 * i < D) out[lane + 64 * i] = (T)(y[i] * inv);
+    if (a.lse != nullptr && lane == 0)
+        a.lse[((int64_t)b * a.heads + head) * a.q_tokens + t] = sum == 0.0f ? -INFINITY : base * 0.6931471805599453f + logf(sum);
+}
+
+template <typename T, int NW>
+static void att_rows(hipStream_t s, const AttArgs &p, unsigned grid) {
+    constexpr int LDS = 4 * 64 * ATT_D * 2;
+    if (p.cap_out > 0.0f || p.a.slopes != nullptr) {
+        MIBC_LDS_ATTR_ONCE((attention_kernel<T, ATT_D, NW, true>), LDS);
+        hipLaunchKernelGGL((attention_kernel<T, ATT_D, NW, true>), dim3(grid), dim3(NW * 64), LDS, s, p);
+    } else {
+        MIBC_LDS_ATTR_ONCE((attention_kernel<T, ATT_D, NW, false>), LDS);
+        hipLaunchKernelGGL((attention_kernel<T, ATT_D, NW, false>), dim3(grid), dim3(NW * 64), LDS, s, p);
+    }
+}
+template <typename T>
+static int att_launch(hipStream_t s, const AttArgs &p, int variant, unsigned grid) {
+    if (variant == 0) att_rows<T, 8>(s, p, grid);
+    else if (variant == 1) att_rows<T, 4>(s, p, grid);
+    else att_rows<T, 2>(s, p, grid);
+    int rc = op_hip(hipGetLastError(), "attention");
+    if (rc != MIBC_OK || p.splits == 1) return rc;
+    hipLaunchKernelGGL((attention_join_kernel<T, ATT_D>), dim3((unsigned)(((int64_t)p.pairs * p.rows + 3) / 4)), dim3(256), 0, s, p);
+    return op_hip(hipGetLastError(), "attention");
+}
+#define ATT_CAT2(a, b) a##b
+#define ATT_CAT(a, b) ATT_CAT2(a, b)
+int ATT_CAT(mibc_att_launch_, ATT_D)(hipStream_t s, const AttArgs &p, int variant, unsigned grid) {
+    return p.a.type == MIBC_TYPE_F16 ? att_launch<half_t>(s, p, variant, grid) : att_launch<bf16_t>(s, p, variant, grid);
+}

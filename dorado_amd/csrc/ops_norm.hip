@@ -1,0 +1,272 @@
+// dorado_amd/csrc/ops_norm.hip — mibc_rms_norm: residual addition, RMS norm and an optional 8-bit output in one pass.
+//   h = x + alpha r,   y = h / sqrt(sum h^2 / C + eps) * w,   q = rne(y / s), s = max|y| / 127 | 448
+// A few flops per element against 2-8 bytes: bound by HBM.  So a row is read once, stays in f32 registers (TPR threads hold
+// NCH chunks of 8 consecutive columns each) through both reductions (sum of squares, then max |y| where the output has 8 bits)
+// and leaves once.  Rows of up to 2048 columns take one wave (or a quarter of one) and reduce by lane shuffles alone; wider ones
+// take a workgroup and one LDS exchange per reduction.
+#include "ops.h"
+
+struct NormArgs {
+    mibc_rms_norm_args a;
+};
+
+template <typename T, bool VEC>
+__device__ __forceinline__ void norm_load(const T *row, int col, int cols, float v[8]) {
+    if (VEC) {
+        op_load8(row + col, v);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = (col + i < cols) ? (float)row[col + i] : 0.0f;
+    }
+}
+template <typename T, bool VEC>
+__device__ __forceinline__ void norm_store(T *row, int col, int cols, const float v[8]) {
+    if (VEC) {
+        op_store8<T>(row + col, v);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            if (col + i < cols) row[col + i] = (T)v[i];
+    }
+}
+
+__device__ __forceinline__ float op_add(float a, float b) { return a + b; }
+__device__ __forceinline__ float op_max(float a, float b) { return fmaxf(a, b); }
+// over the TPR threads that hold a row; `red`: one slot per wave
+template <int TPR, bool MAX>
+__device__ __forceinline__ float norm_reduce(float v, float *red) {
+#pragma unroll
+    for (int o = (TPR < 64 ? TPR : 64) / 2; o > 0; o >>= 1) {
+        const float w = __shfl_xor(v, o, 64);
+        v = MAX ? op_max(v, w) : op_add(v, w);
+    }
+    if (TPR > 64) {
+        const int wave = threadIdx.x >> 6;
+        if ((threadIdx.x & 63) == 0) red[wave] = v;
+        __syncthreads();
+        v = red[0];
+#pragma unroll
+        for (int i = 1; i < TPR / 64; ++i) v = MAX ? op_max(v, red[i]) : op_add(v, red[i]);
+    }
+    return v;
+}
+
+template <typename T, int TPR, int NCH, bool VEC>
+__global__ __launch_bounds__(TPR > 256 ? TPR : 256) void rms_norm_kernel(NormArgs n) {
+    constexpr int NT = TPR > 256 ? TPR : 256;
+    __shared__ float red[2][NT / 64];
+    const mibc_rms_norm_args &a = n.a;
+    const int lane = threadIdx.x % TPR;
+    const int64_t row = (int64_t)blockIdx.x * (NT / TPR) + threadIdx.x / TPR;
+    if (TPR <= 64 && row >= a.rows) return;     // whole rows of lanes; TPR >= 256: one row per workgroup, the grid is exact
+    const int cols = a.cols;
+    const T *x = (const T *)a.x + row * a.x_stride;
+    const T *r = (const T *)a.residual + row * a.residual_stride;
+    float h[NCH][8];
+    float ss = 0.0f;
+#pragma unroll
+    for (int i = 0; i < NCH; ++i) {
+        const int col = (lane + i * TPR) * 8;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) h[i][e] = 0.0f;
+        if (col < cols) norm_load<T, VEC>(x, col, cols, h[i]);
+    }
+    if (a.residual != nullptr) {
+#pragma unroll
+        for (int i = 0; i < NCH; ++i) {
+            const int col = (lane + i * TPR) * 8;
+            if (col < cols) {
+                float v[8];
+                norm_load<T, VEC>(r, col, cols, v);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) h[i][e] = fmaf(a.alpha, v[e], h[i][e]);
+            }
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < NCH; ++i)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) ss = fmaf(h[i][e], h[i][e], ss);
+    if (a.sum_out != nullptr) {
+        T *o = (T *)a.sum_out + row * a.sum_stride;
+#pragma unroll
+        for (int i = 0; i < NCH; ++i) {
+            const int col = (lane + i * TPR) * 8;
+            if (col < cols) norm_store<T, VEC>(o, col, cols, h[i]);
+        }
+    }
+    ss = norm_reduce<TPR, false>(ss, red[0]);
+    const float rstd = 1.0f / sqrtf(ss / (float)cols + a.eps);
+    // y replaces h
+#pragma unroll
+    for (int i = 0; i < NCH; ++i) {
+        const int col = (lane + i * TPR) * 8;
+        float w[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) w[e] = 1.0f;
+        if (a.weight != nullptr && col < cols) {
+            if (a.weight_type == MIBC_TYPE_F32)
+                norm_load<float, VEC>((const float *)a.weight, col, cols, w);
+            else
+                norm_load<T, VEC>((const T *)a.weight, col, cols, w);
+        }
+#pragma unroll
+        for (int e = 0; e < 8; ++e) h[i][e] = h[i][e] * rstd * w[e];
+    }
+    if (a.out_type == a.type) {
+        T *o = (T *)a.out + row * a.out_stride;
+#pragma unroll
+        for (int i = 0; i < NCH; ++i) {
+            const int col = (lane + i * TPR) * 8;
+            if (col < cols) norm_store<T, VEC>(o, col, cols, h[i]);
+        }
+        return;
+    }
+    // 8-bit output.  A value that is not finite makes the group's maximum infinite, and its scale NaN.
+    float top[NCH];
+    float all = 0.0f;
+#pragma unroll
+    for (int i = 0; i < NCH; ++i) {
+        top[i] = 0.0f;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const float m = fabsf(h[i][e]);
+            top[i] = fmaxf(top[i], m <= 3.402823466e38f ? m : INFINITY);   // columns behind the row hold zeros
+        }
+        all = fmaxf(all, top[i]);
+    }
+    const float most = a.out_type == MIBC_TYPE_I8 ? 127.0f : 448.0f;
+    if (a.group == 0) {
+        all = norm_reduce<TPR, true>(all, red[1]);
+#pragma unroll
+        for (int i = 0; i < NCH; ++i) top[i] = all;
+    } else {   // a group is group / 8 = 4, 8 or 16 neighbouring lanes of one chunk index
+#pragma unroll
+        for (int i = 0; i < NCH; ++i)
+#pragma unroll
+            for (int o = 1; o < 16; o <<= 1) {
+                const float w = __shfl_xor(top[i], o, 64);
+                top[i] = (o * 8 < a.group) ? fmaxf(top[i], w) : top[i];
+            }
+    }
+    uint8_t *o = (uint8_t *)a.out + row * a.out_stride;
+    float *sc = a.scale_out + row * a.scale_stride;
+#pragma unroll
+    for (int i = 0; i < NCH; ++i) {
+        const int chunk = lane + i * TPR, col = chunk * 8;
+        if (col >= cols) continue;
+        const bool fine = top[i] < INFINITY;
+        const float s = top[i] == 0.0f ? 1.0f : fine ? top[i] / most : NAN;
+        // the reciprocal of a subnormal scale overflows: such a group divides instead
+        const float inv = 1.0f / s;
+        const bool tiny = s < 1.2e-38f;
+        unsigned lo = 0, hi = 0;
+        if (fine) {
+            float v[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[e] = tiny ? h[i][e] / s : h[i][e] * inv;
+            if (a.out_type == MIBC_TYPE_I8) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    lo |= ((unsigned)(int)rintf(fminf(fmaxf(v[e], -127.0f), 127.0f)) & 0xffu) << (8 * e);
+                    hi |= ((unsigned)(int)rintf(fminf(fmaxf(v[4 + e], -127.0f), 127.0f)) & 0xffu) << (8 * e);
+                }
+            } else {   // |v| <= 448 (1 + 2^-22): rounds to 448, below the conversion's NaN range (> 464)
+                lo = __builtin_amdgcn_cvt_pk_fp8_f32(v[0], v[1], lo, false);
+                lo = __builtin_amdgcn_cvt_pk_fp8_f32(v[2], v[3], lo, true);
+                hi = __builtin_amdgcn_cvt_pk_fp8_f32(v[4], v[5], hi, false);
+                hi = __builtin_amdgcn_cvt_pk_fp8_f32(v[6], v[7], hi, true);
+            }
+        }
+        if (VEC) {
+            *(uintx2 *)(o + col) = (uintx2){lo, hi};
+        } else {
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+                if (col + e < cols) o[col + e] = (uint8_t)((e < 4 ? lo : hi) >> (8 * (e & 3)));
+        }
+        if (a.group == 0 ? chunk == 0 : col % a.group == 0) sc[a.group == 0 ? 0 : col / a.group] = s;
+    }
+}
+
+template <typename T, bool VEC>
+static void norm_launch(hipStream_t s, const NormArgs &n) {
+    const int chunks = (n.a.cols + 7) / 8;
+    const int64_t rows = n.a.rows;
+#define NORM_GO(TPR, NCH, NT) \
+    hipLaunchKernelGGL((rms_norm_kernel<T, TPR, NCH, VEC>), dim3((unsigned)((rows + NT / TPR - 1) / (NT / TPR))), dim3(NT), 0, s, n)
+    if (chunks <= 16) NORM_GO(16, 1, 256);
+    else if (chunks <= 64) NORM_GO(64, 1, 256);
+    else if (chunks <= 128) NORM_GO(64, 2, 256);
+    else if (chunks <= 256) NORM_GO(64, 4, 256);
+    else if (chunks <= 512) NORM_GO(256, 2, 256);
+    else if (chunks <= 1024) NORM_GO(256, 4, 256);
+    else NORM_GO(1024, 4, 1024);
+#undef NORM_GO
+}
+
+static int norm_check(const mibc_rms_norm_args &a, bool *vec) {
+    if (a.type != MIBC_TYPE_F16 && a.type != MIBC_TYPE_BF16 && a.type != MIBC_TYPE_F32)
+        return op_refuse(MIBC_NOT_SUPPORTED, "rms_norm: type must be f16, bf16 or f32");
+    if (a.rows < 0 || a.cols < 1) return op_refuse(MIBC_ERR_ARG, "rms_norm: rows >= 0 and cols >= 1");
+    if (a.cols > 32768) return op_refuse(MIBC_NOT_SUPPORTED, "rms_norm: at most 32768 columns");
+    if (a.rows > (int64_t)0x7fffffff) return op_refuse(MIBC_NOT_SUPPORTED, "rms_norm: at most 2^31 - 1 rows");
+    if (a.weight != nullptr && a.weight_type != MIBC_TYPE_F32 && a.weight_type != a.type)
+        return op_refuse(MIBC_NOT_SUPPORTED, "rms_norm: weight must be f32 or of the input's type");
+    const bool quant = a.out_type == MIBC_TYPE_I8 || a.out_type == MIBC_TYPE_E4M3;
+    if (!quant && a.out_type != a.type) return op_refuse(MIBC_NOT_SUPPORTED, "rms_norm: output is of the input's type, int8 or e4m3");
+    if (quant) {
+        if (a.group != 0 && a.group != 32 && a.group != 64 && a.group != 128)
+            return op_refuse(MIBC_NOT_SUPPORTED, "rms_norm: group must be 0 (a row), 32, 64 or 128");
+        if (a.group != 0 && a.cols % a.group != 0) return op_refuse(MIBC_ERR_ARG, "rms_norm: cols must be a multiple of group");
+    } else if (a.group != 0) {
+        return op_refuse(MIBC_ERR_ARG, "rms_norm: group needs an 8-bit output");
+    }
+    if (!(a.eps >= 0.0f)) return op_refuse(MIBC_ERR_ARG, "rms_norm: eps must not be negative");
+    if (a.reserved != 0) return op_refuse(MIBC_ERR_ARG, "rms_norm: reserved must be 0");
+    if (a.rows == 0) return MIBC_OK;
+    if (a.x == nullptr || a.out == nullptr || (quant && a.scale_out == nullptr))
+        return op_refuse(MIBC_ERR_ARG, "rms_norm: null pointer");
+    const int ngroups = a.group == 0 ? 1 : a.cols / a.group;
+    if (a.rows > 1 && (a.out_stride < a.cols || (a.sum_out != nullptr && a.sum_stride < a.cols) || (quant && a.scale_stride < ngroups)))
+        return op_refuse(MIBC_ERR_ARG, "rms_norm: output rows overlap");
+    if (a.x_stride < 0 || a.residual_stride < 0) return op_refuse(MIBC_ERR_ARG, "rms_norm: negative stride");
+    const unsigned eb = (unsigned)op_type_bytes(a.type);
+    if (!op_aligned(a.x, eb) || !op_aligned(a.residual, eb) || !op_aligned(a.sum_out, eb) || !op_aligned(a.weight, (unsigned)op_type_bytes(a.weight_type)) ||
+        !op_aligned(a.out, (unsigned)op_type_bytes(a.out_type)) || !op_aligned(a.scale_out, 4))
+        return op_refuse(MIBC_ERR_ARG, "rms_norm: pointer not aligned to its type");
+    // 16-byte accesses where every row of every tensor allows them, single elements elsewhere
+    *vec = a.cols % 8 == 0 && op_aligned(a.x, 16) && a.x_stride % 8 == 0 && op_aligned(a.weight, 16) &&
+           (a.residual == nullptr || (op_aligned(a.residual, 16) && a.residual_stride % 8 == 0)) &&
+           (a.sum_out == nullptr || (op_aligned(a.sum_out, 16) && a.sum_stride % 8 == 0)) &&
+           op_aligned(a.out, quant ? 8 : 16) && a.out_stride % 8 == 0;
+    return MIBC_OK;
+}
+
+// launch on a stream of the current device (the engine's own path); checks included
+int mibc_launch_rms_norm(hipStream_t s, const mibc_rms_norm_args &a) {
+    bool vec = false;
+    if (const int rc = norm_check(a, &vec)) return rc;
+    if (a.rows == 0) return MIBC_OK;
+    const NormArgs n{a};
+#define NORM_T(T)                              \
+    do {                                       \
+        if (vec) norm_launch<T, true>(s, n);   \
+        else norm_launch<T, false>(s, n);      \
+    } while (0)
+    if (a.type == MIBC_TYPE_F16) NORM_T(half_t);
+    else if (a.type == MIBC_TYPE_BF16) NORM_T(bf16_t);
+    else NORM_T(float);
+#undef NORM_T
+    return op_hip(hipGetLastError(), "rms_norm");
+}
+
+extern "C" int mibc_rms_norm(int device, void *stream, const mibc_rms_norm_args *a) {
+    if (a == nullptr) return op_refuse(MIBC_ERR_ARG, "rms_norm: null arguments");
+    bool vec;
+    if (const int rc = norm_check(*a, &vec)) return rc;
+    if (a->rows == 0) return MIBC_OK;
+    OpDevice d(device);
+    if (d.rc != hipSuccess) return op_hip(d.rc, "rms_norm: device");
+    return mibc_launch_rms_norm((hipStream_t)stream, *a);
+}

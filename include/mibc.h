@@ -234,6 +234,95 @@ MIBC_API int mibc_call_var_async(mibc_engine *e, int slot, const void *in_host, 
 MIBC_API int mibc_svb16_decode(mibc_engine *e, const uint8_t *streams_dev, const int64_t *stream_off_dev,
                       const int64_t *sample_off_dev, int n_rows, int16_t *out_dev, int *status_dev);
 
+/* ---- operators of transformer layers (no engine, no model) ----
+ * The non-GEMM operators of a transformer layer for any width, head size and mask: what the engine's own transformer path has
+ * fused for one shape family (nn/TxModules.cpp:184-250 rotary, :279-426 attention, :859-906 layer; nn/RMSNorm.cpp:14-18), as
+ * entry points of their own.  All pointers are device pointers of `device`; work is issued on `stream` (a hipStream_t of that
+ * device, NULL = its null stream) and the call returns before it completes (async).  No call allocates, copies to the host,
+ * synchronises or keeps anything for the next one, so all of them can be captured into a graph; the caller's current device is
+ * left as it was.  Refusals are decided from the arguments alone, before anything is launched (text: mibc_last_error(NULL)).
+ * Strides count elements; the innermost dimension is contiguous.  A stride may be 0 on inputs (a broadcast dimension), never
+ * on outputs.  An output may be the input of the same shape and strides (in place); other overlaps are not checked. */
+#define MIBC_TYPE_F16 0
+#define MIBC_TYPE_BF16 1
+#define MIBC_TYPE_F32 2
+#define MIBC_TYPE_I8 3
+#define MIBC_TYPE_E4M3 4 /* OCP e4m3 (no infinity, largest value 448) */
+
+/* h = x + alpha * residual;  y = h / sqrt(mean(h^2) + eps) * weight  over the last dimension, computed in f32, h not rounded
+ * in between.  sum_out (optional) receives h, out receives y, both in `type`; or, out_type I8 / E4M3, out receives
+ * round(y / s) with s = max|y| / 127 (I8) or / 448 (E4M3) over the row (group 0) or over each group of 32, 64 or 128 columns,
+ * and scale_out [rows][cols / group] receives s.  Where max|y| is 0, s = 1; where a value of the group is not finite, s = NaN
+ * and the group's codes are 0.  weight: f32 or `type`, NULL = ones; residual NULL = none.  1 <= cols <= 32768. */
+typedef struct mibc_rms_norm_args {
+    const void *x, *residual, *weight;
+    void *sum_out, *out;
+    float *scale_out;
+    int64_t rows;
+    int64_t x_stride, residual_stride, sum_stride, out_stride, scale_stride; /* elements from row to row */
+    int32_t cols, type, weight_type, out_type, group;
+    float alpha, eps;
+    int32_t reserved; /* 0 */
+} mibc_rms_norm_args;
+MIBC_API int mibc_rms_norm(int device, void *stream, const mibc_rms_norm_args *a);
+
+/* Rotary positions of up to two tensors [batch][tokens][heads][head_dim] (queries and keys) in one launch.  Pair i of the first
+ * rot_dim columns of a head at position p turns by p * freqs[i]:  (a, b) -> amplitude * (a cos - b sin, a sin + b cos); pairs
+ * are columns (i, i + rot_dim / 2), or (2 i, 2 i + 1) if `interleaved`.  The other columns are copied.  Position of token t of
+ * row n: positions[n][t] (contiguous int32 or int64; may be negative, which turns back), or start + t where positions is NULL.
+ * freqs: f64 device [rot_dim / 2], radians per position (mibc_rope_frequencies).  Angles are reduced in f64. */
+typedef struct mibc_rope_args {
+    const void *x[2];  /* x[1] may be NULL */
+    void *out[2];
+    const void *positions; /* or NULL */
+    const double *freqs;
+    int64_t start;
+    int64_t x_stride[2][3], out_stride[2][3]; /* batch, token, head */
+    int64_t batch, tokens;
+    int32_t heads[2];
+    int32_t head_dim, rot_dim, type, interleaved, positions_64;
+    float amplitude;
+} mibc_rope_args;
+MIBC_API int mibc_rope(int device, void *stream, const mibc_rope_args *a);
+#define MIBC_ROPE_PLAIN 0    /* theta^(-2i / rot_dim) */
+#define MIBC_ROPE_LINEAR 1   /* ... / factor: positions squeezed into the trained length */
+#define MIBC_ROPE_BASE 2     /* theta * factor^(rot_dim / (rot_dim - 2)) as the base: the slowest pair slows by factor, the fastest stays */
+#define MIBC_ROPE_BY_PARTS 3 /* pairs with >= turns_high turns over original_length stay, with <= turns_low are / factor, a ramp between */
+/* Host only: the frequencies mibc_rope takes, freqs [rot_dim / 2] on the HOST. */
+MIBC_API int mibc_rope_frequencies(int scaling, int rot_dim, double theta, double factor, double original_length, double turns_low,
+                          double turns_high, double *freqs);
+
+/* out = softmax(scores) v per head, scores = scale * (q . k), then cap * tanh(scores / cap) if softcap > 0, then
+ * - slopes[head] * |i - j| if slopes (i, j: positions of query and key), over the keys a query sees.  q, out:
+ * [batch][q_tokens][heads][head_dim]; k, v: [batch][k_tokens][kv_heads][head_dim], heads a multiple of kv_heads, query head h
+ * reading key head h / (heads / kv_heads).  Row n has len = k_len[n] keys (NULL: k_tokens; clamped to [0, k_tokens]); query t
+ * stands at position i = q_start + t (q_start == MIBC_ATTN_END: len - q_tokens + t, the last query on the last key).  It sees
+ * key j < len if i - window_back <= j <= i + window_ahead (a negative limit: unlimited; window_ahead = 0: causal) or if
+ * j < prefix[n].  doc_offsets [n_docs + 1] (needs batch 1, q_tokens == k_tokens, no k_len, q_start MIBC_ATTN_END; ascending):
+ * document d is the tokens [doc_offsets[d], doc_offsets[d + 1]); a token sees its own document only, prefix is then [n_docs] and
+ * counts from the document's start, tokens in no document see nothing and are seen by none.  A query that sees nothing, or only
+ * scores of -infinity, gives zeros and lse = -infinity.  What a query does not see has no influence on its result, whatever it
+ * holds (NaN and infinity included).  lse (optional) [batch][heads][q_tokens] f32 contiguous: log of the sum of exp(scores).
+ * Types F16, BF16; head_dim 32, 64, 96 or 128; token and head strides multiples of 8 elements, pointers aligned to 16 bytes.
+ * workspace: mibc_attention_workspace(a) bytes on the device (0: may be NULL), the call's own until it has completed. */
+#define MIBC_ATTN_END (-2147483647 - 1)
+typedef struct mibc_attention_args {
+    const void *q, *k, *v;
+    void *out;
+    float *lse;
+    const int32_t *k_len, *prefix, *doc_offsets;
+    const float *slopes;
+    void *workspace;
+    uint64_t workspace_bytes;
+    int64_t q_stride[3], k_stride[3], v_stride[3], out_stride[3]; /* batch, token, head */
+    int32_t batch, heads, kv_heads, q_tokens, k_tokens, head_dim, n_docs, type;
+    int32_t window_back, window_ahead, q_start;
+    float scale, softcap;
+    int32_t reserved; /* 0 */
+} mibc_attention_args;
+MIBC_API int mibc_attention(int device, void *stream, const mibc_attention_args *a);
+MIBC_API uint64_t mibc_attention_workspace(const mibc_attention_args *a);
+
 /* ---- measurement (replaces CudaCaller.cpp:552-569 timing + gpu_profiling.h ranges) ---- */
 MIBC_API int mibc_time_forward(mibc_engine *e, int N, int T_in, float *ms); /* min of 2 runs, like :552-569 */
 MIBC_API int mibc_get_stage_ms(mibc_engine *e, mibc_stage_ms *out);         /* hipEvent times, last call */
