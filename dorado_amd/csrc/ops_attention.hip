@@ -50,18 +50,21 @@ struct AttPlan {
 static AttPlan att_plan(const mibc_attention_args &a) {
     const int64_t rows = (int64_t)a.q_tokens * (a.heads / a.kv_heads), pairs = (int64_t)a.batch * a.kv_heads;
     AttPlan p;
-    p.variant = rows > 128 ? 0 : rows > 64 ? 1 : 2;
-    const int tile = p.variant == 0 ? 256 : p.variant == 1 ? 128 : 64;
+    p.variant = rows <= 16 ? 3 : rows > 128 ? 0 : rows > 64 ? 1 : 2;
+    const int tile = p.variant == 0 ? 256 : p.variant == 1 ? 128 : p.variant == 2 ? 64 : 16;
     p.tiles = (int)((rows + tile - 1) / tile);
-    // keys a row can see at most, in tiles of 64
+    // keys a row can see at most
     int64_t keys = a.k_tokens;
     if (a.window_back >= 0 && a.window_ahead >= 0 && a.prefix == nullptr) {
         const int64_t w = (int64_t)a.window_back + a.window_ahead + 1 + tile;
         keys = keys < w ? keys : w;
     }
-    const int64_t ktiles = (keys + 63) / 64, groups = p.tiles * pairs;
-    int64_t splits = groups >= 512 ? 1 : 512 / groups;
-    if (splits > ktiles / 4) splits = ktiles / 4;     // a part is worth its share of the join from four tiles on
+    const int64_t groups = p.tiles * pairs;
+    // tiles: two workgroups per CU, a part is worth its share of the join from four tiles of 64 keys on;
+    // tokens: eight per CU (rows of a batch differ in length), from four steps of 32 keys for each of the four waves on
+    const int64_t want = p.variant == 3 ? 2048 : 512, least = p.variant == 3 ? 512 : 256;
+    int64_t splits = groups >= want ? 1 : want / groups;
+    if (splits > keys / least) splits = keys / least;
     p.splits = splits < 1 ? 1 : (int)splits;
     return p;
 }

@@ -28,8 +28,11 @@ struct AttType<bf16_t> {
     static __device__ __forceinline__ float4_t mfma16(vec8 a, vec8 b, float4_t c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
 };
 
-__device__ __forceinline__ void att_dma16(att_gptr g, unsigned lds_addr) {
-    __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void *)g, (att_lds_vptr)(size_t)lds_addr, 16, 0, 0);
+// 16 bytes per lane from base + offset straight to LDS at `lds_addr` + 16 * lane (one wait state between M0 and its use).  Written
+// as assembly, because the compiler waits for every LDS load of its own before any LDS read, and the next tile's are meant to
+// stay in flight: the kernels wait for them by vmcnt.  The load writes no register.
+__device__ __forceinline__ void att_dma16(att_gptr base, unsigned offset, unsigned lds_addr) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(lds_addr), "v"(offset), "s"(base) : "memory");
 }
 template <typename V8>
 __device__ __forceinline__ V8 att_lds16(unsigned addr) {
@@ -113,6 +116,25 @@ __device__ __forceinline__ AttRow att_row(const mibc_attention_args &a, int b, i
     return r;
 }
 #define ATT_FAR 0x7fffffff
+
+// 1 where a value is NaN (kind 0), infinity (1), -infinity (2), else 0
+template <typename T>
+__device__ __forceinline__ uintx4 att_places(uintx4 v, int kind) {
+    typedef AttType<T> X;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        unsigned w = 0;
+#pragma unroll
+        for (int z = 0; z < 2; ++z) {
+            const unsigned x = v[e] >> (16 * z);
+            const bool odd = (x & X::EXPONENT) == X::EXPONENT;
+            const int is = (x & X::MANTISSA) ? 0 : (x & 0x8000u) ? 2 : 1;
+            w |= odd && is == kind ? X::ONE << (16 * z) : 0u;
+        }
+        v[e] = w;
+    }
+    return v;
+}
 
 // ------------------------------------------------------------------------------------------------------------------
 // Row tiles of 32 NW rows: one wave per 32 rows, all waves over the same tiles of 64 keys in LDS (two stages, filled by direct
@@ -230,16 +252,16 @@ __global__ __launch_bounds__(NW * 64, 2) void attention_kernel(AttArgs p) {
 #pragma unroll
             for (int i = 0; i < NLD; ++i)
                 if (i * NT + wave * 64 < CH) {
-                    att_dma16(kt + koff[i], to + i * (NT * 16));
-                    att_dma16(vt + voff[i], to + i * (NT * 16) + TILE);
+                    att_dma16(kt, koff[i], to + i * (NT * 16));
+                    att_dma16(vt, voff[i], to + i * (NT * 16) + TILE);
                 }
         } else {   // rows behind the last key repeat it: nobody sees them
 #pragma unroll
             for (int i = 0; i < NLD; ++i)
                 if (i * NT + wave * 64 < CH) {
                     const int c = i * NT + tid, r = c / (D / 8), s = c % (D / 8), rc = min(r, left - 1);
-                    att_dma16(kt + (rc * krow + att_k_slot<D>(r, s) * 16), to + i * (NT * 16));
-                    att_dma16(vt + (rc * vrow + att_v_slot<D>(r, s) * 16), to + i * (NT * 16) + TILE);
+                    att_dma16(kt, rc * krow + att_k_slot<D>(r, s) * 16, to + i * (NT * 16));
+                    att_dma16(vt, rc * vrow + att_v_slot<D>(r, s) * 16, to + i * (NT * 16) + TILE);
                 }
         }
     };
@@ -380,20 +402,8 @@ __global__ __launch_bounds__(NW * 64, 2) void attention_kernel(AttArgs p) {
 #pragma unroll
                         for (int k = 0; k < 4; ++k) {
                             const uintx2 x = att_lds_tr(vaddr[db] + at + k * (16 * PITCH)), y = att_lds_tr(vaddr[db] + at + k * (16 * PITCH) + 8 * PITCH);
-                            uintx4 v = {x[0], x[1], y[0], y[1]};
-#pragma unroll
-                            for (int e = 0; e < 4; ++e) {
-                                unsigned w = 0;
-#pragma unroll
-                                for (int z = 0; z < 2; ++z) {
-                                    const unsigned u = v[e] >> (16 * z);
-                                    const bool odd = (u & X::EXPONENT) == X::EXPONENT;
-                                    const int is = (u & X::MANTISSA) ? 0 : (u & 0x8000u) ? 2 : 1;
-                                    w |= odd && is == kind ? X::ONE << (16 * z) : 0u;
-                                }
-                                v[e] = w;
-                            }
-                            hit = X::mfma32(__builtin_bit_cast(vec8, v), vis[k], hit);
+                            const uintx4 v = {x[0], x[1], y[0], y[1]};
+                            hit = X::mfma32(__builtin_bit_cast(vec8, att_places<T>(v, kind)), vis[k], hit);
                         }
                         const float what = kind == 0 ? NAN : kind == 1 ? INFINITY : -INFINITY;
 #pragma unroll
@@ -439,39 +449,299 @@ __global__ __launch_bounds__(NW * 64, 2) void attention_kernel(AttArgs p) {
 }
 
 // ------------------------------------------------------------------------------------------------------------------
-// Joins the parts of a row: one wave per row.
+// At most 16 rows per (batch, key head) pair: single tokens and short runs of them over long caches.  Bound by reading K and V
+// once, so nothing is shared between waves and nothing waits for a barrier: each of the four waves walks its own steps of 32 keys
+// (wave w the steps w, w + 4, ...), K straight into matrix operands, V through two private LDS stages (transposing reads).  The
+// next step's loads leave as soon as the scores have used up the K operands: 16 KB of a wave are in flight all the time but for
+// the few hundred cycles of its score instructions, 128 KB per CU.  16x16x32 instructions: S^T[key][row], lane (row = lane & 15,
+// quarter = lane >> 4) holds keys 4 quarter + 0..3 of each 16, which are its k-slots in O^T[dim][row] = V^T P^T.  Matrix work is
+// free here, so P goes in as two 16-bit parts (value and remainder): the result is rounded once, at the end.
+template <int D>
+__device__ __forceinline__ int att_v_slot16(int row, int chunk) {
+    return D == 128 ? chunk ^ (((row & 3) << 2) | ((row & 4) >> 1)) : D == 64 ? chunk ^ ((((row >> 1) & 1) << 2) | ((row & 4) >> 1)) : chunk;
+}
+
+template <typename T, int D, bool GEN>
+__global__ __launch_bounds__(256, 2) void attention_token_kernel(AttArgs p) {
+    typedef AttType<T> X;
+    typedef typename X::vec8 vec8;
+    constexpr int PITCH = D * 2;
+    constexpr int STAGE = 32 * PITCH;
+    constexpr int NV = STAGE / 1024;            // LDS loads of a step
+    constexpr int NK = D / 32;                  // K operand pieces of 16 keys
+    extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
+    const unsigned lds = (unsigned)(size_t)(LDSP(unsigned char))smem;
+    const mibc_attention_args &a = p.a;
+    const int tid = threadIdx.x, lane = tid & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int l15 = lane & 15, quarter = lane >> 4;
+    const int pair = blockIdx.x % p.pairs, split = blockIdx.x / p.pairs;
+    const int b = pair / a.kv_heads, kvh = pair - b * a.kv_heads;
+
+    const int rr = min(l15, p.rows - 1);
+    const int t = rr / p.group, head = kvh * p.group + (rr - t * p.group);
+    const AttRow see = att_row(a, b, t);
+    const bool some = see.lo < see.hi, apart = see.plo < see.phi;
+    int w0 = att_wave_min(some ? see.lo : ATT_FAR), w1 = att_wave_max(some ? see.hi : 0);
+    const int lo_max = att_wave_max(some ? see.lo : ATT_FAR), hi_min = att_wave_min(some ? see.hi : 0);
+    const int p0 = att_wave_min(apart ? see.plo : ATT_FAR), p1 = att_wave_max(apart ? see.phi : 0);
+    int np = p0 < p1 ? (p1 - p0 + 31) >> 5 : 0;
+    if (np > 0 && p0 + 32 * np > w0) {
+        w0 = min(w0, p0);
+        w1 = max(w1, p1);
+        np = 0;
+    }
+    const int steps = np + (w0 < w1 ? (w1 - w0 + 31) >> 5 : 0);
+    const int it0 = (int)((int64_t)steps * split / p.splits) + wave, it1 = (int)((int64_t)steps * (split + 1) / p.splits);
+
+    vec8 qf[NK];
+    {
+        const T *q = (const T *)a.q + b * a.q_stride[0] + t * a.q_stride[1] + head * a.q_stride[2] + 8 * quarter;
+#pragma unroll
+        for (int kb = 0; kb < NK; ++kb) qf[kb] = *(const vec8 *)(q + 32 * kb);
+    }
+    const att_gptr kb0 = (att_gptr)a.k + (b * a.k_stride[0] + kvh * a.k_stride[2]) * 2;
+    const att_gptr vb0 = (att_gptr)a.v + (b * a.v_stride[0] + kvh * a.v_stride[2]) * 2;
+    const unsigned krow = (unsigned)a.k_stride[1] * 2, vrow = (unsigned)a.v_stride[1] * 2;
+    const unsigned mine = lds + wave * (2 * STAGE);
+    auto first_key = [&](int it) { return it < np ? p0 + 32 * it : w0 + 32 * (it - np); };
+    auto fetch = [&](int it, vec8 (&kf)[2][NK], int stage) {
+        const int j0 = first_key(it), last = min(32, (it < np ? p1 : w1) - j0) - 1;    // rows behind the last key repeat it
+        const att_gptr kt = kb0 + (int64_t)j0 * krow, vt = vb0 + (int64_t)j0 * vrow;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const unsigned at = min(16 * i + l15, last) * krow + 16 * quarter;
+#pragma unroll
+            for (int kb = 0; kb < NK; ++kb) kf[i][kb] = *(const __attribute__((address_space(1))) vec8 *)(kt + (at + 64 * kb));
+        }
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const int c = i * 64 + lane, r = c / (D / 8), s = c % (D / 8);
+            att_dma16(vt, min(r, last) * vrow + att_v_slot16<D>(r, s) * 16, mine + stage * STAGE + i * 1024);
+        }
+    };
+    unsigned vaddr[D / 16];
+#pragma unroll
+    for (int db = 0; db < D / 16; ++db) {
+        const int r = 4 * quarter + (l15 >> 2);
+        vaddr[db] = mine + r * PITCH + att_v_slot16<D>(r, 2 * db + ((lane >> 1) & 1)) * 16 + (lane & 1) * 8;
+    }
+    const float slope2 = (GEN && a.slopes != nullptr) ? a.slopes[head] * 1.4426950408889634f : 0.0f;
+    const bool cap = GEN && p.cap_out > 0.0f;
+    const float step = GEN ? 1.0f : p.scale2;
+
+    float4_t o[D / 16];
+    float m, l;
+    auto pass = [&](auto safe_) {
+        constexpr bool SAFE = decltype(safe_)::value;
+#pragma unroll
+        for (int db = 0; db < D / 16; ++db) o[db] = (float4_t)(0.0f);
+        m = -INFINITY;
+        l = 0.0f;
+        vec8 kf[2][NK];
+        if (it0 < it1) fetch(it0, kf, 0);
+        for (int it = it0; it < it1; it += 4) {
+            const int stage = ((it - it0) >> 2) & 1;
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+            const int j0 = first_key(it);
+            float4_t s[2];
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                s[i] = (float4_t)(0.0f);
+#pragma unroll
+                for (int kb = 0; kb < NK; ++kb) s[i] = X::mfma16(kf[i][kb], qf[kb], s[i]);
+            }
+            if (it + 4 < it1) fetch(it + 4, kf, stage ^ 1);
+            if (GEN) {
+#pragma unroll
+                for (int i = 0; i < 2; ++i)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        float x = s[i][r];
+                        if (cap) x = fmaf(-2.0f * p.cap_out, __builtin_amdgcn_rcpf(1.0f + att_exp2(x * p.cap_in)), p.cap_out);
+                        else x *= p.scale2;
+                        s[i][r] = fmaf(-slope2, fabsf((float)(see.pos - (j0 + 16 * i + 4 * quarter + r))), x);
+                    }
+            }
+            unsigned seen = 0xff;
+            if (SAFE || j0 < lo_max || j0 + 32 > hi_min) {
+                seen = 0;
+#pragma unroll
+                for (int i = 0; i < 2; ++i)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        const int j = j0 + 16 * i + 4 * quarter + r;
+                        const bool v = (unsigned)(j - see.lo) < (unsigned)(see.hi - see.lo) || (unsigned)(j - see.plo) < (unsigned)(see.phi - see.plo);
+                        s[i][r] = v ? s[i][r] : -INFINITY;
+                        seen |= v ? 1u << (4 * i + r) : 0u;
+                    }
+            }
+            float top = -INFINITY;
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) top = fmaxf(top, s[i][r]);
+            top *= step;
+            if (__any(top > m + 8.0f)) {     // m is the row's, the same in its four lanes
+                top = fmaxf(top, __shfl_xor(top, 16, 64));
+                top = fmaxf(top, __shfl_xor(top, 32, 64));
+                const float mn = fmaxf(m, top);
+                const float f = m == -INFINITY ? 0.0f : att_exp2(m - mn);
+                m = mn;
+                l *= f;
+#pragma unroll
+                for (int db = 0; db < D / 16; ++db)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) o[db][r] *= f;
+            }
+            const float base = m == -INFINITY ? 0.0f : m;
+            uintx4 hi, lo;
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+#pragma unroll
+                for (int r = 0; r < 4; r += 2) {
+                    const float x = att_exp2(fmaf(s[i][r], step, -base)), y = att_exp2(fmaf(s[i][r + 1], step, -base));
+                    l += x + y;
+                    const unsigned h = op_pack2(x, y, T());
+                    hi[2 * i + (r >> 1)] = h;
+                    const T *hx = (const T *)&h;
+                    lo[2 * i + (r >> 1)] = op_pack2(x - (float)hx[0], y - (float)hx[1], T());
+                }
+#pragma unroll
+            for (int db = 0; db < D / 16; ++db) {
+                const uintx2 x = att_lds_tr(vaddr[db] + stage * STAGE), y = att_lds_tr(vaddr[db] + stage * STAGE + 16 * PITCH);
+                uintx4 v = {x[0], x[1], y[0], y[1]};
+                if (SAFE) {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        if ((v[e] & X::EXPONENT) == X::EXPONENT) v[e] &= 0xffff0000u;
+                        if (((v[e] >> 16) & X::EXPONENT) == X::EXPONENT) v[e] &= 0x0000ffffu;
+                    }
+                }
+                o[db] = X::mfma16(__builtin_bit_cast(vec8, v), __builtin_bit_cast(vec8, hi), o[db]);
+                o[db] = X::mfma16(__builtin_bit_cast(vec8, v), __builtin_bit_cast(vec8, lo), o[db]);
+            }
+            if (SAFE) {   // as in attention_kernel
+                uintx4 w;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) w[e] = ((seen >> (2 * e)) & 1 ? X::ONE : 0u) | ((seen >> (2 * e + 1)) & 1 ? X::ONE << 16 : 0u);
+#pragma unroll 1
+                for (int kind = 0; kind < 3; ++kind)
+#pragma unroll
+                    for (int db = 0; db < D / 16; ++db) {
+                        const uintx2 x = att_lds_tr(vaddr[db] + stage * STAGE), y = att_lds_tr(vaddr[db] + stage * STAGE + 16 * PITCH);
+                        const uintx4 v = {x[0], x[1], y[0], y[1]};
+                        const float4_t hit = X::mfma16(__builtin_bit_cast(vec8, att_places<T>(v, kind)), __builtin_bit_cast(vec8, w), (float4_t)(0.0f));
+                        const float what = kind == 0 ? NAN : kind == 1 ? INFINITY : -INFINITY;
+#pragma unroll
+                        for (int r = 0; r < 4; ++r)
+                            if (hit[r] > 0.0f) o[db][r] += what;
+                    }
+            }
+        }
+    };
+    pass(std::false_type());
+    bool odd = false;
+#pragma unroll
+    for (int db = 0; db < D / 16; ++db)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) odd = odd || o[db][r] != o[db][r];
+    if (__any(odd)) pass(std::true_type());
+
+    // the four waves' parts, through LDS: [wave][16 rows][D] sums, [wave][16] maxima and sums of a row
+    l += __shfl_xor(l, 16, 64);
+    l += __shfl_xor(l, 32, 64);
+    __syncthreads();
+    constexpr int OLD = D + 4;
+    float *so = (float *)smem, *sm = so + 4 * 16 * OLD, *sl = sm + 64;
+#pragma unroll
+    for (int db = 0; db < D / 16; ++db) *(floatx4 *)(so + (wave * 16 + l15) * OLD + 16 * db + 4 * quarter) = (floatx4){o[db][0], o[db][1], o[db][2], o[db][3]};
+    if (quarter == 0) {
+        sm[wave * 16 + l15] = m;
+        sl[wave * 16 + l15] = l;
+    }
+    __syncthreads();
+    for (int c = tid; c < p.rows * (D / 4); c += 256) {
+        const int r = c / (D / 4), d4 = c % (D / 4) * 4;
+        float top = -INFINITY;
+#pragma unroll
+        for (int w = 0; w < 4; ++w) top = fmaxf(top, sm[w * 16 + r]);
+        const float base = top == -INFINITY ? 0.0f : top;
+        float sum = 0.0f;
+        floatx4 y = (floatx4)(0.0f);
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+            const float f = sm[w * 16 + r] == -INFINITY ? (sl[w * 16 + r] == 0.0f ? 0.0f : 1.0f) : att_exp2(sm[w * 16 + r] - base);
+            if (f == 0.0f) continue;
+            sum = fmaf(f, sl[w * 16 + r], sum);
+            const floatx4 x = *(const floatx4 *)(so + (w * 16 + r) * OLD + d4);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) y[e] = fmaf(f, x[e], y[e]);
+        }
+        const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+        const int rt = r / p.group, rh = kvh * p.group + (r - rt * p.group);
+        if (p.splits > 1) {
+            const int64_t at = ((int64_t)pair * p.rows + r) * p.splits + split;
+            *(floatx4 *)(p.part_o + at * D + d4) = (floatx4){y[0] * inv, y[1] * inv, y[2] * inv, y[3] * inv};
+            if (d4 == 0) p.part_l[at] = sum == 0.0f ? -INFINITY : base + log2f(sum);
+        } else {
+            T *out = (T *)a.out + b * a.out_stride[0] + rt * a.out_stride[1] + rh * a.out_stride[2] + d4;
+            *(uintx2 *)out = (uintx2){op_pack2(y[0] * inv, y[1] * inv, T()), op_pack2(y[2] * inv, y[3] * inv, T())};
+            if (a.lse != nullptr && d4 == 0)
+                a.lse[((int64_t)b * a.heads + rh) * a.q_tokens + rt] = sum == 0.0f ? -INFINITY : base * 0.6931471805599453f + logf(sum);
+        }
+    }
+}
+
+// ------------------------------------------------------------------------------------------------------------------
+// Joins the parts of a row: one workgroup per row, D / 4 threads per part, 256 / (D / 4) parts at a time.
 template <typename T, int D>
 __global__ __launch_bounds__(256) void attention_join_kernel(AttArgs p) {
+    constexpr int TP = D / 4, G = 256 / TP;     // threads per part, parts at a time (D 96: 24 and 10, the last threads idle)
+    __shared__ float red[G][D + 4];
+    __shared__ float tops[4];
     const mibc_attention_args &a = p.a;
-    const int lane = threadIdx.x & 63;
-    const int64_t r = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-    if (r >= (int64_t)p.pairs * p.rows) return;
+    const int tid = threadIdx.x;
+    const int64_t r = blockIdx.x;
     const int pair = (int)(r / p.rows), row = (int)(r - (int64_t)pair * p.rows);
     const int b = pair / a.kv_heads, kvh = pair - b * a.kv_heads;
     const int t = row / p.group, head = kvh * p.group + (row - t * p.group);
     const float *pl = p.part_l + r * p.splits;
     const float *po = p.part_o + r * p.splits * D;
     float m = -INFINITY;
-    for (int s = 0; s < p.splits; ++s) m = fmaxf(m, pl[s]);
+    for (int s = tid; s < p.splits; s += 256) m = fmaxf(m, pl[s]);
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
+    if ((tid & 63) == 0) tops[tid >> 6] = m;
+    __syncthreads();
+    m = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
     const float base = m == -INFINITY ? 0.0f : m;
-    float sum = 0.0f, y[(D + 63) / 64];
+    const int g = tid / TP, d4 = tid % TP * 4;
+    float sum = 0.0f;
+    floatx4 y = (floatx4)(0.0f);
+    if (g < G) {
+        for (int s = g; s < p.splits; s += G) {
+            const floatx4 x = *(const floatx4 *)(po + (int64_t)s * D + d4);
+            const float w = att_exp2(pl[s] - base);
+            sum += w;
 #pragma unroll
-    for (int i = 0; i < (D + 63) / 64; ++i) y[i] = 0.0f;
-    for (int s = 0; s < p.splits; ++s) {
-        const float w = att_exp2(pl[s] - base);
-        if (w == 0.0f) continue;
-        sum += w;
-#pragma unroll
-        for (int i = 0; i < (D + 63) / 64; ++i)
-            if (lane + 64 * i < D) y[i] = fmaf(w, po[(int64_t)s * D + lane + 64 * i], y[i]);
+            for (int e = 0; e < 4; ++e) y[e] = w == 0.0f ? y[e] : fmaf(w, x[e], y[e]);   // a part without keys holds zeros
+        }
+        *(floatx4 *)(&red[g][d4]) = y;
+        if (d4 == 0) red[g][D] = sum;
     }
-    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-    T *out = (T *)a.out + b * a.out_stride[0] + t * a.out_stride[1] + head * a.out_stride[2];
-#pragma unroll
-    for (int i = 0; i < (D + 63) / 64; ++i)
-        if (lane + 64 * i < D) out[lane + 64 * i] = (T)(y[i] * inv);
-    if (a.lse != nullptr && lane == 0)
-        a.lse[((int64_t)b * a.heads + head) * a.q_tokens + t] = sum == 0.0f ? -INFINITY : base * 0.6931471805599453f + logf(sum);
+    __syncthreads();
+    for (int d = tid; d < D; d += 256) {
+        float v = 0.0f, n = 0.0f;
+        for (int i = 0; i < G; ++i) {
+            v += red[i][d];
+            n += red[i][D];
+        }
+        const float inv = n == 0.0f ? 0.0f : 1.0f / n;
+        ((T *)a.out + b * a.out_stride[0] + t * a.out_stride[1] + head * a.out_stride[2])[d] = (T)(v * inv);
+        if (a.lse != nullptr && d == 0)
+            a.lse[((int64_t)b * a.heads + head) * a.q_tokens + t] = n == 0.0f ? -INFINITY : base * 0.6931471805599453f + logf(n);
+    }
 }
 
 template <typename T, int NW>
@@ -486,13 +756,25 @@ static void att_rows(hipStream_t s, const AttArgs &p, unsigned grid) {
     }
 }
 template <typename T>
+static void att_token(hipStream_t s, const AttArgs &p, unsigned grid) {
+    constexpr int FETCH = 4 * 2 * 32 * ATT_D * 2, JOIN = 4 * 16 * (ATT_D + 4 + 2) * 4, LDS = FETCH > JOIN ? FETCH : JOIN;
+    if (p.cap_out > 0.0f || p.a.slopes != nullptr) {
+        MIBC_LDS_ATTR_ONCE((attention_token_kernel<T, ATT_D, true>), LDS);
+        hipLaunchKernelGGL((attention_token_kernel<T, ATT_D, true>), dim3(grid), dim3(256), LDS, s, p);
+    } else {
+        MIBC_LDS_ATTR_ONCE((attention_token_kernel<T, ATT_D, false>), LDS);
+        hipLaunchKernelGGL((attention_token_kernel<T, ATT_D, false>), dim3(grid), dim3(256), LDS, s, p);
+    }
+}
+template <typename T>
 static int att_launch(hipStream_t s, const AttArgs &p, int variant, unsigned grid) {
-    if (variant == 0) att_rows<T, 8>(s, p, grid);
+    if (variant == 3) att_token<T>(s, p, grid);
+    else if (variant == 0) att_rows<T, 8>(s, p, grid);
     else if (variant == 1) att_rows<T, 4>(s, p, grid);
     else att_rows<T, 2>(s, p, grid);
     int rc = op_hip(hipGetLastError(), "attention");
     if (rc != MIBC_OK || p.splits == 1) return rc;
-    hipLaunchKernelGGL((attention_join_kernel<T, ATT_D>), dim3((unsigned)(((int64_t)p.pairs * p.rows + 3) / 4)), dim3(256), 0, s, p);
+    hipLaunchKernelGGL((attention_join_kernel<T, ATT_D>), dim3((unsigned)((int64_t)p.pairs * p.rows)), dim3(256), 0, s, p);
     return op_hip(hipGetLastError(), "attention");
 }
 #define ATT_CAT2(a, b) a##b
