@@ -117,6 +117,23 @@ __device__ __forceinline__ AttRow att_row(const mibc_attention_args &a, int b, i
 }
 #define ATT_FAR 0x7fffffff
 
+// The exponent (base 2) of a score is mul * x + add, x being what the registers hold.  Plain: x = q.k, mul = scale log2(e).
+// Capped: cap tanh(y) = cap - 2 cap / (1 + e^2y), so x = 1 / (1 + e^2y) and the last product is the exponent's own fma; the
+// largest score is the smallest x.  A slope adds slope * |i - j| to x, in x's unit.
+template <bool CAP>
+struct AttScore {
+    float mul, add, slope, in;
+    static constexpr float HIDDEN = CAP ? INFINITY : -INFINITY;
+    __device__ __forceinline__ AttScore(const AttArgs &p, int head) {
+        mul = CAP ? -2.0f * p.cap_out : p.scale2;
+        add = CAP ? p.cap_out : 0.0f;
+        in = p.cap_in;
+        slope = p.a.slopes != nullptr ? -p.a.slopes[head] * 1.4426950408889634f / mul : 0.0f;
+    }
+    __device__ __forceinline__ float capped(float x) const { return __builtin_amdgcn_rcpf(1.0f + att_exp2(x * in)); }
+    __device__ __forceinline__ float larger(float a, float b) const { return CAP ? fminf(a, b) : fmaxf(a, b); }
+};
+
 // 1 where a value is NaN (kind 0), infinity (1), -infinity (2), else 0
 template <typename T>
 __device__ __forceinline__ uintx4 att_places(uintx4 v, int kind) {
@@ -152,7 +169,7 @@ __device__ __forceinline__ int att_v_slot(int row, int chunk) {
     return D == 128 ? chunk ^ ((row & 3) << 2) : D == 64 ? chunk ^ (((row >> 1) & 1) << 2) : chunk;
 }
 
-template <typename T, int D, int NW, bool GEN>
+template <typename T, int D, int NW, bool CAP>
 __global__ __launch_bounds__(NW * 64, 2) void attention_kernel(AttArgs p) {
     typedef AttType<T> X;
     typedef typename X::vec8 vec8;
@@ -197,6 +214,7 @@ __global__ __launch_bounds__(NW * 64, 2) void attention_kernel(AttArgs p) {
     const int lo_min = att_wave_min(some ? see.lo : ATT_FAR), hi_max = att_wave_max(some ? see.hi : 0);
     const int lo_max = att_wave_max(some ? see.lo : ATT_FAR), hi_min = att_wave_min(some ? see.hi : 0);
     const int plo_min = att_wave_min(apart ? see.plo : ATT_FAR), phi_max = att_wave_max(apart ? see.phi : 0);
+    const bool tail_apart = phi_max > 0;     // some row's prefix does not join on to its window
     if (lane == 0) {
         range[wave][0] = lo_min;
         range[wave][1] = hi_max;
@@ -275,9 +293,8 @@ __global__ __launch_bounds__(NW * 64, 2) void attention_kernel(AttArgs p) {
         const int r = 4 * half + ((lane >> 2) & 3);
         vaddr[db] = lds + TILE + r * PITCH + att_v_slot<D>(r, 4 * db + 2 * ((lane >> 4) & 1) + ((lane >> 1) & 1)) * 16 + (lane & 1) * 8;
     }
-    const float slope2 = (GEN && a.slopes != nullptr) ? a.slopes[head] * 1.4426950408889634f : 0.0f;
-    const bool cap = GEN && p.cap_out > 0.0f;
-    const float step = GEN ? 1.0f : p.scale2;     // what a score is multiplied with in the exponent
+    const AttScore<CAP> score(p, head);
+    const bool slopes = a.slopes != nullptr;
 
     float16_t o[D / 32];
     float m, l;
@@ -306,40 +323,56 @@ __global__ __launch_bounds__(NW * 64, 2) void attention_kernel(AttArgs p) {
 #pragma unroll
                 for (int i = 0; i < 2; ++i)
                     s[i] = X::mfma32(att_lds16<vec8>(kaddr[ks] + at + i * (32 * PITCH)), qf[ks], s[i]);
-            if (GEN) {
+            if (CAP) {
 #pragma unroll
                 for (int i = 0; i < 2; ++i)
 #pragma unroll
-                    for (int r = 0; r < 16; ++r) {
-                        float x = s[i][r];
-                        if (cap) {   // tanh(y) = 1 - 2 / (1 + e^2y)
-                            x = fmaf(-2.0f * p.cap_out, __builtin_amdgcn_rcpf(1.0f + att_exp2(x * p.cap_in)), p.cap_out);
-                        } else {
-                            x *= p.scale2;
-                        }
-                        const int j = j0 + 32 * i + (r & 3) + 8 * (r >> 2) + 4 * half;
-                        s[i][r] = fmaf(-slope2, fabsf((float)(see.pos - j)), x);
-                    }
+                    for (int r = 0; r < 16; ++r) s[i][r] = score.capped(s[i][r]);
+            }
+            if (slopes) {
+                const float away = (float)(see.pos - j0 - 4 * half);
+#pragma unroll
+                for (int i = 0; i < 2; ++i)
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) s[i][r] = fmaf(score.slope, fabsf(away - (float)(32 * i + (r & 3) + 8 * (r >> 2))), s[i][r]);
             }
             unsigned seen = 0xffffffffu;     // bit 16 i + r
             if (!full) {
-                seen = 0;
+                // element e = 32 i + (r & 3) + 8 (r >> 2) of the tile is key j0 + 4 half + e
+                const int at0 = j0 + 4 * half, lo = see.lo - at0, hi = see.hi - at0;
+                if (SAFE || tail_apart) {
+                    const int plo = see.plo - at0, phi = see.phi - at0;
+                    seen = 0;
 #pragma unroll
-                for (int i = 0; i < 2; ++i)
+                    for (int i = 0; i < 2; ++i)
 #pragma unroll
-                    for (int r = 0; r < 16; ++r) {
-                        const int j = j0 + 32 * i + (r & 3) + 8 * (r >> 2) + 4 * half;
-                        const bool v = (unsigned)(j - see.lo) < (unsigned)(see.hi - see.lo) || (unsigned)(j - see.plo) < (unsigned)(see.phi - see.plo);
-                        s[i][r] = v ? s[i][r] : -INFINITY;
-                        if (SAFE) seen |= v ? 1u << (16 * i + r) : 0u;
+                        for (int r = 0; r < 16; ++r) {
+                            const int e = 32 * i + (r & 3) + 8 * (r >> 2);
+                            const bool v = (e >= lo && e < hi) || (e >= plo && e < phi);
+                            s[i][r] = v ? s[i][r] : score.HIDDEN;
+                            if (SAFE) seen |= v ? 1u << (16 * i + r) : 0u;
+                        }
+                } else {
+                    if (j0 + 64 > hi_min) {
+#pragma unroll
+                        for (int i = 0; i < 2; ++i)
+#pragma unroll
+                            for (int r = 0; r < 16; ++r) s[i][r] = 32 * i + (r & 3) + 8 * (r >> 2) < hi ? s[i][r] : score.HIDDEN;
                     }
+                    if (j0 < lo_max) {
+#pragma unroll
+                        for (int i = 0; i < 2; ++i)
+#pragma unroll
+                            for (int r = 0; r < 16; ++r) s[i][r] = 32 * i + (r & 3) + 8 * (r >> 2) >= lo ? s[i][r] : score.HIDDEN;
+                    }
+                }
             }
-            float top = -INFINITY;
+            float top = s[0][0];
 #pragma unroll
             for (int i = 0; i < 2; ++i)
 #pragma unroll
-                for (int r = 0; r < 16; ++r) top = fmaxf(top, s[i][r]);
-            top = att_half_max(top) * step;
+                for (int r = 0; r < 16; ++r) top = score.larger(top, s[i][r]);
+            top = att_half_max(fmaf(top, score.mul, score.add));
             // the maximum is only moved when it grew by more than 2^8: probabilities stay below 256, exact in f32 sums
             if (__any(top > m + 8.0f)) {
                 const float mn = fmaxf(m, top);
@@ -351,7 +384,7 @@ __global__ __launch_bounds__(NW * 64, 2) void attention_kernel(AttArgs p) {
 #pragma unroll
                     for (int r = 0; r < 16; ++r) o[db][r] *= f;
             }
-            const float base = m == -INFINITY ? 0.0f : m;
+            const float off = score.add - (m == -INFINITY ? 0.0f : m);
             float add = 0.0f;
             vec8 pf[4];
 #pragma unroll
@@ -359,7 +392,7 @@ __global__ __launch_bounds__(NW * 64, 2) void attention_kernel(AttArgs p) {
                 uintx4 pk[2];
 #pragma unroll
                 for (int r = 0; r < 16; r += 2) {
-                    const float x = att_exp2(fmaf(s[i][r], step, -base)), y = att_exp2(fmaf(s[i][r + 1], step, -base));
+                    const float x = att_exp2(fmaf(s[i][r], score.mul, off)), y = att_exp2(fmaf(s[i][r + 1], score.mul, off));
                     add += x + y;
                     pk[r >> 3][(r & 7) >> 1] = op_pack2(x, y, T());
                 }
@@ -461,7 +494,7 @@ __device__ __forceinline__ int att_v_slot16(int row, int chunk) {
     return D == 128 ? chunk ^ (((row & 3) << 2) | ((row & 4) >> 1)) : D == 64 ? chunk ^ ((((row >> 1) & 1) << 2) | ((row & 4) >> 1)) : chunk;
 }
 
-template <typename T, int D, bool GEN>
+template <typename T, int D, bool CAP>
 __global__ __launch_bounds__(256, 2) void attention_token_kernel(AttArgs p) {
     typedef AttType<T> X;
     typedef typename X::vec8 vec8;
@@ -526,9 +559,8 @@ __global__ __launch_bounds__(256, 2) void attention_token_kernel(AttArgs p) {
         const int r = 4 * quarter + (l15 >> 2);
         vaddr[db] = mine + r * PITCH + att_v_slot16<D>(r, 2 * db + ((lane >> 1) & 1)) * 16 + (lane & 1) * 8;
     }
-    const float slope2 = (GEN && a.slopes != nullptr) ? a.slopes[head] * 1.4426950408889634f : 0.0f;
-    const bool cap = GEN && p.cap_out > 0.0f;
-    const float step = GEN ? 1.0f : p.scale2;
+    const AttScore<CAP> score(p, head);
+    const bool slopes = a.slopes != nullptr;
 
     float4_t o[D / 16];
     float m, l;
@@ -552,16 +584,18 @@ __global__ __launch_bounds__(256, 2) void attention_token_kernel(AttArgs p) {
                 for (int kb = 0; kb < NK; ++kb) s[i] = X::mfma16(kf[i][kb], qf[kb], s[i]);
             }
             if (it + 4 < it1) fetch(it + 4, kf, stage ^ 1);
-            if (GEN) {
+            if (CAP) {
 #pragma unroll
                 for (int i = 0; i < 2; ++i)
 #pragma unroll
-                    for (int r = 0; r < 4; ++r) {
-                        float x = s[i][r];
-                        if (cap) x = fmaf(-2.0f * p.cap_out, __builtin_amdgcn_rcpf(1.0f + att_exp2(x * p.cap_in)), p.cap_out);
-                        else x *= p.scale2;
-                        s[i][r] = fmaf(-slope2, fabsf((float)(see.pos - (j0 + 16 * i + 4 * quarter + r))), x);
-                    }
+                    for (int r = 0; r < 4; ++r) s[i][r] = score.capped(s[i][r]);
+            }
+            if (slopes) {
+                const float away = (float)(see.pos - j0 - 4 * quarter);
+#pragma unroll
+                for (int i = 0; i < 2; ++i)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) s[i][r] = fmaf(score.slope, fabsf(away - (float)(16 * i + r)), s[i][r]);
             }
             unsigned seen = 0xff;
             if (SAFE || j0 < lo_max || j0 + 32 > hi_min) {
@@ -572,16 +606,16 @@ __global__ __launch_bounds__(256, 2) void attention_token_kernel(AttArgs p) {
                     for (int r = 0; r < 4; ++r) {
                         const int j = j0 + 16 * i + 4 * quarter + r;
                         const bool v = (unsigned)(j - see.lo) < (unsigned)(see.hi - see.lo) || (unsigned)(j - see.plo) < (unsigned)(see.phi - see.plo);
-                        s[i][r] = v ? s[i][r] : -INFINITY;
+                        s[i][r] = v ? s[i][r] : score.HIDDEN;
                         seen |= v ? 1u << (4 * i + r) : 0u;
                     }
             }
-            float top = -INFINITY;
+            float top = s[0][0];
 #pragma unroll
             for (int i = 0; i < 2; ++i)
 #pragma unroll
-                for (int r = 0; r < 4; ++r) top = fmaxf(top, s[i][r]);
-            top *= step;
+                for (int r = 0; r < 4; ++r) top = score.larger(top, s[i][r]);
+            top = fmaf(top, score.mul, score.add);
             if (__any(top > m + 8.0f)) {     // m is the row's, the same in its four lanes
                 top = fmaxf(top, __shfl_xor(top, 16, 64));
                 top = fmaxf(top, __shfl_xor(top, 32, 64));
@@ -594,13 +628,13 @@ __global__ __launch_bounds__(256, 2) void attention_token_kernel(AttArgs p) {
 #pragma unroll
                     for (int r = 0; r < 4; ++r) o[db][r] *= f;
             }
-            const float base = m == -INFINITY ? 0.0f : m;
+            const float off = score.add - (m == -INFINITY ? 0.0f : m);
             uintx4 hi, lo;
 #pragma unroll
             for (int i = 0; i < 2; ++i)
 #pragma unroll
                 for (int r = 0; r < 4; r += 2) {
-                    const float x = att_exp2(fmaf(s[i][r], step, -base)), y = att_exp2(fmaf(s[i][r + 1], step, -base));
+                    const float x = att_exp2(fmaf(s[i][r], score.mul, off)), y = att_exp2(fmaf(s[i][r + 1], score.mul, off));
                     l += x + y;
                     const unsigned h = op_pack2(x, y, T());
                     hi[2 * i + (r >> 1)] = h;
@@ -747,7 +781,7 @@ __global__ __launch_bounds__(256) void attention_join_kernel(AttArgs p) {
 template <typename T, int NW>
 static void att_rows(hipStream_t s, const AttArgs &p, unsigned grid) {
     constexpr int LDS = 4 * 64 * ATT_D * 2;
-    if (p.cap_out > 0.0f || p.a.slopes != nullptr) {
+    if (p.cap_out > 0.0f) {
         MIBC_LDS_ATTR_ONCE((attention_kernel<T, ATT_D, NW, true>), LDS);
         hipLaunchKernelGGL((attention_kernel<T, ATT_D, NW, true>), dim3(grid), dim3(NW * 64), LDS, s, p);
     } else {
@@ -758,7 +792,7 @@ static void att_rows(hipStream_t s, const AttArgs &p, unsigned grid) {
 template <typename T>
 static void att_token(hipStream_t s, const AttArgs &p, unsigned grid) {
     constexpr int FETCH = 4 * 2 * 32 * ATT_D * 2, JOIN = 4 * 16 * (ATT_D + 4 + 2) * 4, LDS = FETCH > JOIN ? FETCH : JOIN;
-    if (p.cap_out > 0.0f || p.a.slopes != nullptr) {
+    if (p.cap_out > 0.0f) {
         MIBC_LDS_ATTR_ONCE((attention_token_kernel<T, ATT_D, true>), LDS);
         hipLaunchKernelGGL((attention_token_kernel<T, ATT_D, true>), dim3(grid), dim3(256), LDS, s, p);
     } else {
