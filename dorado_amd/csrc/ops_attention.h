@@ -3,8 +3,21 @@
 #pragma once
 #include "ops.h"
 
+// n / d for n < 2^31 by a multiplication
+struct AttDiv {
+    unsigned m, s;
+    void set(unsigned d) {
+        s = 0;
+        while ((1ull << s) < d) ++s;
+        m = d == 1 ? 0 : (unsigned)((1ull << (31 + s)) / d + 1);
+    }
+    __device__ __forceinline__ unsigned div(unsigned n) const { return m == 0 ? n : __umulhi(n, m) >> (s - 1); }
+};
+
 struct AttArgs {
     mibc_attention_args a;
+    AttDiv by_pairs, by_splits, by_tiles, by_kv, by_group;
+    int back, ahead;  // the window's limits, -1: none
     int group;        // query heads per key head
     int rows;         // q_tokens * group: row r = (token r / group, head r % group) of a (batch, key head) pair
     int pairs;        // batch * kv_heads
@@ -17,7 +30,7 @@ struct AttArgs {
     float *part_l;    // [pairs * rows][splits] log2 of the sum
 };
 
-// variant: 0 row tiles of 256, 1 of 128, 2 of 64, 3 at most 16 rows per pair (single tokens)
+enum AttVariant { ATT_ROWS_128, ATT_ROWS_64, ATT_TOKENS };   // row tiles of 128 or 64; at most 16 rows per pair (single tokens)
 #define MIBC_ATT_DECLARE(D) int mibc_att_launch_##D(hipStream_t s, const AttArgs &p, int variant, unsigned grid);
 MIBC_ATT_DECLARE(32)
 MIBC_ATT_DECLARE(64)

@@ -13,10 +13,10 @@ static int att_check(const mibc_attention_args &a) {
     if (!(a.scale > 0.0f) || !(a.scale <= 1e30f)) return op_refuse(MIBC_ERR_ARG, "attention: scale must be positive and finite");
     if (!(a.softcap >= 0.0f) || !(a.softcap <= 1e30f)) return op_refuse(MIBC_ERR_ARG, "attention: softcap must be 0 (none) or positive and finite");
     if (a.reserved != 0) return op_refuse(MIBC_ERR_ARG, "attention: reserved must be 0");
-    const int64_t big = (int64_t)1 << 30;
+    const int64_t big = (int64_t)1 << 28;     // positions, and distances between them, stay far inside 32 bits
     if (a.q_tokens > big || a.k_tokens > big || (int64_t)a.q_tokens * (a.heads / a.kv_heads) > big ||
         (int64_t)a.batch * a.kv_heads > big || (a.q_start != MIBC_ATTN_END && (a.q_start > big || a.q_start < -big)))
-        return op_refuse(MIBC_NOT_SUPPORTED, "attention: more than 2^30 tokens, rows or heads");
+        return op_refuse(MIBC_NOT_SUPPORTED, "attention: more than 2^28 tokens, rows or heads");
     if (a.doc_offsets != nullptr) {
         if (a.batch != 1 || a.q_tokens != a.k_tokens || a.k_len != nullptr || a.q_start != MIBC_ATTN_END)
             return op_refuse(MIBC_ERR_ARG, "attention: documents need batch 1, q_tokens == k_tokens, no k_len and no q_start");
@@ -50,8 +50,8 @@ struct AttPlan {
 static AttPlan att_plan(const mibc_attention_args &a) {
     const int64_t rows = (int64_t)a.q_tokens * (a.heads / a.kv_heads), pairs = (int64_t)a.batch * a.kv_heads;
     AttPlan p;
-    p.variant = rows <= 16 ? 3 : rows > 128 ? 0 : rows > 64 ? 1 : 2;
-    const int tile = p.variant == 0 ? 256 : p.variant == 1 ? 128 : p.variant == 2 ? 64 : 16;
+    p.variant = rows <= 16 ? ATT_TOKENS : rows > 64 ? ATT_ROWS_128 : ATT_ROWS_64;
+    const int tile = p.variant == ATT_ROWS_128 ? 128 : p.variant == ATT_ROWS_64 ? 64 : 16;
     p.tiles = (int)((rows + tile - 1) / tile);
     // keys a row can see at most
     int64_t keys = a.k_tokens;
@@ -62,9 +62,10 @@ static AttPlan att_plan(const mibc_attention_args &a) {
     const int64_t groups = p.tiles * pairs;
     // tiles: two workgroups per CU, a part is worth its share of the join from four tiles of 64 keys on;
     // tokens: eight per CU (rows of a batch differ in length), from four steps of 32 keys for each of the four waves on
-    const int64_t want = p.variant == 3 ? 2048 : 512, least = p.variant == 3 ? 512 : 256;
+    const int64_t want = p.variant == ATT_TOKENS ? 2048 : 512, least = p.variant == ATT_TOKENS ? 512 : 256;
     int64_t splits = groups >= want ? 1 : want / groups;
     if (splits > keys / least) splits = keys / least;
+    if (splits > 255) splits = 255;
     p.splits = splits < 1 ? 1 : (int)splits;
     return p;
 }
@@ -100,6 +101,13 @@ int mibc_launch_attention(hipStream_t s, const mibc_attention_args &a) {
     p.pairs = a.batch * a.kv_heads;
     p.tiles = plan.tiles;
     p.splits = plan.splits;
+    p.by_pairs.set((unsigned)p.pairs);
+    p.by_splits.set((unsigned)p.splits);
+    p.by_tiles.set((unsigned)p.tiles);
+    p.by_kv.set((unsigned)a.kv_heads);
+    p.by_group.set((unsigned)p.group);
+    p.back = a.window_back >= 0 && a.window_back < 1 << 30 ? a.window_back : -1;
+    p.ahead = a.window_ahead >= 0 && a.window_ahead < 1 << 30 ? a.window_ahead : -1;
     p.scale2 = a.scale * 1.4426950408889634f;
     if (a.softcap > 0.0f) {
         p.cap_in = 2.0f * a.scale / a.softcap * 1.4426950408889634f;

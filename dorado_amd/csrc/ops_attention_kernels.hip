@@ -52,75 +52,62 @@ __device__ __forceinline__ float att_half_add(float x) {
     const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
     return __uint_as_float(r[0]) + __uint_as_float(r[1]);
 }
-__device__ __forceinline__ int att_wave_min(int x) {
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) x = min(x, __shfl_xor(x, o, 64));
-    return __builtin_amdgcn_readfirstlane(x);
+__device__ __forceinline__ int att_low_half(int x) {   // lane i and i + 32 get lane i's
+    return (int)__builtin_amdgcn_permlane32_swap((unsigned)x, (unsigned)x, false, false)[0];
 }
-__device__ __forceinline__ int att_wave_max(int x) { return -att_wave_min(-x); }
 
-// What a row sees: [lo, hi) and, where a prefix does not join on to it, [plo, phi).  An empty interval is [0, 0).
+// What a row sees: [lo, hi) and, if `apart` kernels ask for it, [plo, phi), the prefix.  Both borders of both grow with the token
+// (documents in order), so the rows between two rows see nothing outside [lo of the first, hi of the last) and the prefixes' hull.
 struct AttRow {
     int lo, hi, plo, phi, pos;
 };
-__device__ __forceinline__ AttRow att_row(const mibc_attention_args &a, int b, int t) {
-    int64_t k0 = 0, k1, pos;
-    int pre = 0;
-    if (a.doc_offsets != nullptr) {
-        // the last border that is <= t; borders out of order end in some document, whose keys are clamped all the same
-        int first = 0, n = a.n_docs + 1;     // borders [0, first) are <= t
-        while (n > 0) {
-            const int half = n >> 1;
-            if (a.doc_offsets[first + half] <= t) {
-                first += half + 1;
-                n -= half + 1;
-            } else {
-                n = half;
-            }
-        }
-        const int d = first - 1;
-        pos = t;
-        k1 = 0;
-        if (d >= 0 && d < a.n_docs) {
-            k0 = max(a.doc_offsets[d], 0);
-            k1 = min(a.doc_offsets[d + 1], a.k_tokens);
+// borders <= t, t the same in all lanes: 64 borders a step
+__device__ __forceinline__ int att_borders(const int32_t *border, int count, int t, int lane) {
+    int base = 0;
+    while (count > 64) {
+        const int stride = (count + 63) >> 6;       // lane's block of borders: is its last one <= t?
+        const int k = __popcll(__ballot(border[base + min((lane + 1) * stride, count) - 1] <= t));
+        const int skip = min(k * stride, count);
+        base += skip;
+        count = min(stride, count - skip);
+    }
+    const bool in = lane < count && border[base + min(lane, max(count - 1, 0))] <= t;
+    return base + __popcll(__ballot(in));
+}
+// t, and the number of borders <= t of a row of documents
+__device__ __forceinline__ AttRow att_row(const AttArgs &p, int b, int t, int borders) {
+    const mibc_attention_args &a = p.a;
+    int k0 = 0, k1, pre = 0;
+    AttRow r;
+    if (a.doc_offsets != nullptr) {     // borders out of order end in some document, whose keys are clamped all the same
+        const int d = min(max(borders - 1, 0), a.n_docs);
+        k0 = min(max(a.doc_offsets[d], 0), a.k_tokens);
+        k1 = k0;                         // in front of the first document, behind the last: nothing
+        if (borders > 0 && d < a.n_docs) {
+            k1 = min(max(a.doc_offsets[d + 1], k0), a.k_tokens);
             if (a.prefix != nullptr) pre = a.prefix[d];
         }
+        r.pos = t;
     } else {
         k1 = a.k_len != nullptr ? min(max(a.k_len[b], 0), a.k_tokens) : a.k_tokens;
-        pos = (a.q_start == MIBC_ATTN_END ? k1 - a.q_tokens : (int64_t)a.q_start) + t;
+        r.pos = (a.q_start == MIBC_ATTN_END ? k1 - a.q_tokens : a.q_start) + t;
         if (a.prefix != nullptr) pre = a.prefix[b];
     }
-    int64_t lo = a.window_back < 0 ? k0 : max(k0, pos - a.window_back);
-    int64_t hi = a.window_ahead < 0 ? k1 : min(k1, pos + a.window_ahead + 1);
-    int64_t ph = min(k1, k0 + max(pre, 0));
-    AttRow r;
-    r.pos = (int)pos;
-    r.lo = r.hi = r.plo = r.phi = 0;
-    if (lo < hi) {
-        if (ph >= lo) {
-            r.lo = (int)(ph > k0 ? k0 : lo);
-            r.hi = (int)max(hi, ph);
-        } else {
-            r.lo = (int)lo;
-            r.hi = (int)hi;
-            if (ph > k0) {
-                r.plo = (int)k0;
-                r.phi = (int)ph;
-            }
-        }
-    } else if (ph > k0) {
-        r.lo = (int)k0;
-        r.hi = (int)ph;
-    }
+    const int lo = p.back < 0 ? k0 : min(max(k0, r.pos - p.back), k1);
+    const int hi = p.ahead < 0 ? k1 : max(min(k1, r.pos + p.ahead + 1), k0);
+    const int ph = k0 + min(max(pre, 0), k1 - k0);
+    const bool join = ph >= lo;          // the prefix reaches the window
+    r.lo = join ? k0 : lo;
+    r.hi = join ? max(hi, ph) : hi;
+    r.plo = k0;
+    r.phi = ph;
     return r;
 }
-#define ATT_FAR 0x7fffffff
 
 // The exponent (base 2) of a score is mul * x + add, x being what the registers hold.  Plain: x = q.k, mul = scale log2(e).
 // Capped: cap tanh(y) = cap - 2 cap / (1 + e^2y), so x = 1 / (1 + e^2y) and the last product is the exponent's own fma; the
 // largest score is the smallest x.  A slope adds slope * |i - j| to x, in x's unit.
-template <bool CAP>
+template <bool CAP, bool SLOPES>
 struct AttScore {
     float mul, add, slope, in;
     static constexpr float HIDDEN = CAP ? INFINITY : -INFINITY;
@@ -128,7 +115,7 @@ struct AttScore {
         mul = CAP ? -2.0f * p.cap_out : p.scale2;
         add = CAP ? p.cap_out : 0.0f;
         in = p.cap_in;
-        slope = p.a.slopes != nullptr ? -p.a.slopes[head] * 1.4426950408889634f / mul : 0.0f;
+        slope = SLOPES ? -p.a.slopes[head] * 1.4426950408889634f / mul : 0.0f;
     }
     __device__ __forceinline__ float capped(float x) const { return __builtin_amdgcn_rcpf(1.0f + att_exp2(x * in)); }
     __device__ __forceinline__ float larger(float a, float b) const { return CAP ? fminf(a, b) : fmaxf(a, b); }
@@ -169,7 +156,7 @@ __device__ __forceinline__ int att_v_slot(int row, int chunk) {
     return D == 128 ? chunk ^ ((row & 3) << 2) : D == 64 ? chunk ^ (((row >> 1) & 1) << 2) : chunk;
 }
 
-template <typename T, int D, int NW, bool CAP>
+template <typename T, int D, int NW, bool CAP, bool SLOPES>
 __global__ __launch_bounds__(NW * 64, 2) void attention_kernel(AttArgs p) {
     typedef AttType<T> X;
     typedef typename X::vec8 vec8;
@@ -179,7 +166,7 @@ __global__ __launch_bounds__(NW * 64, 2) void attention_kernel(AttArgs p) {
     constexpr int CH = TILE / 16;               // 16-byte pieces of a tile
     constexpr int NLD = (CH + NT - 1) / NT;
     extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
-    __shared__ int range[NW][4];
+    __shared__ int flag;                        // some wave's result holds a NaN
     const unsigned lds = (unsigned)(size_t)(LDSP(unsigned char))smem;
     const mibc_attention_args &a = p.a;
     const int tid = threadIdx.x, lane = tid & 63;
@@ -187,68 +174,67 @@ __global__ __launch_bounds__(NW * 64, 2) void attention_kernel(AttArgs p) {
     const int half = lane >> 5;
 
     // workgroup -> (split, tile, pair)
-    unsigned id = blockIdx.x;
+    const unsigned id = blockIdx.x;
     int pair, tile, split;
     if (p.order == 0) {
-        pair = id % p.pairs;
-        id /= p.pairs;
-        split = id % p.splits;
-        tile = p.tiles - 1 - (int)(id / p.splits);      // causal: the long tiles start first
+        const unsigned rest = p.by_pairs.div(id);
+        pair = id - rest * p.pairs;
+        const unsigned z = p.by_splits.div(rest);
+        split = rest - z * p.splits;
+        tile = p.tiles - 1 - (int)z;                    // causal: the long tiles start first
     } else {
-        const int xcd = id & 7;
-        id >>= 3;
-        split = id % p.splits;
-        id /= p.splits;
-        tile = id % p.tiles;
-        pair = (int)(id / p.tiles) * 8 + xcd;
+        const unsigned rest = id >> 3, y = p.by_splits.div(rest), z = p.by_tiles.div(y);
+        split = rest - y * p.splits;
+        tile = y - z * p.tiles;
+        pair = z * 8 + (id & 7);
     }
-    const int b = pair / a.kv_heads, kvh = pair - b * a.kv_heads;
+    const int b = p.by_kv.div(pair), kvh = pair - b * a.kv_heads;
 
-    const int row = tile * (32 * NW) + wave * 32 + (lane & 31);
+    // lanes 32 and 33 look at the workgroup's first and last row instead of their own
+    constexpr int ROWS = 32 * NW;
+    const int row = tile * ROWS + wave * 32 + (lane & 31);
     const bool valid = row < p.rows;
-    const int rr = valid ? row : p.rows - 1;
-    const int t = rr / p.group, head = kvh * p.group + (rr - t * p.group);
-    const AttRow see = att_row(a, b, t);
-    const bool some = see.lo < see.hi, apart = see.plo < see.phi;
-    // the wave's rows together: outside [lo_min, hi_max) no row sees a key, inside [lo_max, hi_min) every row sees it
-    const int lo_min = att_wave_min(some ? see.lo : ATT_FAR), hi_max = att_wave_max(some ? see.hi : 0);
-    const int lo_max = att_wave_max(some ? see.lo : ATT_FAR), hi_min = att_wave_min(some ? see.hi : 0);
-    const int plo_min = att_wave_min(apart ? see.plo : ATT_FAR), phi_max = att_wave_max(apart ? see.phi : 0);
-    const bool tail_apart = phi_max > 0;     // some row's prefix does not join on to its window
-    if (lane == 0) {
-        range[wave][0] = lo_min;
-        range[wave][1] = hi_max;
-        range[wave][2] = plo_min;
-        range[wave][3] = phi_max;
+    const int rr = min(row, p.rows - 1), t = p.by_group.div(rr), head = kvh * p.group + (rr - t * p.group);
+    const int t_first = p.by_group.div(tile * ROWS), t_last = p.by_group.div(min(tile * ROWS + ROWS, p.rows) - 1);
+    const int tt = lane == 32 ? t_first : lane == 33 ? t_last : t;
+    int borders = 0;
+    if (a.doc_offsets != nullptr) {
+        const int n = a.n_docs + 1, w_first = __builtin_amdgcn_readfirstlane(t), w_last = __builtin_amdgcn_readlane(t, 31);
+        borders = att_borders(a.doc_offsets, n, w_first, lane);
+        for (int i = borders; i < n; ++i) {             // a few borders at most lie between a wave's rows
+            const int at = a.doc_offsets[i];
+            if (at > w_last) break;
+            if (lane < 32 && at <= t) ++borders;
+        }
+        const int f = att_borders(a.doc_offsets, n, t_first, lane), g = att_borders(a.doc_offsets, n, t_last, lane);
+        borders = lane == 32 ? f : lane == 33 ? g : borders;
     }
-    vec8 qf[D / 16];
-    {
-        const T *q = (const T *)a.q + b * a.q_stride[0] + t * a.q_stride[1] + head * a.q_stride[2] + 8 * half;
-#pragma unroll
-        for (int ks = 0; ks < D / 16; ++ks) qf[ks] = *(const vec8 *)(q + 16 * ks);
-    }
-    __syncthreads();
-    int w0 = ATT_FAR, w1 = 0, p0 = ATT_FAR, p1 = 0;
-#pragma unroll
-    for (int i = 0; i < NW; ++i) {
-        w0 = min(w0, range[i][0]);
-        w1 = max(w1, range[i][1]);
-        p0 = min(p0, range[i][2]);
-        p1 = max(p1, range[i][3]);
-    }
-    w0 = __builtin_amdgcn_readfirstlane(w0);
-    w1 = __builtin_amdgcn_readfirstlane(w1);
-    p0 = __builtin_amdgcn_readfirstlane(p0);
-    p1 = __builtin_amdgcn_readfirstlane(p1);
+    AttRow see = att_row(p, b, tt, borders);
+    int w0 = __builtin_amdgcn_readlane(see.lo, 32), w1 = __builtin_amdgcn_readlane(see.hi, 33);
+    int p0 = __builtin_amdgcn_readlane(see.plo, 32), p1 = __builtin_amdgcn_readlane(see.phi, 33);
+    const bool apart = a.prefix != nullptr && p.back >= 0;
     // tiles of the prefix, then of the window; one range where their tiles would overlap
-    int np = p0 < p1 ? (p1 - p0 + 63) >> 6 : 0;
+    int np = apart && p0 < p1 ? (p1 - p0 + 63) >> 6 : 0;
     if (np > 0 && p0 + 64 * np > w0) {
         w0 = min(w0, p0);
         w1 = max(w1, p1);
         np = 0;
     }
     const int ntiles = np + (w0 < w1 ? (w1 - w0 + 63) >> 6 : 0);
-    const int it0 = (int)((int64_t)ntiles * split / p.splits), it1 = (int)((int64_t)ntiles * (split + 1) / p.splits);
+    int it0 = 0, it1 = ntiles;
+    if (p.splits > 1) {
+        it0 = (int)p.by_splits.div((unsigned)ntiles * split);      // ntiles * splits < 2^31
+        it1 = (int)p.by_splits.div((unsigned)ntiles * (split + 1));
+    }
+    // the wave's rows: outside [lo_min, hi_max) no row sees a key, inside [lo_max, hi_min) every row sees it
+    see.lo = att_low_half(see.lo);
+    see.hi = att_low_half(see.hi);
+    see.plo = att_low_half(see.plo);
+    see.phi = att_low_half(see.phi);
+    see.pos = att_low_half(see.pos);
+    const int lo_min = __builtin_amdgcn_readfirstlane(see.lo), lo_max = __builtin_amdgcn_readlane(see.lo, 31);
+    const int hi_min = __builtin_amdgcn_readfirstlane(see.hi), hi_max = __builtin_amdgcn_readlane(see.hi, 31);
+    const int plo_min = __builtin_amdgcn_readfirstlane(see.plo), phi_max = apart ? __builtin_amdgcn_readlane(see.phi, 31) : 0;
 
     // pieces of a tile this thread moves: LDS order is linear in the thread, the swizzle permutes what is fetched
     const att_gptr kb = (att_gptr)a.k + (b * a.k_stride[0] + kvh * a.k_stride[2]) * 2;
@@ -284,6 +270,14 @@ __global__ __launch_bounds__(NW * 64, 2) void attention_kernel(AttArgs p) {
         }
     };
 
+    if (it0 < it1) fetch(it0, 0);
+    if (tid == 0) flag = 0;
+    vec8 qf[D / 16];
+    {
+        const T *q = (const T *)a.q + b * a.q_stride[0] + t * a.q_stride[1] + head * a.q_stride[2] + 8 * half;
+#pragma unroll
+        for (int ks = 0; ks < D / 16; ++ks) qf[ks] = *(const vec8 *)(q + 16 * ks);
+    }
     // fragment addresses of this lane
     unsigned kaddr[D / 16], vaddr[D / 32];
 #pragma unroll
@@ -293,8 +287,7 @@ __global__ __launch_bounds__(NW * 64, 2) void attention_kernel(AttArgs p) {
         const int r = 4 * half + ((lane >> 2) & 3);
         vaddr[db] = lds + TILE + r * PITCH + att_v_slot<D>(r, 4 * db + 2 * ((lane >> 4) & 1) + ((lane >> 1) & 1)) * 16 + (lane & 1) * 8;
     }
-    const AttScore<CAP> score(p, head);
-    const bool slopes = a.slopes != nullptr;
+    const AttScore<CAP, SLOPES> score(p, head);
 
     float16_t o[D / 32];
     float m, l;
@@ -304,7 +297,7 @@ __global__ __launch_bounds__(NW * 64, 2) void attention_kernel(AttArgs p) {
         for (int db = 0; db < D / 32; ++db) o[db] = (float16_t)(0.0f);
         m = -INFINITY;
         l = 0.0f;
-        if (it0 < it1) fetch(it0, 0);
+        if (SAFE && it0 < it1) fetch(it0, 0);
         for (int it = it0; it < it1; ++it) {
             const int stage = (it - it0) & 1;
             asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
@@ -329,7 +322,7 @@ __global__ __launch_bounds__(NW * 64, 2) void attention_kernel(AttArgs p) {
 #pragma unroll
                     for (int r = 0; r < 16; ++r) s[i][r] = score.capped(s[i][r]);
             }
-            if (slopes) {
+            if (SLOPES) {
                 const float away = (float)(see.pos - j0 - 4 * half);
 #pragma unroll
                 for (int i = 0; i < 2; ++i)
@@ -340,7 +333,7 @@ __global__ __launch_bounds__(NW * 64, 2) void attention_kernel(AttArgs p) {
             if (!full) {
                 // element e = 32 i + (r & 3) + 8 (r >> 2) of the tile is key j0 + 4 half + e
                 const int at0 = j0 + 4 * half, lo = see.lo - at0, hi = see.hi - at0;
-                if (SAFE || tail_apart) {
+                if (SAFE || apart) {
                     const int plo = see.plo - at0, phi = see.phi - at0;
                     seen = 0;
 #pragma unroll
@@ -453,7 +446,9 @@ __global__ __launch_bounds__(NW * 64, 2) void attention_kernel(AttArgs p) {
 #pragma unroll
         for (int r = 0; r < 16; ++r) odd = odd || o[db][r] != o[db][r];
     // a NaN: from a value or key that the row sees, or 0 * (a value that it does not see); the second pass tells them apart
-    if (__syncthreads_or(odd)) pass(std::true_type());
+    if (__any(odd) && lane == 0) flag = 1;
+    __syncthreads();
+    if (flag) pass(std::true_type());
 
     l = att_half_add(l);
     const float base = m == -INFINITY ? 0.0f : m;
@@ -494,7 +489,7 @@ __device__ __forceinline__ int att_v_slot16(int row, int chunk) {
     return D == 128 ? chunk ^ (((row & 3) << 2) | ((row & 4) >> 1)) : D == 64 ? chunk ^ ((((row >> 1) & 1) << 2) | ((row & 4) >> 1)) : chunk;
 }
 
-template <typename T, int D, bool CAP>
+template <typename T, int D, bool CAP, bool SLOPES>
 __global__ __launch_bounds__(256, 2) void attention_token_kernel(AttArgs p) {
     typedef AttType<T> X;
     typedef typename X::vec8 vec8;
@@ -508,24 +503,28 @@ __global__ __launch_bounds__(256, 2) void attention_token_kernel(AttArgs p) {
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int l15 = lane & 15, quarter = lane >> 4;
-    const int pair = blockIdx.x % p.pairs, split = blockIdx.x / p.pairs;
-    const int b = pair / a.kv_heads, kvh = pair - b * a.kv_heads;
+    const int split = p.by_pairs.div(blockIdx.x), pair = blockIdx.x - split * p.pairs;
+    const int b = p.by_kv.div(pair), kvh = pair - b * a.kv_heads;
 
-    const int rr = min(l15, p.rows - 1);
-    const int t = rr / p.group, head = kvh * p.group + (rr - t * p.group);
-    const AttRow see = att_row(a, b, t);
-    const bool some = see.lo < see.hi, apart = see.plo < see.phi;
-    int w0 = att_wave_min(some ? see.lo : ATT_FAR), w1 = att_wave_max(some ? see.hi : 0);
-    const int lo_max = att_wave_max(some ? see.lo : ATT_FAR), hi_min = att_wave_min(some ? see.hi : 0);
-    const int p0 = att_wave_min(apart ? see.plo : ATT_FAR), p1 = att_wave_max(apart ? see.phi : 0);
-    int np = p0 < p1 ? (p1 - p0 + 31) >> 5 : 0;
+    const int rr = min(l15, p.rows - 1), t = p.by_group.div(rr), head = kvh * p.group + (rr - t * p.group);
+    int borders = 0;
+    if (a.doc_offsets != nullptr)
+        for (int i = 0; i < a.n_docs + 1 && a.doc_offsets[i] < a.q_tokens; ++i) borders += a.doc_offsets[i] <= t;   // at most 16 tokens
+    const AttRow see = att_row(p, b, t, borders);
+    // rows grow with the lane up to the last, which lane 15 repeats
+    const int lo_min = __builtin_amdgcn_readfirstlane(see.lo), lo_max = __builtin_amdgcn_readlane(see.lo, 15);
+    const int hi_min = __builtin_amdgcn_readfirstlane(see.hi), hi_max = __builtin_amdgcn_readlane(see.hi, 15);
+    const int p0 = __builtin_amdgcn_readfirstlane(see.plo), p1 = __builtin_amdgcn_readlane(see.phi, 15);
+    const bool apart = a.prefix != nullptr && p.back >= 0;
+    int w0 = lo_min, w1 = hi_max, np = apart && p0 < p1 ? (p1 - p0 + 31) >> 5 : 0;
     if (np > 0 && p0 + 32 * np > w0) {
         w0 = min(w0, p0);
         w1 = max(w1, p1);
         np = 0;
     }
     const int steps = np + (w0 < w1 ? (w1 - w0 + 31) >> 5 : 0);
-    const int it0 = (int)((int64_t)steps * split / p.splits) + wave, it1 = (int)((int64_t)steps * (split + 1) / p.splits);
+    const int it0 = (int)p.by_splits.div((unsigned)steps * split) + wave;      // steps * splits < 2^31
+    const int it1 = (int)p.by_splits.div((unsigned)steps * (split + 1));
 
     vec8 qf[NK];
     {
@@ -559,8 +558,7 @@ __global__ __launch_bounds__(256, 2) void attention_token_kernel(AttArgs p) {
         const int r = 4 * quarter + (l15 >> 2);
         vaddr[db] = mine + r * PITCH + att_v_slot16<D>(r, 2 * db + ((lane >> 1) & 1)) * 16 + (lane & 1) * 8;
     }
-    const AttScore<CAP> score(p, head);
-    const bool slopes = a.slopes != nullptr;
+    const AttScore<CAP, SLOPES> score(p, head);
 
     float4_t o[D / 16];
     float m, l;
@@ -590,7 +588,7 @@ __global__ __launch_bounds__(256, 2) void attention_token_kernel(AttArgs p) {
 #pragma unroll
                     for (int r = 0; r < 4; ++r) s[i][r] = score.capped(s[i][r]);
             }
-            if (slopes) {
+            if (SLOPES) {
                 const float away = (float)(see.pos - j0 - 4 * quarter);
 #pragma unroll
                 for (int i = 0; i < 2; ++i)
@@ -713,7 +711,7 @@ __global__ __launch_bounds__(256, 2) void attention_token_kernel(AttArgs p) {
             for (int e = 0; e < 4; ++e) y[e] = fmaf(f, x[e], y[e]);
         }
         const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-        const int rt = r / p.group, rh = kvh * p.group + (r - rt * p.group);
+        const int rt = p.by_group.div(r), rh = kvh * p.group + (r - rt * p.group);
         if (p.splits > 1) {
             const int64_t at = ((int64_t)pair * p.rows + r) * p.splits + split;
             *(floatx4 *)(p.part_o + at * D + d4) = (floatx4){y[0] * inv, y[1] * inv, y[2] * inv, y[3] * inv};
@@ -738,8 +736,8 @@ __global__ __launch_bounds__(256) void attention_join_kernel(AttArgs p) {
     const int tid = threadIdx.x;
     const int64_t r = blockIdx.x;
     const int pair = (int)(r / p.rows), row = (int)(r - (int64_t)pair * p.rows);
-    const int b = pair / a.kv_heads, kvh = pair - b * a.kv_heads;
-    const int t = row / p.group, head = kvh * p.group + (row - t * p.group);
+    const int b = p.by_kv.div(pair), kvh = pair - b * a.kv_heads;
+    const int t = p.by_group.div(row), head = kvh * p.group + (row - t * p.group);
     const float *pl = p.part_l + r * p.splits;
     const float *po = p.part_o + r * p.splits * D;
     float m = -INFINITY;
@@ -778,34 +776,23 @@ __global__ __launch_bounds__(256) void attention_join_kernel(AttArgs p) {
     }
 }
 
-template <typename T, int NW>
-static void att_rows(hipStream_t s, const AttArgs &p, unsigned grid) {
-    constexpr int LDS = 4 * 64 * ATT_D * 2;
-    if (p.cap_out > 0.0f) {
-        MIBC_LDS_ATTR_ONCE((attention_kernel<T, ATT_D, NW, true>), LDS);
-        hipLaunchKernelGGL((attention_kernel<T, ATT_D, NW, true>), dim3(grid), dim3(NW * 64), LDS, s, p);
-    } else {
-        MIBC_LDS_ATTR_ONCE((attention_kernel<T, ATT_D, NW, false>), LDS);
-        hipLaunchKernelGGL((attention_kernel<T, ATT_D, NW, false>), dim3(grid), dim3(NW * 64), LDS, s, p);
-    }
-}
-template <typename T>
-static void att_token(hipStream_t s, const AttArgs &p, unsigned grid) {
-    constexpr int FETCH = 4 * 2 * 32 * ATT_D * 2, JOIN = 4 * 16 * (ATT_D + 4 + 2) * 4, LDS = FETCH > JOIN ? FETCH : JOIN;
-    if (p.cap_out > 0.0f) {
-        MIBC_LDS_ATTR_ONCE((attention_token_kernel<T, ATT_D, true>), LDS);
-        hipLaunchKernelGGL((attention_token_kernel<T, ATT_D, true>), dim3(grid), dim3(256), LDS, s, p);
-    } else {
-        MIBC_LDS_ATTR_ONCE((attention_token_kernel<T, ATT_D, false>), LDS);
-        hipLaunchKernelGGL((attention_token_kernel<T, ATT_D, false>), dim3(grid), dim3(256), LDS, s, p);
-    }
+template <typename T, bool CAP, bool SLOPES>
+static void att_one(hipStream_t s, const AttArgs &p, int variant, unsigned grid) {
+    constexpr int ROWS = 4 * 64 * ATT_D * 2, STEPS = 4 * 2 * 32 * ATT_D * 2, JOIN = 4 * 16 * (ATT_D + 4 + 2) * 4, TOKEN = STEPS > JOIN ? STEPS : JOIN;
+#define ATT_GO(KERNEL, THREADS, LDS)                                                    \
+    do {                                                                                \
+        MIBC_LDS_ATTR_ONCE(KERNEL, LDS);                                                \
+        hipLaunchKernelGGL(KERNEL, dim3(grid), dim3(THREADS), LDS, s, p);               \
+    } while (0)
+    if (variant == ATT_TOKENS) ATT_GO((attention_token_kernel<T, ATT_D, CAP, SLOPES>), 256, TOKEN);
+    else if (variant == ATT_ROWS_128) ATT_GO((attention_kernel<T, ATT_D, 4, CAP, SLOPES>), 256, ROWS);
+    else ATT_GO((attention_kernel<T, ATT_D, 2, CAP, SLOPES>), 128, ROWS);
+#undef ATT_GO
 }
 template <typename T>
 static int att_launch(hipStream_t s, const AttArgs &p, int variant, unsigned grid) {
-    if (variant == 3) att_token<T>(s, p, grid);
-    else if (variant == 0) att_rows<T, 8>(s, p, grid);
-    else if (variant == 1) att_rows<T, 4>(s, p, grid);
-    else att_rows<T, 2>(s, p, grid);
+    if (p.cap_out > 0.0f) p.a.slopes ? att_one<T, true, true>(s, p, variant, grid) : att_one<T, true, false>(s, p, variant, grid);
+    else p.a.slopes ? att_one<T, false, true>(s, p, variant, grid) : att_one<T, false, false>(s, p, variant, grid);
     int rc = op_hip(hipGetLastError(), "attention");
     if (rc != MIBC_OK || p.splits == 1) return rc;
     hipLaunchKernelGGL((attention_join_kernel<T, ATT_D>), dim3((unsigned)((int64_t)p.pairs * p.rows)), dim3(256), 0, s, p);

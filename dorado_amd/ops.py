@@ -243,8 +243,8 @@ def attention(q, k, v, *, scale=None, causal: bool = False, window=(-1, -1), sof
     offs = _index32("attention", "doc_offsets", doc_offsets, docs + 1)
     if q_start is None:
         q_start = ATTN_END
-    elif not -(1 << 30) <= q_start <= 1 << 30:
-        raise MibcNotSupported("attention: q_start beyond 2^30")
+    elif not -(1 << 28) <= q_start <= 1 << 28:
+        raise MibcNotSupported("attention: q_start beyond 2^28")
     limits = [max(-1, min(int(w), (1 << 31) - 1)) for w in window]
     lse = torch.empty((b, h, n), dtype=torch.float32, device=q.device) if return_lse else None
 
