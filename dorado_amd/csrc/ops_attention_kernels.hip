@@ -42,6 +42,8 @@ __device__ __forceinline__ V8 att_lds16(unsigned addr) {
 __device__ __forceinline__ uintx2 att_lds_tr(unsigned addr) {
     return __builtin_bit_cast(uintx2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((LDSP(short4_att))(size_t)addr));
 }
+#define ATT_FENCE() __builtin_amdgcn_sched_barrier(0)     // the compiler moves nothing across
+
 __device__ __forceinline__ float att_exp2(float x) { return __builtin_amdgcn_exp2f(x); }
 // over the two half waves
 __device__ __forceinline__ float att_half_max(float x) {
@@ -157,7 +159,7 @@ __device__ __forceinline__ int att_v_slot(int row, int chunk) {
 }
 
 template <typename T, int D, int NW, bool CAP, bool SLOPES>
-__global__ __launch_bounds__(NW * 64, 2) void attention_kernel(AttArgs p) {
+__global__ __launch_bounds__(NW * 64, D <= 64 ? 3 : 2) void attention_kernel(AttArgs p) {
     typedef AttType<T> X;
     typedef typename X::vec8 vec8;
     constexpr int NT = NW * 64;
@@ -193,7 +195,6 @@ __global__ __launch_bounds__(NW * 64, 2) void attention_kernel(AttArgs p) {
     // lanes 32 and 33 look at the workgroup's first and last row instead of their own
     constexpr int ROWS = 32 * NW;
     const int row = tile * ROWS + wave * 32 + (lane & 31);
-    const bool valid = row < p.rows;
     const int rr = min(row, p.rows - 1), t = p.by_group.div(rr), head = kvh * p.group + (rr - t * p.group);
     const int t_first = p.by_group.div(tile * ROWS), t_last = p.by_group.div(min(tile * ROWS + ROWS, p.rows) - 1);
     const int tt = lane == 32 ? t_first : lane == 33 ? t_last : t;
@@ -236,13 +237,15 @@ __global__ __launch_bounds__(NW * 64, 2) void attention_kernel(AttArgs p) {
     const int hi_min = __builtin_amdgcn_readfirstlane(see.hi), hi_max = __builtin_amdgcn_readlane(see.hi, 31);
     const int plo_min = __builtin_amdgcn_readfirstlane(see.plo), phi_max = apart ? __builtin_amdgcn_readlane(see.phi, 31) : 0;
 
-    // pieces of a tile this thread moves: LDS order is linear in the thread, the swizzle permutes what is fetched
+    // pieces of a tile this thread moves: LDS order is linear in the thread, the swizzle permutes what is fetched.  Where the
+    // rows that all threads move at once are whole periods of the swizzle, the pieces of a thread differ by the row alone
+    constexpr bool EVEN = NT % (D / 8) == 0 && NT / (D / 8) % 16 == 0;
     const att_gptr kb = (att_gptr)a.k + (b * a.k_stride[0] + kvh * a.k_stride[2]) * 2;
     const att_gptr vb = (att_gptr)a.v + (b * a.v_stride[0] + kvh * a.v_stride[2]) * 2;
     const unsigned krow = (unsigned)a.k_stride[1] * 2, vrow = (unsigned)a.v_stride[1] * 2;
-    unsigned koff[NLD], voff[NLD];
+    unsigned koff[EVEN ? 1 : NLD], voff[EVEN ? 1 : NLD];
 #pragma unroll
-    for (int i = 0; i < NLD; ++i) {
+    for (int i = 0; i < (EVEN ? 1 : NLD); ++i) {
         const int c = i * NT + tid, r = c / (D / 8), s = c % (D / 8);
         koff[i] = r * krow + att_k_slot<D>(r, s) * 16;
         voff[i] = r * vrow + att_v_slot<D>(r, s) * 16;
@@ -252,22 +255,20 @@ __global__ __launch_bounds__(NW * 64, 2) void attention_kernel(AttArgs p) {
         const int j0 = first_key(it), left = (it < np ? p1 : w1) - j0;
         const att_gptr kt = kb + (int64_t)j0 * krow, vt = vb + (int64_t)j0 * vrow;
         const unsigned to = lds + stage * (2 * TILE) + wave * 1024;
-        if (left >= 64) {
 #pragma unroll
-            for (int i = 0; i < NLD; ++i)
-                if (i * NT + wave * 64 < CH) {
-                    att_dma16(kt, koff[i], to + i * (NT * 16));
-                    att_dma16(vt, voff[i], to + i * (NT * 16) + TILE);
-                }
-        } else {   // rows behind the last key repeat it: nobody sees them
-#pragma unroll
-            for (int i = 0; i < NLD; ++i)
-                if (i * NT + wave * 64 < CH) {
+        for (int i = 0; i < NLD; ++i)
+            if (i * NT + wave * 64 < CH) {
+                const unsigned at = to + i * (NT * 16);
+                if (left >= 64) {
+                    const int more = EVEN ? i * (NT / (D / 8)) : 0;
+                    att_dma16(kt + (int64_t)more * krow, koff[EVEN ? 0 : i], at);
+                    att_dma16(vt + (int64_t)more * vrow, voff[EVEN ? 0 : i], at + TILE);
+                } else {   // rows behind the last key repeat it: nobody sees them
                     const int c = i * NT + tid, r = c / (D / 8), s = c % (D / 8), rc = min(r, left - 1);
-                    att_dma16(kt, rc * krow + att_k_slot<D>(r, s) * 16, to + i * (NT * 16));
-                    att_dma16(vt, rc * vrow + att_v_slot<D>(r, s) * 16, to + i * (NT * 16) + TILE);
+                    att_dma16(kt, rc * krow + att_k_slot<D>(r, s) * 16, at);
+                    att_dma16(vt, rc * vrow + att_v_slot<D>(r, s) * 16, at + TILE);
                 }
-        }
+            }
     };
 
     if (it0 < it1) fetch(it0, 0);
@@ -278,7 +279,7 @@ __global__ __launch_bounds__(NW * 64, 2) void attention_kernel(AttArgs p) {
 #pragma unroll
         for (int ks = 0; ks < D / 16; ++ks) qf[ks] = *(const vec8 *)(q + 16 * ks);
     }
-    // fragment addresses of this lane
+    // fragment addresses of this lane in stage 0
     unsigned kaddr[D / 16], vaddr[D / 32];
 #pragma unroll
     for (int ks = 0; ks < D / 16; ++ks) kaddr[ks] = lds + (lane & 31) * PITCH + att_k_slot<D>(lane & 31, 2 * ks + half) * 16;
@@ -289,191 +290,223 @@ __global__ __launch_bounds__(NW * 64, 2) void attention_kernel(AttArgs p) {
     }
     const AttScore<CAP, SLOPES> score(p, head);
 
-    float16_t o[D / 32];
+    float16_t o[D / 32], s[2];
     float m, l;
-    auto pass = [&](auto safe_) {
-        constexpr bool SAFE = decltype(safe_)::value;
+    auto start = [&]() {
 #pragma unroll
         for (int db = 0; db < D / 32; ++db) o[db] = (float16_t)(0.0f);
         m = -INFINITY;
         l = 0.0f;
-        if (SAFE && it0 < it1) fetch(it0, 0);
-        for (int it = it0; it < it1; ++it) {
-            const int stage = (it - it0) & 1;
-            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-            __builtin_amdgcn_s_barrier();
-            if (it + 1 < it1) fetch(it + 1, stage ^ 1);
-            const int j0 = first_key(it);
-            if ((j0 >= hi_max || j0 + 64 <= lo_min) && (j0 >= phi_max || j0 + 64 <= plo_min)) continue;   // no row of the wave
-            const bool full = !SAFE && j0 >= lo_max && j0 + 64 <= hi_min;
-            const unsigned at = stage * (2 * TILE);
-
-            float16_t s[2];
-            s[0] = (float16_t)(0.0f);
-            s[1] = (float16_t)(0.0f);
+    };
+    // operands are read four instructions ahead of their use (the fences keep the compiler from moving reads down to it)
+    auto products = [&](unsigned at) {
+        constexpr int N = D / 8;
+        auto key = [&](int i) { return att_lds16<vec8>(kaddr[i >> 1] + (at + (i & 1) * (32 * PITCH))); };
+        vec8 kf[4];
+        s[0] = s[1] = (float16_t)(0.0f);
 #pragma unroll
-            for (int ks = 0; ks < D / 16; ++ks)
+        for (int i = 0; i < 4; ++i) kf[i] = key(i);
+        ATT_FENCE();
 #pragma unroll
-                for (int i = 0; i < 2; ++i)
-                    s[i] = X::mfma32(att_lds16<vec8>(kaddr[ks] + at + i * (32 * PITCH)), qf[ks], s[i]);
-            if (CAP) {
-#pragma unroll
-                for (int i = 0; i < 2; ++i)
-#pragma unroll
-                    for (int r = 0; r < 16; ++r) s[i][r] = score.capped(s[i][r]);
+        for (int i = 0; i < N; ++i) {
+            s[i & 1] = X::mfma32(kf[i & 3], qf[i >> 1], s[i & 1]);
+            if (i + 4 < N) kf[i & 3] = key(i + 4);
+            if (i & 1) ATT_FENCE();
+        }
+    };
+    // element e = 32 i + (r & 3) + 8 (r >> 2) of a tile is key j0 + 4 half + e
+#define ATT_EACH                             \
+    _Pragma("unroll") for (int i = 0; i < 2; ++i) \
+    _Pragma("unroll") for (int r = 0, e = 32 * i; r < 16; ++r, e = 32 * i + (r & 3) + 8 * (r >> 2))
+    auto shape = [&](int j0) {      // raw products -> what AttScore calls x
+        if (CAP) {
+            ATT_EACH s[i][r] = score.capped(s[i][r]);
+        }
+        if (SLOPES) {
+            const float away = (float)(see.pos - j0 - 4 * half);
+            ATT_EACH s[i][r] = fmaf(score.slope, fabsf(away - (float)e), s[i][r]);
+        }
+    };
+    // what a row does not see leaves its scores; returns the bits 16 i + r of what it sees
+    auto hide_all = [&](int j0) {
+        const int at0 = j0 + 4 * half, lo = see.lo - at0, hi = see.hi - at0, plo = apart ? see.plo - at0 : 0, phi = apart ? see.phi - at0 : 0;
+        unsigned seen = 0;
+        ATT_EACH {
+            const bool v = (e >= lo && e < hi) || (e >= plo && e < phi);
+            s[i][r] = v ? s[i][r] : score.HIDDEN;
+            seen |= v ? 1u << (16 * i + r) : 0u;
+        }
+        return seen;
+    };
+    auto hide = [&](int j0) {
+        const int at0 = j0 + 4 * half, lo = see.lo - at0, hi = see.hi - at0;
+        if (apart) {
+            (void)hide_all(j0);
+        } else {
+            if (j0 + 64 > hi_min) {
+                ATT_EACH s[i][r] = e < hi ? s[i][r] : score.HIDDEN;
             }
-            if (SLOPES) {
-                const float away = (float)(see.pos - j0 - 4 * half);
-#pragma unroll
-                for (int i = 0; i < 2; ++i)
-#pragma unroll
-                    for (int r = 0; r < 16; ++r) s[i][r] = fmaf(score.slope, fabsf(away - (float)(32 * i + (r & 3) + 8 * (r >> 2))), s[i][r]);
-            }
-            unsigned seen = 0xffffffffu;     // bit 16 i + r
-            if (!full) {
-                // element e = 32 i + (r & 3) + 8 (r >> 2) of the tile is key j0 + 4 half + e
-                const int at0 = j0 + 4 * half, lo = see.lo - at0, hi = see.hi - at0;
-                if (SAFE || apart) {
-                    const int plo = see.plo - at0, phi = see.phi - at0;
-                    seen = 0;
-#pragma unroll
-                    for (int i = 0; i < 2; ++i)
-#pragma unroll
-                        for (int r = 0; r < 16; ++r) {
-                            const int e = 32 * i + (r & 3) + 8 * (r >> 2);
-                            const bool v = (e >= lo && e < hi) || (e >= plo && e < phi);
-                            s[i][r] = v ? s[i][r] : score.HIDDEN;
-                            if (SAFE) seen |= v ? 1u << (16 * i + r) : 0u;
-                        }
-                } else {
-                    if (j0 + 64 > hi_min) {
-#pragma unroll
-                        for (int i = 0; i < 2; ++i)
-#pragma unroll
-                            for (int r = 0; r < 16; ++r) s[i][r] = 32 * i + (r & 3) + 8 * (r >> 2) < hi ? s[i][r] : score.HIDDEN;
-                    }
-                    if (j0 < lo_max) {
-#pragma unroll
-                        for (int i = 0; i < 2; ++i)
-#pragma unroll
-                            for (int r = 0; r < 16; ++r) s[i][r] = 32 * i + (r & 3) + 8 * (r >> 2) >= lo ? s[i][r] : score.HIDDEN;
-                    }
-                }
-            }
-            float top = s[0][0];
-#pragma unroll
-            for (int i = 0; i < 2; ++i)
-#pragma unroll
-                for (int r = 0; r < 16; ++r) top = score.larger(top, s[i][r]);
-            top = att_half_max(fmaf(top, score.mul, score.add));
-            // the maximum is only moved when it grew by more than 2^8: probabilities stay below 256, exact in f32 sums
-            if (__any(top > m + 8.0f)) {
-                const float mn = fmaxf(m, top);
-                const float f = m == -INFINITY ? 0.0f : att_exp2(m - mn);
-                m = mn;
-                l *= f;
-#pragma unroll
-                for (int db = 0; db < D / 32; ++db)
-#pragma unroll
-                    for (int r = 0; r < 16; ++r) o[db][r] *= f;
-            }
-            const float off = score.add - (m == -INFINITY ? 0.0f : m);
-            float add = 0.0f;
-            vec8 pf[4];
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                uintx4 pk[2];
-#pragma unroll
-                for (int r = 0; r < 16; r += 2) {
-                    const float x = att_exp2(fmaf(s[i][r], score.mul, off)), y = att_exp2(fmaf(s[i][r + 1], score.mul, off));
-                    add += x + y;
-                    pk[r >> 3][(r & 7) >> 1] = op_pack2(x, y, T());
-                }
-                pf[2 * i] = __builtin_bit_cast(vec8, pk[0]);
-                pf[2 * i + 1] = __builtin_bit_cast(vec8, pk[1]);
-            }
-            l += add;
-#pragma unroll
-            for (int db = 0; db < D / 32; ++db)
-#pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                    const uintx2 x = att_lds_tr(vaddr[db] + at + k * (16 * PITCH)), y = att_lds_tr(vaddr[db] + at + k * (16 * PITCH) + 8 * PITCH);
-                    uintx4 v = {x[0], x[1], y[0], y[1]};
-                    if (SAFE) {
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            if ((v[e] & X::EXPONENT) == X::EXPONENT) v[e] &= 0xffff0000u;
-                            if (((v[e] >> 16) & X::EXPONENT) == X::EXPONENT) v[e] &= 0x0000ffffu;
-                        }
-                    }
-                    o[db] = X::mfma32(__builtin_bit_cast(vec8, v), pf[k], o[db]);
-                }
-            if (SAFE) {
-                // values that are not finite reach the rows that see their key, and no other: 0 * NaN stays out of the product
-                // above, and the places of NaN (kind 0), infinity (1) and -infinity (2) are multiplied with the mask instead
-                vec8 vis[4];
-#pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                    uintx4 w;
-#pragma unroll
-                    for (int e = 0; e < 4; ++e)
-                        w[e] = ((seen >> (8 * k + 2 * e)) & 1 ? X::ONE : 0u) | ((seen >> (8 * k + 2 * e + 1)) & 1 ? X::ONE << 16 : 0u);
-                    vis[k] = __builtin_bit_cast(vec8, w);
-                }
-#pragma unroll 1
-                for (int kind = 0; kind < 3; ++kind)
-#pragma unroll
-                    for (int db = 0; db < D / 32; ++db) {
-                        float16_t hit = (float16_t)(0.0f);
-#pragma unroll
-                        for (int k = 0; k < 4; ++k) {
-                            const uintx2 x = att_lds_tr(vaddr[db] + at + k * (16 * PITCH)), y = att_lds_tr(vaddr[db] + at + k * (16 * PITCH) + 8 * PITCH);
-                            const uintx4 v = {x[0], x[1], y[0], y[1]};
-                            hit = X::mfma32(__builtin_bit_cast(vec8, att_places<T>(v, kind)), vis[k], hit);
-                        }
-                        const float what = kind == 0 ? NAN : kind == 1 ? INFINITY : -INFINITY;
-#pragma unroll
-                        for (int r = 0; r < 16; ++r)
-                            if (hit[r] > 0.0f) o[db][r] += what;
-                    }
+            if (j0 < lo_max) {
+                ATT_EACH s[i][r] = e >= lo ? s[i][r] : score.HIDDEN;
             }
         }
     };
-    pass(std::false_type());
+    float off;
+    auto maxima = [&]() {
+        float top = s[0][0];
+        ATT_EACH top = score.larger(top, s[i][r]);
+        top = att_half_max(fmaf(top, score.mul, score.add));
+        // the maximum is only moved when it grew by more than 2^8: probabilities stay below 256, which 16 bits and f32 sums
+        // hold as well as values below 1
+        if (__any(top > m + 8.0f)) {
+            const float mn = fmaxf(m, top);
+            const float f = m == -INFINITY ? 0.0f : att_exp2(m - mn);
+            m = mn;
+            l *= f;
+#pragma unroll
+            for (int db = 0; db < D / 32; ++db)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) o[db][r] *= f;
+        }
+        off = score.add - (m == -INFINITY ? 0.0f : m);
+    };
+    auto probabilities = [&](int k) {       // of 16 keys
+        uintx4 w;
+        float sum = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const float x = att_exp2(fmaf(s[k >> 1][8 * (k & 1) + 2 * i], score.mul, off));
+            const float y = att_exp2(fmaf(s[k >> 1][8 * (k & 1) + 2 * i + 1], score.mul, off));
+            sum += x + y;                   // before the rounding: the sum is also a result
+            w[i] = op_pack2(x, y, T());
+        }
+        l += sum;
+        return __builtin_bit_cast(vec8, w);
+    };
+    auto values = [&](unsigned at, int db, int k) {      // V^T operand: 32 dims x 16 keys
+        const uintx2 x = att_lds_tr(vaddr[db] + (at + k * (16 * PITCH))), y = att_lds_tr(vaddr[db] + (at + k * (16 * PITCH) + 8 * PITCH));
+        return (uintx4){x[0], x[1], y[0], y[1]};
+    };
+    auto step = [&](auto stage_, int it) {
+        constexpr unsigned AT = decltype(stage_)::value * (2 * TILE);
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        __builtin_amdgcn_s_barrier();
+        if (it + 1 < it1) fetch(it + 1, decltype(stage_)::value ^ 1);
+        const int j0 = first_key(it);
+        if ((j0 >= hi_max || j0 + 64 <= lo_min) && (j0 >= phi_max || j0 + 64 <= plo_min)) return;   // no row of the wave
+        products(AT);
+        shape(j0);
+        if (j0 < lo_max || j0 + 64 > hi_min) hide(j0);
+        maxima();
+        // the products of 16 keys run beside the probabilities of the next 16, whose values are read meanwhile
+        constexpr int N = D / 32;
+        uintx4 v[2][N];
+#pragma unroll
+        for (int db = 0; db < N; ++db) v[0][db] = values(AT, db, 0);
+        vec8 pf[2];
+        pf[0] = probabilities(0);
+        ATT_FENCE();
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            if (k < 3) {
+#pragma unroll
+                for (int db = 0; db < N; ++db) v[(k + 1) & 1][db] = values(AT, db, k + 1);
+                pf[(k + 1) & 1] = probabilities(k + 1);
+            }
+#pragma unroll
+            for (int db = 0; db < N; ++db) o[db] = X::mfma32(__builtin_bit_cast(vec8, v[k & 1][db]), pf[k & 1], o[db]);
+            ATT_FENCE();
+        }
+    };
+    start();
+    for (int it = it0; it < it1; it += 2) {
+        step(std::integral_constant<int, 0>(), it);
+        if (it + 1 < it1) step(std::integral_constant<int, 1>(), it + 1);
+    }
     bool odd = false;
 #pragma unroll
     for (int db = 0; db < D / 32; ++db)
 #pragma unroll
         for (int r = 0; r < 16; ++r) odd = odd || o[db][r] != o[db][r];
-    // a NaN: from a value or key that the row sees, or 0 * (a value that it does not see); the second pass tells them apart
     if (__any(odd) && lane == 0) flag = 1;
     __syncthreads();
-    if (flag) pass(std::true_type());
+    if (flag) {
+        // a NaN: from a value or key that the row sees, or 0 * (a value that it does not see).  Once more, tile by tile: values
+        // that are not finite stay out of the products, and the places of NaN (kind 0), infinity (1) and -infinity (2) are
+        // multiplied with the mask instead, so that they reach the rows that see their key and no other
+        start();
+#pragma unroll 1
+        for (int it = it0; it < it1; ++it) {
+            __syncthreads();
+            fetch(it, 0);
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+            __syncthreads();
+            const int j0 = first_key(it);
+            products(0);
+            shape(j0);
+            const unsigned seen = hide_all(j0);
+            maxima();
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const vec8 pf = probabilities(k);
+                uintx4 w;
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    w[e] = ((seen >> (8 * k + 2 * e)) & 1 ? X::ONE : 0u) | ((seen >> (8 * k + 2 * e + 1)) & 1 ? X::ONE << 16 : 0u);
+                const vec8 vis = __builtin_bit_cast(vec8, w);
+#pragma unroll
+                for (int db = 0; db < D / 32; ++db) {
+                    const uintx4 v = values(0, db, k);
+                    uintx4 fine = v;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        if ((v[e] & X::EXPONENT) == X::EXPONENT) fine[e] &= 0xffff0000u;
+                        if (((v[e] >> 16) & X::EXPONENT) == X::EXPONENT) fine[e] &= 0x0000ffffu;
+                    }
+                    o[db] = X::mfma32(__builtin_bit_cast(vec8, fine), pf, o[db]);
+#pragma unroll 1
+                    for (int kind = 0; kind < 3; ++kind) {
+                        const float what = kind == 0 ? NAN : kind == 1 ? INFINITY : -INFINITY;
+                        const float16_t hit = X::mfma32(__builtin_bit_cast(vec8, att_places<T>(v, kind)), vis, (float16_t)(0.0f));
+#pragma unroll
+                        for (int r = 0; r < 16; ++r)
+                            if (hit[r] > 0.0f) o[db][r] += what;
+                    }
+                }
+            }
+        }
+    }
 
     l = att_half_add(l);
     const float base = m == -INFINITY ? 0.0f : m;
     const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-    if (!valid) return;
-    if (p.splits > 1) {
-        const int64_t at = ((int64_t)pair * p.rows + row) * p.splits + split;
-        float *po = p.part_o + at * D + 4 * half;
+    int place = tile;
+    asm volatile("" : "+s"(place));     // row, token and head are worked out again rather than kept in registers over the loop
+    {
+        const int row = place * ROWS + wave * 32 + (lane & 31);
+        if (row >= p.rows) return;
+        const int t = p.by_group.div(row), head = kvh * p.group + (row - t * p.group);
+        if (p.splits > 1) {
+            const int64_t at = ((int64_t)pair * p.rows + row) * p.splits + split;
+            float *po = p.part_o + at * D + 4 * half;
+#pragma unroll
+            for (int db = 0; db < D / 32; ++db)
+#pragma unroll
+                for (int g = 0; g < 4; ++g)
+                    *(floatx4 *)(po + 32 * db + 8 * g) = (floatx4){o[db][4 * g] * inv, o[db][4 * g + 1] * inv, o[db][4 * g + 2] * inv, o[db][4 * g + 3] * inv};
+            if (half == 0) p.part_l[at] = l == 0.0f ? -INFINITY : base + log2f(l);
+            return;
+        }
+        T *out = (T *)a.out + b * a.out_stride[0] + t * a.out_stride[1] + head * a.out_stride[2] + 4 * half;
 #pragma unroll
         for (int db = 0; db < D / 32; ++db)
 #pragma unroll
             for (int g = 0; g < 4; ++g)
-                *(floatx4 *)(po + 32 * db + 8 * g) = (floatx4){o[db][4 * g] * inv, o[db][4 * g + 1] * inv, o[db][4 * g + 2] * inv, o[db][4 * g + 3] * inv};
-        if (half == 0) p.part_l[at] = l == 0.0f ? -INFINITY : base + log2f(l);
-        return;
+                *(uintx2 *)(out + 32 * db + 8 * g) = (uintx2){op_pack2(o[db][4 * g] * inv, o[db][4 * g + 1] * inv, T()),
+                                                              op_pack2(o[db][4 * g + 2] * inv, o[db][4 * g + 3] * inv, T())};
+        if (a.lse != nullptr && half == 0)
+            a.lse[((int64_t)b * a.heads + head) * a.q_tokens + t] = l == 0.0f ? -INFINITY : base * 0.6931471805599453f + logf(l);
     }
-    T *out = (T *)a.out + b * a.out_stride[0] + t * a.out_stride[1] + head * a.out_stride[2] + 4 * half;
-#pragma unroll
-    for (int db = 0; db < D / 32; ++db)
-#pragma unroll
-        for (int g = 0; g < 4; ++g)
-            *(uintx2 *)(out + 32 * db + 8 * g) = (uintx2){op_pack2(o[db][4 * g] * inv, o[db][4 * g + 1] * inv, T()),
-                                                          op_pack2(o[db][4 * g + 2] * inv, o[db][4 * g + 3] * inv, T())};
-    if (a.lse != nullptr && half == 0)
-        a.lse[((int64_t)b * a.heads + head) * a.q_tokens + t] = l == 0.0f ? -INFINITY : base * 0.6931471805599453f + logf(l);
 }
 
 // ------------------------------------------------------------------------------------------------------------------
