@@ -332,7 +332,7 @@ __global__ __launch_bounds__(NW * 64, D <= 64 ? 3 : 2) void attention_kernel(Att
         const int at0 = j0 + 4 * half, lo = see.lo - at0, hi = see.hi - at0, plo = apart ? see.plo - at0 : 0, phi = apart ? see.phi - at0 : 0;
         unsigned seen = 0;
         ATT_EACH {
-            const bool v = (e >= lo && e < hi) || (e >= plo && e < phi);
+            const bool v = ((e >= lo) & (e < hi)) | ((e >= plo) & (e < phi));
             s[i][r] = v ? s[i][r] : score.HIDDEN;
             seen |= v ? 1u << (16 * i + r) : 0u;
         }

@@ -15,6 +15,7 @@ import torch
 from .capi import MIBC_OK, MibcError, MibcNotSupported, lib
 
 _TYPE = {torch.float16: 0, torch.bfloat16: 1, torch.float32: 2, torch.int8: 3, torch.float8_e4m3fn: 4}
+_FLOATS = (torch.float16, torch.bfloat16, torch.float32)
 _QUANT = {"int8": torch.int8, "e4m3": torch.float8_e4m3fn}
 ATTN_END = -2147483648
 SCALINGS = {"none": 0, "linear": 1, "base": 2, "by_parts": 3}
@@ -50,26 +51,44 @@ def _device(what: str, first: torch.Tensor, *others) -> int:
     dev = first.device
     if dev.type != "cuda":
         raise MibcError(f"{what}: tensors must be on a HIP device (got {dev}); there is no CPU form")
-    grad = torch.is_grad_enabled()
-    for t in (first,) + others:
-        if t is None:
-            continue
-        if t.device != dev:
-            raise MibcError(f"{what}: tensors on {dev} and {t.device}")
-        if grad and t.requires_grad:
-            raise MibcNotSupported(f"{what}: forward only; call it under torch.no_grad() or on detached tensors")
+    grad = first.requires_grad
+    for t in others:
+        if t is not None:
+            if t.device != dev:
+                raise MibcError(f"{what}: tensors on {dev} and {t.device}")
+            grad = grad or t.requires_grad
+    if grad and torch.is_grad_enabled():
+        raise MibcNotSupported(f"{what}: forward only; call it under torch.no_grad() or on detached tensors")
     return dev.index
 
 
-def _stream(device: int) -> int:
-    return torch.cuda.current_stream(device).cuda_stream
+# the current stream's handle, without a Stream object around it where this torch offers that
+_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda device: torch.cuda.current_stream(device).cuda_stream)
 
 
-def _index32(what: str, name: str, t, n: int):
-    """Pointer of a contiguous int32 tensor of n elements, 0 for None."""
-    if t is None:
-        return 0
-    if t.dtype is not torch.int32 or t.dim() != 1 or t.shape[0] != n or (n > 1 and t.stride(0) != 1):
+def _row_stride(what: str, name: str, t: torch.Tensor, cols: int) -> int:
+    """Elements from row to row of `t` seen as rows of `cols`."""
+    st = t.stride()
+    if st[-1] != 1 and cols > 1:
+        raise MibcError(f"{what}: the last dimension of {name} must be contiguous")
+    n = len(st)
+    if n == 2:
+        return st[0]
+    if n == 1 or t.is_contiguous():
+        return cols
+    try:
+        return t.view(-1, cols).stride(0)
+    except RuntimeError:
+        raise MibcError(f"{what}: the leading dimensions of {name} must be viewable as rows") from None
+
+
+def _new(like: torch.Tensor) -> torch.Tensor:
+    return torch.empty_like(like) if like.is_contiguous() else like.new_empty(like.shape)
+
+
+def _index32(what: str, name: str, t, n: int) -> int:
+    """Pointer of a contiguous int32 tensor of n elements."""
+    if t.dtype is not torch.int32 or t.shape != (n,) or not t.is_contiguous():
         raise MibcError(f"{what}: {name} must be a contiguous int32 tensor of {n} elements")
     return t.data_ptr()
 
@@ -82,57 +101,46 @@ def rms_norm(x, weight=None, *, residual=None, alpha: float = 1.0, eps: float = 
     quant "int8" / "e4m3": the codes round(y / s) and the f32 scales s [..., groups], one per row (group 0) or per `group`
     (32, 64, 128) columns.  Returns y or (codes, scales), followed by h (x's type) if return_sum or sum_out is given."""
     dev = _device("rms_norm", x, weight, residual, out, sum_out)
-    if x.dtype not in (torch.float16, torch.bfloat16, torch.float32):
-        raise MibcNotSupported(f"rms_norm: type {x.dtype}")
-    if quant is not None and quant not in _QUANT:
-        raise MibcError(f"rms_norm: quant must be None, 'int8' or 'e4m3', not {quant!r}")
-    if x.dim() < 1 or x.shape[-1] == 0:
+    dtype, shape = x.dtype, x.shape
+    if dtype not in _FLOATS:
+        raise MibcNotSupported(f"rms_norm: type {dtype}")
+    if not shape or shape[-1] == 0:
         raise MibcError("rms_norm: x needs a last dimension")
-    shape, cols = x.shape, x.shape[-1]
-    if weight is not None and (weight.dim() != 1 or weight.shape[0] != cols or weight.dtype not in (torch.float32, x.dtype)
-                               or weight.stride(0) not in (1,) and cols > 1):
-        raise MibcError(f"rms_norm: weight must be a contiguous [{cols}] tensor, f32 or {x.dtype}")
-
-    def rows_of(t, name, dtype, width=cols):
-        """(tensor, row stride) of `t` seen as rows."""
-        if t.shape[:-1] != shape[:-1] or t.shape[-1] != width or t.dtype is not dtype:
-            raise MibcError(f"rms_norm: {name} must be {list(shape[:-1]) + [width]} {dtype}")
-        if width > 1 and t.stride(-1) != 1:
-            raise MibcError(f"rms_norm: the last dimension of {name} must be contiguous")
-        if t.dim() == 1:
-            return t, width
-        if t.dim() > 2:
-            if t.is_contiguous():
-                return t, width
-            try:
-                t = t.view(-1, width)
-            except RuntimeError:
-                raise MibcError(f"rms_norm: the leading dimensions of {name} must be viewable as rows") from None
-        return t, t.stride(0)
-
-    x2, xs = rows_of(x, "x", x.dtype)
-    r2, rs = (None, 0) if residual is None else rows_of(residual, "residual", x.dtype)
-    out_dtype = x.dtype if quant is None else _QUANT[quant]
-    if out is None:
-        out = torch.empty(shape, dtype=out_dtype, device=x.device)
-    o2, os_ = rows_of(out, "out", out_dtype)
-    if sum_out is None and return_sum:
-        sum_out = torch.empty(shape, dtype=x.dtype, device=x.device)
-    s2, ss = (None, 0) if sum_out is None else rows_of(sum_out, "sum_out", x.dtype)
-    scale, groups = None, 0
+    cols = shape[-1]
+    if weight is not None and (weight.shape != (cols,) or not (weight.dtype is torch.float32 or weight.dtype is dtype)
+                               or not weight.is_contiguous()):
+        raise MibcError(f"rms_norm: weight must be a contiguous [{cols}] tensor, f32 or {dtype}")
+    if residual is not None and (residual.shape != shape or residual.dtype is not dtype):
+        raise MibcError(f"rms_norm: residual must be {list(shape)} {dtype}")
+    out_dtype, scale, groups = dtype, None, 0
     if quant is not None:
-        if group and cols % group:
+        if quant not in _QUANT:
+            raise MibcError(f"rms_norm: quant must be None, 'int8' or 'e4m3', not {quant!r}")
+        if group < 0 or (group and cols % group):
             raise MibcError("rms_norm: the columns must be a multiple of group")
-        groups = cols // group if group else 1
+        out_dtype, groups = _QUANT[quant], cols // group if group else 1
         scale = torch.empty(shape[:-1] + (groups,), dtype=torch.float32, device=x.device)
-    args = _NORM_ARGS.pack(x2.data_ptr(), 0 if r2 is None else r2.data_ptr(), 0 if weight is None else weight.data_ptr(),
-                           0 if s2 is None else s2.data_ptr(), o2.data_ptr(), 0 if scale is None else scale.data_ptr(),
-                           x.numel() // cols, xs, rs, ss, os_, groups, cols, _TYPE[x.dtype],
-                           _TYPE[x.dtype if weight is None else weight.dtype], _TYPE[out_dtype], group, alpha, eps, 0)
-    _check(_entry()[0](dev, _stream(dev), args), "rms_norm")
-    if scale is None and sum_out is None:
-        return out
-    return (out,) + (() if scale is None else (scale,)) + (() if sum_out is None else (sum_out,))
+    if out is None:
+        out = _new(x) if quant is None else torch.empty(shape, dtype=out_dtype, device=x.device)
+    elif out.shape != shape or out.dtype is not out_dtype:
+        raise MibcError(f"rms_norm: out must be {list(shape)} {out_dtype}")
+    if sum_out is None:
+        if return_sum:
+            sum_out = _new(x)
+    elif sum_out.shape != shape or sum_out.dtype is not dtype:
+        raise MibcError(f"rms_norm: sum_out must be {list(shape)} {dtype}")
+    args = _NORM_ARGS.pack(
+        x.data_ptr(), 0 if residual is None else residual.data_ptr(), 0 if weight is None else weight.data_ptr(),
+        0 if sum_out is None else sum_out.data_ptr(), out.data_ptr(), 0 if scale is None else scale.data_ptr(), x.numel() // cols,
+        _row_stride("rms_norm", "x", x, cols), 0 if residual is None else _row_stride("rms_norm", "residual", residual, cols),
+        0 if sum_out is None else _row_stride("rms_norm", "sum_out", sum_out, cols), _row_stride("rms_norm", "out", out, cols), groups,
+        cols, _TYPE[dtype], _TYPE[dtype if weight is None else weight.dtype], _TYPE[out_dtype], group, alpha, eps, 0)
+    rc = (_fns or _entry())[0](dev, _stream(dev), args)
+    if rc:
+        _check(rc, "rms_norm")
+    if scale is None:
+        return out if sum_out is None else (out, sum_out)
+    return (out, scale) if sum_out is None else (out, scale, sum_out)
 
 
 def rope_frequencies(rot_dim: int, theta: float = 10000.0, *, scaling: str = "none", factor: float = 1.0,
@@ -159,42 +167,51 @@ def rope(q, k=None, *, freqs, positions=None, start: int = 0, interleaved: bool 
     dev = _device("rope", q, k, freqs, positions)
     if q.dim() != 4:
         raise MibcError("rope: q must be [batch, tokens, heads, head_dim]")
-    b, t, h, d = q.shape
-    if q.dtype not in (torch.float16, torch.bfloat16, torch.float32):
-        raise MibcNotSupported(f"rope: type {q.dtype}")
-    if k is not None and (k.dim() != 4 or k.shape[0] != b or k.shape[1] != t or k.shape[3] != d or k.dtype is not q.dtype):
-        raise MibcError("rope: k must be like q but for the number of heads")
-    if freqs.dtype is not torch.float64 or freqs.dim() != 1 or (freqs.shape[0] > 1 and freqs.stride(0) != 1):
+    shape, dtype = q.shape, q.dtype
+    b, t, h, d = shape
+    if dtype not in _FLOATS:
+        raise MibcNotSupported(f"rope: type {dtype}")
+    if freqs.dtype is not torch.float64 or freqs.dim() != 1 or not freqs.is_contiguous():
         raise MibcError("rope: freqs must be a contiguous f64 tensor [rot_dim / 2]")
-    rot = 2 * freqs.shape[0]
+    where = 0
     if positions is not None:
         if positions.dtype not in (torch.int32, torch.int64):
             raise MibcError("rope: positions must be int32 or int64")
-        if positions.shape == (t,) and b != 1:
+        if positions.shape != (b, t):
+            if positions.shape != (t,):
+                raise MibcError(f"rope: positions must be [{b}, {t}] or [{t}]")
             positions = positions.expand(b, t)
-        elif positions.shape not in ((b, t), (t,)):
-            raise MibcError(f"rope: positions must be [{b}, {t}] or [{t}]")
         positions = positions.contiguous()
-    outs = out if isinstance(out, (tuple, list)) else (out, None)
-    if out is not None and k is not None and (len(outs) != 2 or outs[1] is None):
-        raise MibcError("rope: out must be a pair where k is given")
-    if out is not None:
-        _device("rope", q, *outs)
-    qo = torch.empty((b, t, h, d), dtype=q.dtype, device=q.device) if out is None else outs[0]
-    ko = None if k is None else torch.empty(k.shape, dtype=q.dtype, device=q.device) if out is None else outs[1]
-    for x, o in ((q, qo), (k, ko)):
-        if x is None:
-            continue
-        if o.shape != x.shape or o.dtype is not x.dtype:
+        where = positions.data_ptr()
+    if out is None:
+        qo, ko = _new(q), None if k is None else _new(k)
+    else:
+        qo, ko = out if isinstance(out, (tuple, list)) else (out, None)
+        if qo is None or (k is None) != (ko is None):
+            raise MibcError("rope: out must be a tensor, or a pair where k is given")
+        _device("rope", q, qo, ko)
+        if qo.shape != shape or qo.dtype is not dtype:
             raise MibcError("rope: out must have the input's shape and type")
-        if d > 1 and (x.stride(3) != 1 or o.stride(3) != 1):
-            raise MibcError("rope: head_dim must be contiguous")
-    ks, kos = (0, 0, 0) if k is None else k.stride()[:3], (0, 0, 0) if k is None else ko.stride()[:3]
-    args = _ROPE_ARGS.pack(q.data_ptr(), 0 if k is None else k.data_ptr(), qo.data_ptr(), 0 if k is None else ko.data_ptr(),
-                           0 if positions is None else positions.data_ptr(), freqs.data_ptr(), start, *q.stride()[:3], *ks,
-                           *qo.stride()[:3], *kos, b, t, h, 0 if k is None else k.shape[2], d, rot, _TYPE[q.dtype],
-                           int(interleaved), int(positions is not None and positions.dtype is torch.int64), amplitude)
-    _check(_entry()[1](dev, _stream(dev), args), "rope")
+    qs, qos = q.stride(), qo.stride()
+    plain = qs[3] == 1 and qos[3] == 1
+    if k is None:
+        kp, kop, kh, ks, kos = 0, 0, 0, (0, 0, 0, 1), (0, 0, 0, 1)
+    else:
+        kshape = k.shape
+        if len(kshape) != 4 or kshape[0] != b or kshape[1] != t or kshape[3] != d or k.dtype is not dtype:
+            raise MibcError("rope: k must be like q but for the number of heads")
+        if out is not None and (ko.shape != kshape or ko.dtype is not dtype):
+            raise MibcError("rope: out must have the input's shape and type")
+        kp, kop, kh, ks, kos = k.data_ptr(), ko.data_ptr(), kshape[2], k.stride(), ko.stride()
+        plain = plain and ks[3] == 1 and kos[3] == 1
+    if not plain and d > 1:
+        raise MibcError("rope: head_dim must be contiguous")
+    args = _ROPE_ARGS.pack(q.data_ptr(), kp, qo.data_ptr(), kop, where, freqs.data_ptr(), start, qs[0], qs[1], qs[2], ks[0], ks[1], ks[2],
+                           qos[0], qos[1], qos[2], kos[0], kos[1], kos[2], b, t, h, kh, d, 2 * freqs.shape[0], _TYPE[dtype],
+                           bool(interleaved), where != 0 and positions.dtype is torch.int64, amplitude)
+    rc = (_fns or _entry())[1](dev, _stream(dev), args)
+    if rc:
+        _check(rc, "rope")
     return qo if k is None else (qo, ko)
 
 
@@ -210,55 +227,59 @@ def attention(q, k, v, *, scale=None, causal: bool = False, window=(-1, -1), sof
     other, each seeing itself only; prefix is then [n] and counts from the document's start.  A query that sees nothing gives
     zeros.  Returns out like q, or (out, lse f32 [batch, heads, q_tokens])."""
     dev = _device("attention", q, k, v, slopes, k_len, prefix, doc_offsets, out)
-    if q.dim() != 4 or k.dim() != 4 or v.dim() != 4:
+    shape, kshape, dtype = q.shape, k.shape, q.dtype
+    if len(shape) != 4 or len(kshape) != 4:
         raise MibcError("attention: q, k, v must be [batch, tokens, heads, head_dim]")
-    b, n, h, d = q.shape
-    m, kh = k.shape[1], k.shape[2]
-    if k.shape != v.shape or k.shape[0] != b or k.shape[3] != d:
+    b, n, h, d = shape
+    if v.shape != kshape or kshape[0] != b or kshape[3] != d:
         raise MibcError("attention: k and v must be [batch, k_tokens, kv_heads, head_dim] like q")
-    if k.dtype is not q.dtype or v.dtype is not q.dtype:
+    if k.dtype is not dtype or v.dtype is not dtype:
         raise MibcError("attention: q, k and v must be of one type")
-    if q.dtype not in (torch.float16, torch.bfloat16):
-        raise MibcNotSupported(f"attention: type {q.dtype}")
+    if dtype is not torch.float16 and dtype is not torch.bfloat16:
+        raise MibcNotSupported(f"attention: type {dtype}")
+    m, kh = kshape[1], kshape[2]
+    back, ahead = window
     if causal:
-        if tuple(window) != (-1, -1):
+        if back != -1 or ahead != -1:
             raise MibcError("attention: causal is window (-1, 0); give one of the two")
-        window = (-1, 0)
+        ahead = 0
+    back, ahead = max(-1, min(int(back), 0x7fffffff)), max(-1, min(int(ahead), 0x7fffffff))
     if out is None:
-        out = torch.empty((b, n, h, d), dtype=q.dtype, device=q.device)
-    elif out.shape != q.shape or out.dtype is not q.dtype:
+        out = _new(q)
+    elif out.shape != shape or out.dtype is not dtype:
         raise MibcError("attention: out must have q's shape and type")
     qs, ks, vs, os_ = q.stride(), k.stride(), v.stride(), out.stride()
-    if qs[3] != 1 or os_[3] != 1 or (m and kh and (ks[3] != 1 or vs[3] != 1)):
+    if qs[3] != 1 or os_[3] != 1 or ((ks[3] != 1 or vs[3] != 1) and m and kh):
         raise MibcError("attention: head_dim must be contiguous")
-    if slopes is not None and (slopes.dtype is not torch.float32 or slopes.shape != (h,) or not slopes.is_contiguous()):
-        raise MibcError(f"attention: slopes must be a contiguous f32 tensor [{h}]")
-    docs = 0
+    lens = pre = offs = slope = docs = 0
+    if slopes is not None:
+        if slopes.dtype is not torch.float32 or slopes.shape != (h,) or not slopes.is_contiguous():
+            raise MibcError(f"attention: slopes must be a contiguous f32 tensor [{h}]")
+        slope = slopes.data_ptr()
     if doc_offsets is not None:
         docs = doc_offsets.shape[0] - 1 if doc_offsets.dim() == 1 else -1
         if docs < 0:
             raise MibcError("attention: doc_offsets must be [n + 1]")
-    lens = _index32("attention", "k_len", k_len, b)
-    pre = _index32("attention", "prefix", prefix, docs if doc_offsets is not None else b)
-    offs = _index32("attention", "doc_offsets", doc_offsets, docs + 1)
+        offs = _index32("attention", "doc_offsets", doc_offsets, docs + 1)
+    if k_len is not None:
+        lens = _index32("attention", "k_len", k_len, b)
+    if prefix is not None:
+        pre = _index32("attention", "prefix", prefix, docs if doc_offsets is not None else b)
     if q_start is None:
         q_start = ATTN_END
     elif not -(1 << 28) <= q_start <= 1 << 28:
         raise MibcNotSupported("attention: q_start beyond 2^28")
-    limits = [max(-1, min(int(w), (1 << 31) - 1)) for w in window]
     lse = torch.empty((b, h, n), dtype=torch.float32, device=q.device) if return_lse else None
-
-    def pack(ws, nbytes):
-        return _ATTN_ARGS.pack(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), 0 if lse is None else lse.data_ptr(), lens,
-                               pre, offs, 0 if slopes is None else slopes.data_ptr(), ws, nbytes, qs[0], qs[1], qs[2], ks[0], ks[1],
-                               ks[2], vs[0], vs[1], vs[2], os_[0], os_[1], os_[2], b, h, kh, n, m, d, docs, _TYPE[q.dtype],
-                               limits[0], limits[1], q_start, d ** -0.5 if scale is None else scale, softcap, 0)
-
-    _, _, run, workspace = _entry()
-    args = pack(0, 0)
+    head = (q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), 0 if lse is None else lse.data_ptr(), lens, pre, offs, slope)
+    tail = (qs[0], qs[1], qs[2], ks[0], ks[1], ks[2], vs[0], vs[1], vs[2], os_[0], os_[1], os_[2], b, h, kh, n, m, d, docs, _TYPE[dtype],
+            back, ahead, q_start, d ** -0.5 if scale is None else scale, softcap, 0)
+    _, _, run, workspace = _fns or _entry()
+    args = _ATTN_ARGS.pack(*head, 0, 0, *tail)
     need = workspace(args)
     if need:
         room = torch.empty(need, dtype=torch.uint8, device=q.device)
-        args = pack(room.data_ptr(), need)
-    _check(run(dev, _stream(dev), args), "attention")
+        args = _ATTN_ARGS.pack(*head, room.data_ptr(), need, *tail)
+    rc = run(dev, _stream(dev), args)
+    if rc:
+        _check(rc, "attention")
     return out if lse is None else (out, lse)
