@@ -60,11 +60,31 @@ static AttPlan att_plan(const mibc_attention_args &a) {
         keys = keys < w ? keys : w;
     }
     const int64_t groups = p.tiles * pairs;
-    // tiles: two workgroups per CU, a part is worth its share of the join from four tiles of 64 keys on;
-    // tokens: eight per CU (rows of a batch differ in length), from four steps of 32 keys for each of the four waves on
-    const int64_t want = p.variant == ATT_TOKENS ? 2048 : 512, least = p.variant == ATT_TOKENS ? 512 : 256;
-    int64_t splits = groups >= want ? 1 : want / groups;
-    if (splits > keys / least) splits = keys / least;
+    int64_t splits = 1;
+    if (p.variant == ATT_TOKENS) {
+        // the smallest number of parts that fills whole rounds of one workgroup per CU to nine tenths (one token over 131072 keys,
+        // 2 key heads: 128 parts 34 us, 255 parts 41, 64 parts 38; 32 pairs x 4096 keys: 8 parts 17 us, 4 parts 20, 32 parts 20);
+        // rows of different lengths: five or more parts per pair even out the lengths (48 x 8 pairs of 2048 .. 8192 keys: 191 us
+        // against 248 unsplit).  At least four steps of 32 keys for each of the four waves: a
+        // shorter part costs more in the second launch than it saves (512 keys: 9.0 us whole, 13.9 in two)
+        const int64_t most = keys / 512 < 255 ? keys / 512 : 255, cus = 256;
+        double best = 0.0;
+        for (int64_t s = 1; s <= most; ++s) {
+            const int64_t all = groups * s;
+            const double full = (double)all / (double)((all + cus - 1) / cus * cus);
+            if (full > best + 1e-9) {
+                best = full;
+                splits = s;
+            }
+            if (best >= 0.9) break;
+        }
+        if (a.k_len != nullptr && splits * groups < 2048) splits = 2048 / groups < most ? 2048 / groups : most;
+    } else if (groups < 256) {
+        // tiles: a workgroup per CU, and at least four tiles of 64 keys in a part (64 rows of 16 heads over 16384 keys, 8 tiles:
+        // 32 parts 26 us, 64 parts 30, 16 parts 32, 8 parts 51)
+        splits = 256 / groups;
+        if (splits > keys / 256) splits = keys / 256;
+    }
     if (splits > 255) splits = 255;
     p.splits = splits < 1 ? 1 : (int)splits;
     return p;

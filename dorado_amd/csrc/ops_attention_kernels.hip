@@ -391,14 +391,20 @@ __global__ __launch_bounds__(NW * 64, D <= 64 ? 3 : 2) void attention_kernel(Att
         constexpr unsigned AT = decltype(stage_)::value * (2 * TILE);
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         __builtin_amdgcn_s_barrier();
-        if (it + 1 < it1) fetch(it + 1, decltype(stage_)::value ^ 1);
         const int j0 = first_key(it);
-        if ((j0 >= hi_max || j0 + 64 <= lo_min) && (j0 >= phi_max || j0 + 64 <= plo_min)) return;   // no row of the wave
+        if ((j0 >= hi_max || j0 + 64 <= lo_min) && (j0 >= phi_max || j0 + 64 <= plo_min)) {      // no row of the wave
+            if (it + 1 < it1) fetch(it + 1, decltype(stage_)::value ^ 1);
+            return;
+        }
         products(AT);
+        if (it + 1 < it1) fetch(it + 1, decltype(stage_)::value ^ 1);      // behind the reads of K, which it would hold up
         shape(j0);
         if (j0 < lo_max || j0 + 64 > hi_min) hide(j0);
         maxima();
         // the products of 16 keys run beside the probabilities of the next 16, whose values are read meanwhile
+        // a wave that forms probabilities goes before the SIMD's other waves: both pipes have work from it then, and the others'
+        // score products fill the matrix pipe meanwhile (4 % at head size 128, 8 % capped)
+        __builtin_amdgcn_s_setprio(1);
         constexpr int N = D / 32;
         uintx4 v[2][N];
 #pragma unroll
@@ -416,6 +422,7 @@ __global__ __launch_bounds__(NW * 64, D <= 64 ? 3 : 2) void attention_kernel(Att
 #pragma unroll
             for (int db = 0; db < N; ++db) o[db] = X::mfma32(__builtin_bit_cast(vec8, v[k & 1][db]), pf[k & 1], o[db]);
             ATT_FENCE();
+            if (k == 2) __builtin_amdgcn_s_setprio(0);
         }
     };
     start();
