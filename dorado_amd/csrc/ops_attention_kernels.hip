@@ -106,6 +106,13 @@ __device__ __forceinline__ AttRow att_row(const AttArgs &p, int b, int t, int bo
     return r;
 }
 
+// The kernel's arguments, read again where they are next needed: kept in scalar registers over the main loop they spill
+__device__ __forceinline__ const AttArgs &att_args_again() {
+    auto at = __builtin_amdgcn_kernarg_segment_ptr();
+    asm volatile("" : "+s"(at));
+    return *(const AttArgs *)at;
+}
+
 // The exponent (base 2) of a score is mul * x + add, x being what the registers hold.  Plain: x = q.k, mul = scale log2(e).
 // Capped: cap tanh(y) = cap - 2 cap / (1 + e^2y), so x = 1 / (1 + e^2y) and the last product is the exponent's own fma; the
 // largest score is the smallest x.  A slope adds slope * |i - j| to x, in x's unit.
@@ -487,10 +494,10 @@ __global__ __launch_bounds__(NW * 64, D <= 64 ? 3 : 2) void attention_kernel(Att
     l = att_half_add(l);
     const float base = m == -INFINITY ? 0.0f : m;
     const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-    int place = tile;
-    asm volatile("" : "+s"(place));     // row, token and head are worked out again rather than kept in registers over the loop
-    {
-        const int row = place * ROWS + wave * 32 + (lane & 31);
+    {   // row, token and head are worked out again rather than kept in registers over the loop
+        const AttArgs &p = att_args_again();
+        const mibc_attention_args &a = p.a;
+        const int row = tile * ROWS + wave * 32 + (lane & 31);
         if (row >= p.rows) return;
         const int t = p.by_group.div(row), head = kvh * p.group + (row - t * p.group);
         if (p.splits > 1) {
