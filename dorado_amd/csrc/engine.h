@@ -213,6 +213,11 @@ struct mibc_engine {
         std::vector<TxLayer> layers;
         half_t *wup = nullptr, *wcrf = nullptr;
         float *bup = nullptr, *rope = nullptr;
+        // attention by the operators (ops_rope.hip, ops_attention.hip) instead of the window kernels: other head sizes than 64,
+        // windows beyond those kernels' 256 keys
+        bool by_ops = false;
+        int hd = 64;
+        double *freqs = nullptr;      // [hd / 2] radians per position
         int D = 0, H = 0, FF = 0, depth = 0, sf = 1, conv_stride = 1;
         int fused = 1;                // layer tail through txlayer.hip (tests compare against the five-launch path)
         // workspace
@@ -249,6 +254,11 @@ std::vector<half_t> tx_layer_image(const float *wo, const float *w1, const float
 bool tx_layer_supported(int d_model, int ff);
 extern "C" int mibc_launch_tx_layer(hipStream_t s, const half_t *attn, half_t *x, const half_t *wimg, const float *bo,
                                     const float *n1, const float *n2, float alpha, long R, int FF, int mode);
+
+// transformer-layer operators on a stream of the current device (ops_norm.hip, ops_rope.hip, ops_attention.hip)
+int mibc_launch_rms_norm(hipStream_t s, const mibc_rms_norm_args &a);
+int mibc_launch_rope(hipStream_t s, const mibc_rope_args &a);
+int mibc_launch_attention(hipStream_t s, const mibc_attention_args &a, bool whole);
 
 // engine_tx.hip
 int tx_create(mibc_engine *e, const mibc_model_desc &d, const float *const *weights, int n_weights);

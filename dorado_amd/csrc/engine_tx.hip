@@ -28,18 +28,20 @@ int tx_create(mibc_engine *e, const mibc_model_desc &d, const float *const *weig
     if (d.n_convs < 2 || d.num_features != 1 || d.conv_insize[0] != 1 || d.conv_size[0] != 64 ||
         d.conv_winlen[0] != 5 || d.conv_stride[0] != 1)
         return fail(e, MIBC_NOT_SUPPORTED, "tx conv front-end must start with 1->64 (w5,s1)");
-    if (d.conv_size[d.n_convs - 1] != C || C % 128 != 0 || d.tx_nhead * 64 != C)
-        return fail(e, MIBC_NOT_SUPPORTED, "tx: d_model must be nhead*64 and a multiple of 128");
-    if ((C != 128 && C != 256 && C != 512) || d.tx_dim_ff % 64 != 0 || d.up_size != C)
-        return fail(e, MIBC_NOT_SUPPORTED, "tx: d_model must be 128/256/512");
-    if (64 + d.tx_win_upper + d.tx_win_lower > 320)
-        return fail(e, MIBC_NOT_SUPPORTED, "tx: attention window too large");
+    if (d.conv_size[d.n_convs - 1] != C || C % 128 != 0 || C > 2048 || d.tx_nhead < 1 || C % d.tx_nhead != 0)
+        return fail(e, MIBC_NOT_SUPPORTED, "tx: d_model must be a multiple of 128 (at most 2048) and of nhead");
+    const int hd = C / d.tx_nhead;
+    if (hd != 32 && hd != 64 && hd != 96 && hd != 128) return fail(e, MIBC_NOT_SUPPORTED, "tx: head size must be 32, 64, 96 or 128");
+    if (d.tx_dim_ff % 64 != 0 || d.up_size != C) return fail(e, MIBC_NOT_SUPPORTED, "tx: feed-forward width must be a multiple of 64, upsample width d_model");
+    if (d.tx_win_upper < 0 || d.tx_win_lower < 0) return fail(e, MIBC_NOT_SUPPORTED, "tx: attention window must be limited to both sides");
     if (n_weights != 2 * d.n_convs + 7 * d.tx_depth + 3)
         return fail(e, MIBC_ERR_ARG, "tx: unexpected number of weight tensors");
     auto &tx = e->tx;
     e->is_tx = true;
     tx.D = C;
     tx.H = d.tx_nhead;
+    tx.hd = hd;
+    tx.by_ops = hd != 64 || 64 + d.tx_win_upper + d.tx_win_lower > 320;
     tx.FF = d.tx_dim_ff;
     tx.depth = d.tx_depth;
     tx.sf = d.up_scale_factor;
@@ -112,7 +114,11 @@ int tx_create(mibc_engine *e, const mibc_model_desc &d, const float *const *weig
         // LinearScaledCRF: weight *= scale once (nn/TxModules.cpp:1010-1016)
         if (mibc_upload(e, &tx.wcrf, f2h(wcrf, (size_t)e->K * C, d.crf_scale))) return MIBC_ERR_HIP;
     }
-    {  // rotary table [max_seq_len][32] {cos, sin}  (nn/TxModules.cpp:184-220, head_dim 64)
+    if (tx.by_ops) {  // radians per position, in the reference's f32 (nn/TxModules.cpp:184-220)
+        std::vector<double> f((size_t)hd / 2);
+        for (int i = 0; i < hd / 2; ++i) f[i] = (double)(1.0f / (float)pow((double)d.tx_theta, (double)((float)(2 * i) / (float)hd)));
+        if (mibc_upload(e, &tx.freqs, f)) return MIBC_ERR_HIP;
+    } else {  // rotary table [max_seq_len][32] {cos, sin}  (nn/TxModules.cpp:184-220, head_dim 64)
         const int L = d.tx_max_seq_len > 0 ? d.tx_max_seq_len : 2048;
         std::vector<float> tab((size_t)L * 32 * 2);
         for (int i = 0; i < 32; ++i) {
@@ -147,7 +153,7 @@ void tx_free_ws(mibc_engine *e) {
 void tx_destroy(mibc_engine *e) {
     auto &tx = e->tx;
     tx_free_ws(e);
-    void *ptrs[] = {tx.c1w, tx.c1b, tx.wup, tx.wcrf, tx.bup, tx.rope};
+    void *ptrs[] = {tx.c1w, tx.c1b, tx.wup, tx.wcrf, tx.bup, tx.rope, tx.freqs};
     for (void *p : ptrs)
         if (p) (void)hipFree(p);
     for (auto &c : tx.convs) {
@@ -279,6 +285,75 @@ static int gemm(mibc_engine *e, const half_t *A, const half_t *B, const float *b
     return mibc_launch_gemm_tn(e->stream, &g);
 }
 
+// rotary positions and window attention of one layer by the operators: qkv [N*T][3*C] (plain projection) -> attn [N*T][C].  The
+// CPU reference evaluates 12 query splits whose K/V slice is [qb - win_lower, qe + win_upper) (nn/TxModules.cpp:398-411): one
+// launch per split over exactly that slice.
+static int tx_attention_by_ops(mibc_engine *e, int N, int T) {
+    auto &tx = e->tx;
+    const int C = tx.D, hd = tx.hd;
+    mibc_rope_args r{};
+    r.x[0] = tx.qkv;
+    r.out[0] = tx.qkv;
+    r.freqs = tx.freqs;
+    r.x_stride[0][0] = r.out_stride[0][0] = (int64_t)T * 3 * C;
+    r.x_stride[0][1] = r.out_stride[0][1] = 3 * C;
+    r.x_stride[0][2] = r.out_stride[0][2] = hd;
+    r.batch = N;
+    r.tokens = T;
+    r.heads[0] = 2 * tx.H;      // queries and keys lie side by side
+    r.head_dim = r.rot_dim = hd;
+    r.type = MIBC_TYPE_F16;
+    r.amplitude = 1.0f;
+    if (const int rc = mibc_launch_rope(e->stream, r)) return rc;
+    const int split = (((T + 11) / 12) + 3) / 4 * 4;
+    for (int qb = 0; qb < T; qb += split) {
+        const int qe = qb + split < T ? qb + split : T;
+        const int kb = qb > e->d.tx_win_lower ? qb - e->d.tx_win_lower : 0, ke = T - qe > e->d.tx_win_upper ? qe + e->d.tx_win_upper : T;
+        mibc_attention_args a{};
+        a.q = tx.qkv + (size_t)qb * 3 * C;
+        a.k = tx.qkv + (size_t)kb * 3 * C + C;
+        a.v = tx.qkv + (size_t)kb * 3 * C + 2 * C;
+        a.out = tx.attn + (size_t)qb * C;
+        for (int64_t *s : {a.q_stride, a.k_stride, a.v_stride}) {
+            s[0] = (int64_t)T * 3 * C;
+            s[1] = 3 * C;
+            s[2] = hd;
+        }
+        a.out_stride[0] = (int64_t)T * C;
+        a.out_stride[1] = C;
+        a.out_stride[2] = hd;
+        a.batch = N;
+        a.heads = a.kv_heads = tx.H;
+        a.q_tokens = qe - qb;
+        a.k_tokens = ke - kb;
+        a.head_dim = hd;
+        a.type = MIBC_TYPE_F16;
+        a.window_back = e->d.tx_win_upper;
+        a.window_ahead = e->d.tx_win_lower;
+        a.q_start = qb - kb;
+        a.scale = 1.0f / sqrtf((float)hd);
+        if (const int rc = mibc_launch_attention(e->stream, a, true)) return rc;
+    }
+    return MIBC_OK;
+}
+
+// x <- RMSNorm(in + alpha * x) * w: the fixed-width kernel where there is one, the operator elsewhere
+static int tx_residual_norm(mibc_engine *e, const half_t *in, half_t *x, const float *w, long rows, int C, float alpha) {
+    if (mibc_launch_residual_rmsnorm(e->stream, in, x, w, rows, C, alpha) == 0) return MIBC_OK;
+    mibc_rms_norm_args a{};
+    a.x = in;
+    a.residual = x;
+    a.weight = w;
+    a.out = x;
+    a.rows = rows;
+    a.x_stride = a.residual_stride = a.out_stride = a.cols = C;
+    a.type = a.out_type = MIBC_TYPE_F16;
+    a.weight_type = MIBC_TYPE_F32;
+    a.alpha = alpha;
+    a.eps = 1e-5f;
+    return mibc_launch_rms_norm(e->stream, a);
+}
+
 int tx_run_network(mibc_engine *e, const half_t *in_dev, int N, int T_in) {
     auto &tx = e->tx;
     const mibc_model_desc &d = e->d;
@@ -323,10 +398,12 @@ int tx_run_network(mibc_engine *e, const half_t *in_dev, int N, int T_in) {
     for (int l = 0; l < tx.depth; ++l) {
         const auto &L = tx.layers[l];
         MibcRange r_layer(e, "TxEncoder");
-        if (gemm(e, tx.x, L.wqkv, nullptr, tx.qkv, R, 3 * C, C, -1, /*rope*/ 1) != 0)
+        if (gemm(e, tx.x, L.wqkv, nullptr, tx.qkv, R, 3 * C, C, -1, /*rope*/ tx.by_ops ? 0 : 1) != 0)
             return fail(e, MIBC_NOT_SUPPORTED, "tx qkv gemm");
         int arc;
-        if (tx.vT && T % 128 == 0)
+        if (tx.by_ops)
+            arc = tx_attention_by_ops(e, N, T);
+        else if (tx.vT && T % 128 == 0)
             arc = mibc_launch_window_attention_v2(e->stream, tx.qkv, tx.vT, tx.attn, N, T, C, tx.H, 3 * C,
                                                   d.tx_win_upper, d.tx_win_lower);
         else
@@ -338,13 +415,11 @@ int tx_run_network(mibc_engine *e, const half_t *in_dev, int N, int T_in) {
             mibc_launch_tx_layer(e->stream, tx.attn, tx.x, L.wimg, L.bo, L.n1, L.n2, d.tx_deepnorm_alpha, R, tx.FF, 3) == 0)
             continue;
         if (gemm(e, tx.attn, L.wo, L.bo, tx.tmp, R, C, C, -1) != 0) return fail(e, MIBC_NOT_SUPPORTED, "tx out_proj");
-        if (mibc_launch_residual_rmsnorm(e->stream, tx.tmp, tx.x, L.n1, R, C, d.tx_deepnorm_alpha) != 0)
-            return fail(e, MIBC_NOT_SUPPORTED, "tx rmsnorm");
+        if (tx_residual_norm(e, tx.tmp, tx.x, L.n1, R, C, d.tx_deepnorm_alpha) != 0) return fail(e, MIBC_NOT_SUPPORTED, "tx rmsnorm");
         if (gemm(e, tx.x, L.wfc1, nullptr, tx.ff, R, 2 * tx.FF, C, -1, /*swiglu*/ 2, 0, tx.FF) != 0)
             return fail(e, MIBC_NOT_SUPPORTED, "tx fc1");
         if (gemm(e, tx.ff, L.wfc2, nullptr, tx.tmp, R, C, tx.FF, -1) != 0) return fail(e, MIBC_NOT_SUPPORTED, "tx fc2");
-        if (mibc_launch_residual_rmsnorm(e->stream, tx.tmp, tx.x, L.n2, R, C, d.tx_deepnorm_alpha) != 0)
-            return fail(e, MIBC_NOT_SUPPORTED, "tx rmsnorm");
+        if (tx_residual_norm(e, tx.tmp, tx.x, L.n2, R, C, d.tx_deepnorm_alpha) != 0) return fail(e, MIBC_NOT_SUPPORTED, "tx rmsnorm");
     }
     // upsample: [R][C] -> [R][sf*C] == [N][sf*T][C]
     if (gemm(e, tx.x, tx.wup, tx.bup, tx.up, R, tx.sf * C, C, -1) != 0) return fail(e, MIBC_NOT_SUPPORTED, "tx upsample");

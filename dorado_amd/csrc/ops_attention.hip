@@ -108,11 +108,13 @@ extern "C" uint64_t mibc_attention_workspace(const mibc_attention_args *a) {
     return att_room(*a, att_plan(*a));
 }
 
-// launch on a stream of the current device (the engine's own path); checks included
-int mibc_launch_attention(hipStream_t s, const mibc_attention_args &a) {
+// launch on a stream of the current device (the engine's own path); checks included.  whole: the keys are not split, so there is
+// no workspace (the engine's batches fill the device)
+int mibc_launch_attention(hipStream_t s, const mibc_attention_args &a, bool whole) {
     if (const int rc = att_check(a)) return rc;
     if (a.batch == 0 || a.q_tokens == 0) return MIBC_OK;
-    const AttPlan plan = att_plan(a);
+    AttPlan plan = att_plan(a);
+    if (whole) plan.splits = 1;
     if (const int rc = att_check_plan(a, plan)) return rc;
     AttArgs p{};
     p.a = a;
@@ -154,5 +156,5 @@ extern "C" int mibc_attention(int device, void *stream, const mibc_attention_arg
     if (const int rc = att_check_plan(*a, att_plan(*a))) return rc;
     OpDevice d(device);
     if (d.rc != hipSuccess) return op_hip(d.rc, "attention: device");
-    return mibc_launch_attention((hipStream_t)stream, *a);
+    return mibc_launch_attention((hipStream_t)stream, *a, false);
 }
