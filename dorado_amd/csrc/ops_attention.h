@@ -30,8 +30,8 @@ struct AttArgs {
     float *part_l;    // [pairs * rows][splits] log2 of the sum
 };
 
-enum AttVariant { ATT_ROWS_128, ATT_ROWS_64, ATT_TOKENS };   // row tiles of 128 or 64; at most 16 rows per pair (single tokens)
-#define MIBC_ATT_DECLARE(D) int mibc_att_launch_##D(hipStream_t s, const AttArgs &p, int variant, unsigned grid);
+// tokens: the kernel for at most 16 rows per pair, else tiles of 128 rows
+#define MIBC_ATT_DECLARE(D) int mibc_att_launch_##D(hipStream_t s, const AttArgs &p, bool tokens, unsigned grid);
 MIBC_ATT_DECLARE(32)
 MIBC_ATT_DECLARE(64)
 MIBC_ATT_DECLARE(96)

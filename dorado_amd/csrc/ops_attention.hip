@@ -12,6 +12,7 @@ static int att_check(const mibc_attention_args &a) {
     if (a.heads % a.kv_heads != 0) return op_refuse(MIBC_ERR_ARG, "attention: heads must be a multiple of kv_heads");
     if (!(a.scale > 0.0f) || !(a.scale <= 1e30f)) return op_refuse(MIBC_ERR_ARG, "attention: scale must be positive and finite");
     if (!(a.softcap >= 0.0f) || !(a.softcap <= 1e30f)) return op_refuse(MIBC_ERR_ARG, "attention: softcap must be 0 (none) or positive and finite");
+    if (a.softcap > 0.0f && !(3.0f * a.scale / a.softcap <= 3e38f)) return op_refuse(MIBC_ERR_ARG, "attention: softcap too small for this scale");
     if (a.reserved != 0) return op_refuse(MIBC_ERR_ARG, "attention: reserved must be 0");
     const int64_t big = (int64_t)1 << 28;     // positions, and distances between them, stay far inside 32 bits
     if (a.q_tokens > big || a.k_tokens > big || (int64_t)a.q_tokens * (a.heads / a.kv_heads) > big ||
@@ -45,13 +46,14 @@ static int att_check(const mibc_attention_args &a) {
 }
 
 struct AttPlan {
-    int variant, tiles, splits;
+    bool tokens;     // at most 16 rows per (batch, key head) pair
+    int tiles, splits;
 };
 static AttPlan att_plan(const mibc_attention_args &a) {
     const int64_t rows = (int64_t)a.q_tokens * (a.heads / a.kv_heads), pairs = (int64_t)a.batch * a.kv_heads;
     AttPlan p;
-    p.variant = rows <= 16 ? ATT_TOKENS : rows > 64 ? ATT_ROWS_128 : ATT_ROWS_64;
-    const int tile = p.variant == ATT_ROWS_128 ? 128 : p.variant == ATT_ROWS_64 ? 64 : 16;
+    p.tokens = rows <= 16;
+    const int tile = p.tokens ? 16 : 128;
     p.tiles = (int)((rows + tile - 1) / tile);
     // keys a row can see at most
     int64_t keys = a.k_tokens;
@@ -61,7 +63,7 @@ static AttPlan att_plan(const mibc_attention_args &a) {
     }
     const int64_t groups = p.tiles * pairs;
     int64_t splits = 1;
-    if (p.variant == ATT_TOKENS) {
+    if (p.tokens) {
         // the smallest number of parts that fills whole rounds of one workgroup per CU to nine tenths (one token over 131072 keys,
         // 2 key heads: 128 parts 34 us, 255 parts 41, 64 parts 38; 32 pairs x 4096 keys: 8 parts 17 us, 4 parts 20, 32 parts 20);
         // rows of different lengths: five or more parts per pair even out the lengths (48 x 8 pairs of 2048 .. 8192 keys: 191 us
@@ -79,10 +81,12 @@ static AttPlan att_plan(const mibc_attention_args &a) {
             if (best >= 0.9) break;
         }
         if (a.k_len != nullptr && splits * groups < 2048) splits = 2048 / groups < most ? 2048 / groups : most;
-    } else if (groups < 256) {
-        // tiles: a workgroup per CU, and at least four tiles of 64 keys in a part (64 rows of 16 heads over 16384 keys, 8 tiles:
-        // 32 parts 26 us, 64 parts 30, 16 parts 32, 8 parts 51)
-        splits = 256 / groups;
+    } else {
+        // tiles: a workgroup per CU (64 rows of 4 heads each over 16384 keys, 8 tiles: 32 parts 26 us, 64 parts 30, 16 parts 32), two
+        // where a tile is half empty and reading the keys is what takes the time (8 x 8 pairs of 32 rows over 8192 keys: 8 parts
+        // 58 us, 4 parts 69), and at least four tiles of 64 keys in a part
+        const int64_t want = rows <= 64 ? 512 : 256;
+        if (groups < want) splits = want / groups;
         if (splits > keys / 256) splits = keys / 256;
     }
     if (splits > 255) splits = 255;
@@ -142,10 +146,10 @@ int mibc_launch_attention(hipStream_t s, const mibc_attention_args &a, bool whol
     const int64_t grid = (int64_t)p.pairs * p.tiles * p.splits;
     p.order = (a.window_ahead != 0 && p.pairs % 8 == 0) ? 1 : 0;
     switch (a.head_dim) {
-        case 32: return mibc_att_launch_32(s, p, plan.variant, (unsigned)grid);
-        case 64: return mibc_att_launch_64(s, p, plan.variant, (unsigned)grid);
-        case 96: return mibc_att_launch_96(s, p, plan.variant, (unsigned)grid);
-        default: return mibc_att_launch_128(s, p, plan.variant, (unsigned)grid);
+        case 32: return mibc_att_launch_32(s, p, plan.tokens, (unsigned)grid);
+        case 64: return mibc_att_launch_64(s, p, plan.tokens, (unsigned)grid);
+        case 96: return mibc_att_launch_96(s, p, plan.tokens, (unsigned)grid);
+        default: return mibc_att_launch_128(s, p, plan.tokens, (unsigned)grid);
     }
 }
 

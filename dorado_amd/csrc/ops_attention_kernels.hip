@@ -150,7 +150,7 @@ __device__ __forceinline__ uintx4 att_places(uintx4 v, int kind) {
 }
 
 // ------------------------------------------------------------------------------------------------------------------
-// Row tiles of 32 NW rows: one wave per 32 rows, all waves over the same tiles of 64 keys in LDS (two stages, filled by direct
+// Row tiles of 128 rows: four waves of 32, all over the same tiles of 64 keys in LDS (two stages, filled by direct
 // global -> LDS loads while the tile before is worked on).
 //   S^T[key][row] = K Q^T   on 32x32x16: lane (row = lane & 31, half = lane >> 5) holds keys 8 g + 4 half + 0..3 of each 32
 //   O^T[dim][row] = V^T P^T  takes P^T from those very registers: the 16 k-slots of a step are enumerated as the keys a lane holds,
@@ -165,11 +165,11 @@ __device__ __forceinline__ int att_v_slot(int row, int chunk) {
     return D == 128 ? chunk ^ ((row & 3) << 2) : D == 64 ? chunk ^ (((row >> 1) & 1) << 2) : chunk;
 }
 
-template <typename T, int D, int NW, bool CAP, bool SLOPES>
-__global__ __launch_bounds__(NW * 64, D <= 64 ? 3 : 2) void attention_kernel(AttArgs p) {
+template <typename T, int D, bool CAP, bool SLOPES>
+__global__ __launch_bounds__(256, D <= 64 ? 3 : 2) void attention_kernel(AttArgs p) {
     typedef AttType<T> X;
     typedef typename X::vec8 vec8;
-    constexpr int NT = NW * 64;
+    constexpr int NT = 256, ROWS = 128;
     constexpr int PITCH = D * 2;
     constexpr int TILE = 64 * PITCH;
     constexpr int CH = TILE / 16;               // 16-byte pieces of a tile
@@ -200,7 +200,6 @@ __global__ __launch_bounds__(NW * 64, D <= 64 ? 3 : 2) void attention_kernel(Att
     const int b = p.by_kv.div(pair), kvh = pair - b * a.kv_heads;
 
     // lanes 32 and 33 look at the workgroup's first and last row instead of their own
-    constexpr int ROWS = 32 * NW;
     const int row = tile * ROWS + wave * 32 + (lane & 31);
     const int rr = min(row, p.rows - 1), t = p.by_group.div(rr), head = kvh * p.group + (rr - t * p.group);
     const int t_first = p.by_group.div(tile * ROWS), t_last = p.by_group.div(min(tile * ROWS + ROWS, p.rows) - 1);
@@ -409,9 +408,10 @@ __global__ __launch_bounds__(NW * 64, D <= 64 ? 3 : 2) void attention_kernel(Att
         if (j0 < lo_max || j0 + 64 > hi_min) hide(j0);
         maxima();
         // the products of 16 keys run beside the probabilities of the next 16, whose values are read meanwhile
-        // a wave that forms probabilities goes before the SIMD's other waves: both pipes have work from it then, and the others'
-        // score products fill the matrix pipe meanwhile (4 % at head size 128, 8 % capped)
-        __builtin_amdgcn_s_setprio(1);
+        // two waves per SIMD (head sizes from 96): the one that forms probabilities goes first; both pipes have work from it then,
+        // and the other's score products fill the matrix pipe meanwhile (causal 16384 x 16 heads of 128: 1053 -> 1030 us, capped
+        // 1267 -> 1211).  With three, windows and documents lose 3 % by it
+        if (D > 64) __builtin_amdgcn_s_setprio(1);
         constexpr int N = D / 32;
         uintx4 v[2][N];
 #pragma unroll
@@ -429,7 +429,7 @@ __global__ __launch_bounds__(NW * 64, D <= 64 ? 3 : 2) void attention_kernel(Att
 #pragma unroll
             for (int db = 0; db < N; ++db) o[db] = X::mfma32(__builtin_bit_cast(vec8, v[k & 1][db]), pf[k & 1], o[db]);
             ATT_FENCE();
-            if (k == 2) __builtin_amdgcn_s_setprio(0);
+            if (D > 64 && k == 2) __builtin_amdgcn_s_setprio(0);
         }
     };
     start();
@@ -824,22 +824,21 @@ __global__ __launch_bounds__(256) void attention_join_kernel(AttArgs p) {
 }
 
 template <typename T, bool CAP, bool SLOPES>
-static void att_one(hipStream_t s, const AttArgs &p, int variant, unsigned grid) {
+static void att_one(hipStream_t s, const AttArgs &p, bool tokens, unsigned grid) {
     constexpr int ROWS = 4 * 64 * ATT_D * 2, STEPS = 4 * 2 * 32 * ATT_D * 2, JOIN = 4 * 16 * (ATT_D + 4 + 2) * 4, TOKEN = STEPS > JOIN ? STEPS : JOIN;
-#define ATT_GO(KERNEL, THREADS, LDS)                                                    \
+#define ATT_GO(KERNEL, LDS)                                                             \
     do {                                                                                \
         MIBC_LDS_ATTR_ONCE(KERNEL, LDS);                                                \
-        hipLaunchKernelGGL(KERNEL, dim3(grid), dim3(THREADS), LDS, s, p);               \
+        hipLaunchKernelGGL(KERNEL, dim3(grid), dim3(256), LDS, s, p);                   \
     } while (0)
-    if (variant == ATT_TOKENS) ATT_GO((attention_token_kernel<T, ATT_D, CAP, SLOPES>), 256, TOKEN);
-    else if (variant == ATT_ROWS_128) ATT_GO((attention_kernel<T, ATT_D, 4, CAP, SLOPES>), 256, ROWS);
-    else ATT_GO((attention_kernel<T, ATT_D, 2, CAP, SLOPES>), 128, ROWS);
+    if (tokens) ATT_GO((attention_token_kernel<T, ATT_D, CAP, SLOPES>), TOKEN);
+    else ATT_GO((attention_kernel<T, ATT_D, CAP, SLOPES>), ROWS);
 #undef ATT_GO
 }
 template <typename T>
-static int att_launch(hipStream_t s, const AttArgs &p, int variant, unsigned grid) {
-    if (p.cap_out > 0.0f) p.a.slopes ? att_one<T, true, true>(s, p, variant, grid) : att_one<T, true, false>(s, p, variant, grid);
-    else p.a.slopes ? att_one<T, false, true>(s, p, variant, grid) : att_one<T, false, false>(s, p, variant, grid);
+static int att_launch(hipStream_t s, const AttArgs &p, bool tokens, unsigned grid) {
+    if (p.cap_out > 0.0f) p.a.slopes ? att_one<T, true, true>(s, p, tokens, grid) : att_one<T, true, false>(s, p, tokens, grid);
+    else p.a.slopes ? att_one<T, false, true>(s, p, tokens, grid) : att_one<T, false, false>(s, p, tokens, grid);
     int rc = op_hip(hipGetLastError(), "attention");
     if (rc != MIBC_OK || p.splits == 1) return rc;
     hipLaunchKernelGGL((attention_join_kernel<T, ATT_D>), dim3((unsigned)((int64_t)p.pairs * p.rows)), dim3(256), 0, s, p);
@@ -847,6 +846,6 @@ static int att_launch(hipStream_t s, const AttArgs &p, int variant, unsigned gri
 }
 #define ATT_CAT2(a, b) a##b
 #define ATT_CAT(a, b) ATT_CAT2(a, b)
-int ATT_CAT(mibc_att_launch_, ATT_D)(hipStream_t s, const AttArgs &p, int variant, unsigned grid) {
-    return p.a.type == MIBC_TYPE_F16 ? att_launch<half_t>(s, p, variant, grid) : att_launch<bf16_t>(s, p, variant, grid);
+int ATT_CAT(mibc_att_launch_, ATT_D)(hipStream_t s, const AttArgs &p, bool tokens, unsigned grid) {
+    return p.a.type == MIBC_TYPE_F16 ? att_launch<half_t>(s, p, tokens, grid) : att_launch<bf16_t>(s, p, tokens, grid);
 }

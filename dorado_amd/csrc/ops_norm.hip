@@ -156,7 +156,8 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void rms_norm_kernel(NormArg
         const int chunk = lane + i * TPR, col = chunk * 8;
         if (col >= cols) continue;
         const bool fine = top[i] < INFINITY;
-        const float s = top[i] == 0.0f ? 1.0f : fine ? top[i] / most : NAN;
+        float s = fine ? top[i] / most : NAN;
+        if (s == 0.0f) s = 1.0f;     // nothing but zeros, or values whose scale is below f32
         // the reciprocal of a subnormal scale overflows: such a group divides instead
         const float inv = 1.0f / s;
         const bool tiny = s < 1.2e-38f;

@@ -69,6 +69,13 @@ def test_rms_norm_values():
         assert (s[1] == 1).all() and (q[1].float() == 0).all()
         assert s[2].isnan().all() and (q[2].float() == 0).all()
         assert s[3, 0].isnan() and (s[3, 1:] == 1).all()
+    # values below 448 of f32's smallest: their scale would be 0
+    w = torch.full((64,), 1e-41, device="cuda")
+    for quant in ("int8", "e4m3"):
+        q, s = ops.rms_norm(torch.ones((1, 64), device="cuda"), w * 1e-3, quant=quant)
+        assert float(s) == 1 and (q.float() == 0).all()
+        q, s = ops.rms_norm(torch.ones((1, 64), device="cuda"), w, quant=quant)       # a scale of few bits: codes stay finite
+        assert q.float().isfinite().all() and 0 < float(s) < 1e-40
     b = rnd((2, 64), BF16, 9)
     b[0] = torch.finfo(BF16).min                  # squares beyond f32: the root is infinite and y is 0, as in f32 arithmetic
     assert (ops.rms_norm(b)[0] == 0).all()

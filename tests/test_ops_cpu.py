@@ -70,7 +70,7 @@ def test_rope_refuses(change, code):
 @pytest.mark.parametrize("change,code", [
     (dict(type=2), 1), (dict(type=4), 1), (dict(head_dim=48), 1), (dict(head_dim=256), 1), (dict(heads=0), -1), (dict(kv_heads=0), -1), (dict(heads=3), -1),
     (dict(batch=-1), -1), (dict(q_tokens=-1), -1), (dict(k_tokens=-1), -1), (dict(scale=0.0), -1), (dict(scale=-1.0), -1), (dict(scale=math.nan), -1),
-    (dict(scale=math.inf), -1), (dict(softcap=-1.0), -1), (dict(softcap=math.inf), -1), (dict(softcap=math.nan), -1), (dict(q=0), -1), (dict(k=0), -1), (dict(out=0), -1),
+    (dict(scale=math.inf), -1), (dict(softcap=-1.0), -1), (dict(softcap=math.inf), -1), (dict(softcap=math.nan), -1), (dict(softcap=1e-40), -1), (dict(q=0), -1), (dict(k=0), -1), (dict(out=0), -1),
     (dict(q=P + 8), 1), (dict(v=P + 2), 1), (dict(q_stride=(1024, 129, 64)), 1), (dict(k_stride=(1024, 128, 63)), 1), (dict(k_stride=(1024, -128, 64)), -1),
     (dict(out_stride=(1024, 128, 0)), -1), (dict(out_stride=(0, 128, 64)), -1), (dict(k_stride=(1024, 1 << 25, 64)), 1), (dict(lse=P + 2), -1),
     (dict(doc_offsets=P, n_docs=1), -1), (dict(doc_offsets=P, n_docs=-1, batch=1), -1), (dict(doc_offsets=P, n_docs=1, batch=1, q_tokens=4), -1),
