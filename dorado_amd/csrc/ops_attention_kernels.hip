@@ -76,19 +76,25 @@ __device__ __forceinline__ int att_borders(const int32_t *border, int count, int
     const bool in = lane < count && border[base + min(lane, max(count - 1, 0))] <= t;
     return base + __popcll(__ballot(in));
 }
-// t, and the number of borders <= t of a row of documents
-__device__ __forceinline__ AttRow att_row(const AttArgs &p, int b, int t, int borders) {
+// where in the borders a token's document lies: its index, start and end (no document: an empty one)
+struct AttDoc {
+    int index, start, end;
+};
+__device__ __forceinline__ AttDoc att_doc(const mibc_attention_args &a, int t, int borders, int at, int next) {
+    AttDoc d;     // borders out of order end in some document, whose keys are clamped all the same
+    d.index = min(max(borders - 1, 0), a.n_docs);
+    d.start = min(max(at, 0), a.k_tokens);
+    d.end = borders > 0 && d.index < a.n_docs ? min(max(next, d.start), a.k_tokens) : d.start;
+    return d;
+}
+__device__ __forceinline__ AttRow att_row(const AttArgs &p, int b, int t, const AttDoc &doc) {
     const mibc_attention_args &a = p.a;
     int k0 = 0, k1, pre = 0;
     AttRow r;
-    if (a.doc_offsets != nullptr) {     // borders out of order end in some document, whose keys are clamped all the same
-        const int d = min(max(borders - 1, 0), a.n_docs);
-        k0 = min(max(a.doc_offsets[d], 0), a.k_tokens);
-        k1 = k0;                         // in front of the first document, behind the last: nothing
-        if (borders > 0 && d < a.n_docs) {
-            k1 = min(max(a.doc_offsets[d + 1], k0), a.k_tokens);
-            if (a.prefix != nullptr) pre = a.prefix[d];
-        }
+    if (a.doc_offsets != nullptr) {
+        k0 = doc.start;
+        k1 = doc.end;
+        if (a.prefix != nullptr && k1 > k0) pre = a.prefix[doc.index];
         r.pos = t;
     } else {
         k1 = a.k_len != nullptr ? min(max(a.k_len[b], 0), a.k_tokens) : a.k_tokens;
@@ -175,7 +181,7 @@ __global__ __launch_bounds__(256, D <= 64 ? 3 : 2) void attention_kernel(AttArgs
     constexpr int CH = TILE / 16;               // 16-byte pieces of a tile
     constexpr int NLD = (CH + NT - 1) / NT;
     extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
-    __shared__ int flag;                        // some wave's result holds a NaN
+    __shared__ int flag;                        // some wave's result is not finite
     const unsigned lds = (unsigned)(size_t)(LDSP(unsigned char))smem;
     const mibc_attention_args &a = p.a;
     const int tid = threadIdx.x, lane = tid & 63;
@@ -204,19 +210,39 @@ __global__ __launch_bounds__(256, D <= 64 ? 3 : 2) void attention_kernel(AttArgs
     const int rr = min(row, p.rows - 1), t = p.by_group.div(rr), head = kvh * p.group + (rr - t * p.group);
     const int t_first = p.by_group.div(tile * ROWS), t_last = p.by_group.div(min(tile * ROWS + ROWS, p.rows) - 1);
     const int tt = lane == 32 ? t_first : lane == 33 ? t_last : t;
-    int borders = 0;
+    AttDoc doc{};
     if (a.doc_offsets != nullptr) {
         const int n = a.n_docs + 1, w_first = __builtin_amdgcn_readfirstlane(t), w_last = __builtin_amdgcn_readlane(t, 31);
-        borders = att_borders(a.doc_offsets, n, w_first, lane);
-        for (int i = borders; i < n; ++i) {             // a few borders at most lie between a wave's rows
-            const int at = a.doc_offsets[i];
-            if (at > w_last) break;
-            if (lane < 32 && at <= t) ++borders;
+        int borders, f, g, at, next;
+        if (n <= 64) {      // all borders in the lanes: one load
+            const int mine = a.doc_offsets[min(lane, n - 1)];
+            auto upto = [&](int x) { return (int)__popcll(__ballot(lane < n && mine <= x)); };
+            const int first = upto(w_first), last = upto(w_last);
+            borders = first;
+            for (int i = first; i < last; ++i) borders += __builtin_amdgcn_readlane(mine, i) <= t;     // borders between the wave's rows
+            f = upto(t_first);
+            g = upto(t_last);
+            borders = lane == 32 ? f : lane == 33 ? g : borders;
+            const int d = min(max(borders - 1, 0), n - 1);
+            at = __shfl(mine, d, 64);
+            next = __shfl(mine, min(d + 1, n - 1), 64);
+        } else {
+            borders = att_borders(a.doc_offsets, n, w_first, lane);
+            for (int i = borders; i < n; ++i) {
+                const int x = a.doc_offsets[i];
+                if (x > w_last) break;
+                if (x <= t) ++borders;
+            }
+            f = att_borders(a.doc_offsets, n, t_first, lane);
+            g = att_borders(a.doc_offsets, n, t_last, lane);
+            borders = lane == 32 ? f : lane == 33 ? g : borders;
+            const int d = min(max(borders - 1, 0), n - 1);
+            at = a.doc_offsets[d];
+            next = a.doc_offsets[min(d + 1, n - 1)];
         }
-        const int f = att_borders(a.doc_offsets, n, t_first, lane), g = att_borders(a.doc_offsets, n, t_last, lane);
-        borders = lane == 32 ? f : lane == 33 ? g : borders;
+        doc = att_doc(a, tt, borders, at, next);
     }
-    AttRow see = att_row(p, b, tt, borders);
+    AttRow see = att_row(p, b, tt, doc);
     int w0 = __builtin_amdgcn_readlane(see.lo, 32), w1 = __builtin_amdgcn_readlane(see.hi, 33);
     int p0 = __builtin_amdgcn_readlane(see.plo, 32), p1 = __builtin_amdgcn_readlane(see.phi, 33);
     const bool apart = a.prefix != nullptr && p.back >= 0;
@@ -437,15 +463,16 @@ __global__ __launch_bounds__(256, D <= 64 ? 3 : 2) void attention_kernel(AttArgs
         step(std::integral_constant<int, 0>(), it);
         if (it + 1 < it1) step(std::integral_constant<int, 1>(), it + 1);
     }
-    bool odd = false;
+    float zero[4] = {0.0f, 0.0f, 0.0f, 0.0f};      // 0 * x: 0, or NaN where x is not finite
 #pragma unroll
     for (int db = 0; db < D / 32; ++db)
 #pragma unroll
-        for (int r = 0; r < 16; ++r) odd = odd || o[db][r] != o[db][r];
+        for (int r = 0; r < 16; ++r) zero[r & 3] = fmaf(o[db][r], 0.0f, zero[r & 3]);
+    const bool odd = !(zero[0] + zero[1] + zero[2] + zero[3] == 0.0f);
     if (__any(odd) && lane == 0) flag = 1;
     __syncthreads();
     if (flag) {
-        // a NaN: from a value or key that the row sees, or 0 * (a value that it does not see).  Once more, tile by tile: values
+        // something is not finite: from a value or key that the row sees, or 0 * (a value that it does not see).  Once more, tile by tile: values
         // that are not finite stay out of the products, and the places of NaN (kind 0), infinity (1) and -infinity (2) are
         // multiplied with the mask instead, so that they reach the rows that see their key and no other
         start();
@@ -493,7 +520,7 @@ __global__ __launch_bounds__(256, D <= 64 ? 3 : 2) void attention_kernel(AttArgs
 
     l = att_half_add(l);
     const float base = m == -INFINITY ? 0.0f : m;
-    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+    const float inv = l == 0.0f ? 0.0f : __builtin_amdgcn_rcpf(l);
     {   // row, token and head are worked out again rather than kept in registers over the loop
         const AttArgs &p = att_args_again();
         const mibc_attention_args &a = p.a;
@@ -554,10 +581,14 @@ __global__ __launch_bounds__(256, 2) void attention_token_kernel(AttArgs p) {
     const int b = p.by_kv.div(pair), kvh = pair - b * a.kv_heads;
 
     const int rr = min(l15, p.rows - 1), t = p.by_group.div(rr), head = kvh * p.group + (rr - t * p.group);
-    int borders = 0;
-    if (a.doc_offsets != nullptr)
+    AttDoc doc{};
+    if (a.doc_offsets != nullptr) {
+        int borders = 0;
         for (int i = 0; i < a.n_docs + 1 && a.doc_offsets[i] < a.q_tokens; ++i) borders += a.doc_offsets[i] <= t;   // at most 16 tokens
-    const AttRow see = att_row(p, b, t, borders);
+        const int d = min(max(borders - 1, 0), a.n_docs);
+        doc = att_doc(a, t, borders, a.doc_offsets[d], a.doc_offsets[min(d + 1, a.n_docs)]);
+    }
+    const AttRow see = att_row(p, b, t, doc);
     // rows grow with the lane up to the last, which lane 15 repeats
     const int lo_min = __builtin_amdgcn_readfirstlane(see.lo), lo_max = __builtin_amdgcn_readlane(see.lo, 15);
     const int hi_min = __builtin_amdgcn_readfirstlane(see.hi), hi_max = __builtin_amdgcn_readlane(see.hi, 15);

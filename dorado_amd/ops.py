@@ -120,21 +120,27 @@ def rms_norm(x, weight=None, *, residual=None, alpha: float = 1.0, eps: float = 
             raise MibcError("rms_norm: the columns must be a multiple of group")
         out_dtype, groups = _QUANT[quant], cols // group if group else 1
         scale = torch.empty(shape[:-1] + (groups,), dtype=torch.float32, device=x.device)
+    xs = cols if x.is_contiguous() else _row_stride("rms_norm", "x", x, cols)
+    rs = ss = os_ = cols
+    if residual is not None and not residual.is_contiguous():
+        rs = _row_stride("rms_norm", "residual", residual, cols)
     if out is None:
         out = _new(x) if quant is None else torch.empty(shape, dtype=out_dtype, device=x.device)
     elif out.shape != shape or out.dtype is not out_dtype:
         raise MibcError(f"rms_norm: out must be {list(shape)} {out_dtype}")
+    elif not out.is_contiguous():
+        os_ = _row_stride("rms_norm", "out", out, cols)
     if sum_out is None:
         if return_sum:
             sum_out = _new(x)
     elif sum_out.shape != shape or sum_out.dtype is not dtype:
         raise MibcError(f"rms_norm: sum_out must be {list(shape)} {dtype}")
+    elif not sum_out.is_contiguous():
+        ss = _row_stride("rms_norm", "sum_out", sum_out, cols)
     args = _NORM_ARGS.pack(
         x.data_ptr(), 0 if residual is None else residual.data_ptr(), 0 if weight is None else weight.data_ptr(),
         0 if sum_out is None else sum_out.data_ptr(), out.data_ptr(), 0 if scale is None else scale.data_ptr(), x.numel() // cols,
-        _row_stride("rms_norm", "x", x, cols), 0 if residual is None else _row_stride("rms_norm", "residual", residual, cols),
-        0 if sum_out is None else _row_stride("rms_norm", "sum_out", sum_out, cols), _row_stride("rms_norm", "out", out, cols), groups,
-        cols, _TYPE[dtype], _TYPE[dtype if weight is None else weight.dtype], _TYPE[out_dtype], group, alpha, eps, 0)
+        xs, rs, ss, os_, groups, cols, _TYPE[dtype], _TYPE[dtype if weight is None else weight.dtype], _TYPE[out_dtype], group, alpha, eps, 0)
     rc = (_fns or _entry())[0](dev, _stream(dev), args)
     if rc:
         _check(rc, "rms_norm")
