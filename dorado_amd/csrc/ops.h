@@ -41,22 +41,38 @@ static inline int op_hip(hipError_t rc, const char *what) {
 static inline int op_type_bytes(int type) { return type == MIBC_TYPE_F32 ? 4 : (type == MIBC_TYPE_I8 || type == MIBC_TYPE_E4M3) ? 1 : 2; }
 static inline bool op_aligned(const void *p, unsigned bytes) { return ((uintptr_t)p & (bytes - 1)) == 0; }
 
-// eight consecutive elements <-> f32; the 16-bit ones round to nearest even (v_cvt_pk_*_f32)
+// eight consecutive elements <-> f32; the 16-bit ones round to nearest even (v_cvt_pk_*_f32).  ANY: at any address (global memory
+// takes 16-byte accesses there too, at about two thirds of the rate)
+template <typename V, bool ANY>
+__device__ __forceinline__ V op_get(const void *p) {
+    if (!ANY) return *(const V *)p;
+    V v;
+    __builtin_memcpy(&v, p, sizeof(V));
+    return v;
+}
+template <typename V, bool ANY>
+__device__ __forceinline__ void op_put(void *p, V v) {
+    if (!ANY) *(V *)p = v;
+    else __builtin_memcpy(p, &v, sizeof(V));
+}
+template <bool ANY = false>
 __device__ __forceinline__ void op_load8(const half_t *p, float v[8]) {
-    const half8_t x = *(const half8_t *)p;
+    const half8_t x = op_get<half8_t, ANY>(p);
 #pragma unroll
     for (int i = 0; i < 8; ++i) v[i] = (float)x[i];
 }
+template <bool ANY = false>
 __device__ __forceinline__ void op_load8(const bf16_t *p, float v[8]) {
-    const uintx4 x = *(const uintx4 *)p;
+    const uintx4 x = op_get<uintx4, ANY>(p);
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         v[2 * i] = __uint_as_float(x[i] << 16);
         v[2 * i + 1] = __uint_as_float(x[i] & 0xffff0000u);
     }
 }
+template <bool ANY = false>
 __device__ __forceinline__ void op_load8(const float *p, float v[8]) {
-    const floatx4 a = *(const floatx4 *)p, b = *(const floatx4 *)(p + 4);
+    const floatx4 a = op_get<floatx4, ANY>(p), b = op_get<floatx4, ANY>(p + 4);
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         v[i] = a[i];
@@ -71,15 +87,15 @@ __device__ __forceinline__ unsigned op_pack2(float a, float b, bf16_t) {
     const float2_ops x = {a, b};
     return __builtin_bit_cast(unsigned, __builtin_convertvector(x, bf16x2_t));
 }
-template <typename T>
+template <typename T, bool ANY = false>
 __device__ __forceinline__ void op_store8(T *p, const float v[8]) {
-    uintx4 x;
+    if constexpr (sizeof(T) == 4) {
+        op_put<floatx4, ANY>(p, (floatx4){v[0], v[1], v[2], v[3]});
+        op_put<floatx4, ANY>(p + 4, (floatx4){v[4], v[5], v[6], v[7]});
+    } else {
+        uintx4 x;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) x[i] = op_pack2(v[2 * i], v[2 * i + 1], T());
-    *(uintx4 *)p = x;
-}
-template <>
-__device__ __forceinline__ void op_store8<float>(float *p, const float v[8]) {
-    *(floatx4 *)p = (floatx4){v[0], v[1], v[2], v[3]};
-    *(floatx4 *)(p + 4) = (floatx4){v[4], v[5], v[6], v[7]};
+        for (int i = 0; i < 4; ++i) x[i] = op_pack2(v[2 * i], v[2 * i + 1], T());
+        op_put<uintx4, ANY>(p, x);
+    }
 }

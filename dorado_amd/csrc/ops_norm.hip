@@ -14,6 +14,8 @@ template <typename T, bool VEC>
 __device__ __forceinline__ void norm_load(const T *row, int col, int cols, float v[8]) {
     if (VEC) {
         op_load8(row + col, v);
+    } else if (col + 8 <= cols) {
+        op_load8<true>(row + col, v);
     } else {
 #pragma unroll
         for (int i = 0; i < 8; ++i) v[i] = (col + i < cols) ? (float)row[col + i] : 0.0f;
@@ -23,6 +25,8 @@ template <typename T, bool VEC>
 __device__ __forceinline__ void norm_store(T *row, int col, int cols, const float v[8]) {
     if (VEC) {
         op_store8<T>(row + col, v);
+    } else if (col + 8 <= cols) {
+        op_store8<T, true>(row + col, v);
     } else {
 #pragma unroll
         for (int i = 0; i < 8; ++i)
@@ -30,23 +34,30 @@ __device__ __forceinline__ void norm_store(T *row, int col, int cols, const floa
     }
 }
 
-__device__ __forceinline__ float op_add(float a, float b) { return a + b; }
-__device__ __forceinline__ float op_max(float a, float b) { return fmaxf(a, b); }
 // over the TPR threads that hold a row; `red`: one slot per wave
-template <int TPR, bool MAX>
-__device__ __forceinline__ float norm_reduce(float v, float *red) {
+template <int TPR>
+__device__ __forceinline__ float norm_reduce_sum(float v, float *red) {
 #pragma unroll
-    for (int o = (TPR < 64 ? TPR : 64) / 2; o > 0; o >>= 1) {
-        const float w = __shfl_xor(v, o, 64);
-        v = MAX ? op_max(v, w) : op_add(v, w);
-    }
+    for (int o = (TPR < 64 ? TPR : 64) / 2; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
     if (TPR > 64) {
-        const int wave = threadIdx.x >> 6;
-        if ((threadIdx.x & 63) == 0) red[wave] = v;
+        if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
         __syncthreads();
         v = red[0];
 #pragma unroll
-        for (int i = 1; i < TPR / 64; ++i) v = MAX ? op_max(v, red[i]) : op_add(v, red[i]);
+        for (int i = 1; i < TPR / 64; ++i) v += red[i];
+    }
+    return v;
+}
+template <int TPR>
+__device__ __forceinline__ unsigned norm_reduce_max(unsigned v, unsigned *red) {
+#pragma unroll
+    for (int o = (TPR < 64 ? TPR : 64) / 2; o > 0; o >>= 1) v = max(v, (unsigned)__shfl_xor((int)v, o, 64));
+    if (TPR > 64) {
+        if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
+        __syncthreads();
+        v = red[0];
+#pragma unroll
+        for (int i = 1; i < TPR / 64; ++i) v = max(v, red[i]);
     }
     return v;
 }
@@ -95,7 +106,7 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void rms_norm_kernel(NormArg
             if (col < cols) norm_store<T, VEC>(o, col, cols, h[i]);
         }
     }
-    ss = norm_reduce<TPR, false>(ss, red[0]);
+    ss = norm_reduce_sum<TPR>(ss, red[0]);
     const float rstd = 1.0f / sqrtf(ss / (float)cols + a.eps);
     // y replaces h
 #pragma unroll
@@ -122,22 +133,19 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void rms_norm_kernel(NormArg
         }
         return;
     }
-    // 8-bit output.  A value that is not finite makes the group's maximum infinite, and its scale NaN.
-    float top[NCH];
-    float all = 0.0f;
+    // 8-bit output.  Magnitudes are compared as whole numbers: NaN and infinity are larger than every finite value then
+    unsigned top[NCH];
+    unsigned all = 0;
 #pragma unroll
     for (int i = 0; i < NCH; ++i) {
-        top[i] = 0.0f;
+        top[i] = 0;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            const float m = fabsf(h[i][e]);
-            top[i] = fmaxf(top[i], m <= 3.402823466e38f ? m : INFINITY);   // columns behind the row hold zeros
-        }
-        all = fmaxf(all, top[i]);
+        for (int e = 0; e < 8; ++e) top[i] = max(top[i], __float_as_uint(h[i][e]) & 0x7fffffffu);   // columns behind the row hold zeros
+        all = max(all, top[i]);
     }
     const float most = a.out_type == MIBC_TYPE_I8 ? 127.0f : 448.0f;
     if (a.group == 0) {
-        all = norm_reduce<TPR, true>(all, red[1]);
+        all = norm_reduce_max<TPR>(all, (unsigned *)red[1]);
 #pragma unroll
         for (int i = 0; i < NCH; ++i) top[i] = all;
     } else {   // a group is group / 8 = 4, 8 or 16 neighbouring lanes of one chunk index
@@ -145,8 +153,8 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void rms_norm_kernel(NormArg
         for (int i = 0; i < NCH; ++i)
 #pragma unroll
             for (int o = 1; o < 16; o <<= 1) {
-                const float w = __shfl_xor(top[i], o, 64);
-                top[i] = (o * 8 < a.group) ? fmaxf(top[i], w) : top[i];
+                const unsigned w = (unsigned)__shfl_xor((int)top[i], o, 64);
+                top[i] = (o * 8 < a.group) ? max(top[i], w) : top[i];
             }
     }
     uint8_t *o = (uint8_t *)a.out + row * a.out_stride;
@@ -155,24 +163,23 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void rms_norm_kernel(NormArg
     for (int i = 0; i < NCH; ++i) {
         const int chunk = lane + i * TPR, col = chunk * 8;
         if (col >= cols) continue;
-        const bool fine = top[i] < INFINITY;
-        float s = fine ? top[i] / most : NAN;
+        const bool fine = top[i] < 0x7f800000u;
+        float s = fine ? __uint_as_float(top[i]) / most : NAN;
         if (s == 0.0f) s = 1.0f;     // nothing but zeros, or values whose scale is below f32
-        // the reciprocal of a subnormal scale overflows: such a group divides instead
-        const float inv = 1.0f / s;
-        const bool tiny = s < 1.2e-38f;
+        // the reciprocal of a scale below 2^-126 overflows: both sides are lifted by 2^64 first
+        const float lift = s < 1e-30f ? 0x1p64f : 1.0f, inv = 1.0f / (s * lift);
         unsigned lo = 0, hi = 0;
         if (fine) {
-            float v[8];
+            float v[8];              // at most 127 or 448 times 1 + 2^-22: rounds to the largest code
 #pragma unroll
-            for (int e = 0; e < 8; ++e) v[e] = tiny ? h[i][e] / s : h[i][e] * inv;
+            for (int e = 0; e < 8; ++e) v[e] = h[i][e] * lift * inv;
             if (a.out_type == MIBC_TYPE_I8) {
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    lo |= ((unsigned)(int)rintf(fminf(fmaxf(v[e], -127.0f), 127.0f)) & 0xffu) << (8 * e);
-                    hi |= ((unsigned)(int)rintf(fminf(fmaxf(v[4 + e], -127.0f), 127.0f)) & 0xffu) << (8 * e);
+                    lo |= ((unsigned)(int)rintf(v[e]) & 0xffu) << (8 * e);
+                    hi |= ((unsigned)(int)rintf(v[4 + e]) & 0xffu) << (8 * e);
                 }
-            } else {   // |v| <= 448 (1 + 2^-22): rounds to 448, below the conversion's NaN range (> 464)
+            } else {                 // the conversion's NaN range begins above 464
                 lo = __builtin_amdgcn_cvt_pk_fp8_f32(v[0], v[1], lo, false);
                 lo = __builtin_amdgcn_cvt_pk_fp8_f32(v[2], v[3], lo, true);
                 hi = __builtin_amdgcn_cvt_pk_fp8_f32(v[4], v[5], hi, false);
@@ -181,6 +188,8 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void rms_norm_kernel(NormArg
         }
         if (VEC) {
             *(uintx2 *)(o + col) = (uintx2){lo, hi};
+        } else if (col + 8 <= cols) {
+            op_put<uintx2, true>(o + col, (uintx2){lo, hi});
         } else {
 #pragma unroll
             for (int e = 0; e < 8; ++e)
@@ -202,6 +211,7 @@ static void norm_launch(hipStream_t s, const NormArgs &n) {
     else if (chunks <= 256) NORM_GO(64, 4, 256);
     else if (chunks <= 512) NORM_GO(256, 2, 256);
     else if (chunks <= 1024) NORM_GO(256, 4, 256);
+    else if (chunks <= 1536) NORM_GO(256, 6, 256);
     else NORM_GO(1024, 4, 1024);
 #undef NORM_GO
 }
@@ -236,7 +246,7 @@ static int norm_check(const mibc_rms_norm_args &a, bool *vec) {
     if (!op_aligned(a.x, eb) || !op_aligned(a.residual, eb) || !op_aligned(a.sum_out, eb) || !op_aligned(a.weight, (unsigned)op_type_bytes(a.weight_type)) ||
         !op_aligned(a.out, (unsigned)op_type_bytes(a.out_type)) || !op_aligned(a.scale_out, 4))
         return op_refuse(MIBC_ERR_ARG, "rms_norm: pointer not aligned to its type");
-    // 16-byte accesses where every row of every tensor allows them, single elements elsewhere
+    // aligned 16-byte accesses where every row of every tensor allows them, unaligned ones and single elements at a row's end elsewhere
     *vec = a.cols % 8 == 0 && op_aligned(a.x, 16) && a.x_stride % 8 == 0 && op_aligned(a.weight, 16) &&
            (a.residual == nullptr || (op_aligned(a.residual, 16) && a.residual_stride % 8 == 0)) &&
            (a.sum_out == nullptr || (op_aligned(a.sum_out, 16) && a.sum_stride % 8 == 0)) &&
