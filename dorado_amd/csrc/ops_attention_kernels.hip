@@ -45,6 +45,8 @@ __device__ __forceinline__ uintx2 att_lds_tr(unsigned addr) {
 #define ATT_FENCE() __builtin_amdgcn_sched_barrier(0)     // the compiler moves nothing across
 
 __device__ __forceinline__ float att_exp2(float x) { return __builtin_amdgcn_exp2f(x); }
+// f x for weights f >= 0: an infinity that a row sees stays one, also where the weight is 0 in f32
+__device__ __forceinline__ float att_weigh(float f, float x) { return __builtin_isinf(x) ? x : f * x; }
 // over the two half waves
 __device__ __forceinline__ float att_half_max(float x) {
     const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
@@ -161,7 +163,13 @@ __device__ __forceinline__ uintx4 att_places(uintx4 v, int kind) {
 //   S^T[key][row] = K Q^T   on 32x32x16: lane (row = lane & 31, half = lane >> 5) holds keys 8 g + 4 half + 0..3 of each 32
 //   O^T[dim][row] = V^T P^T  takes P^T from those very registers: the 16 k-slots of a step are enumerated as the keys a lane holds,
 //   and V^T comes out of the row-major V tile through transposing LDS reads (ds_read_b64_tr_b16).
-// A row's maximum and sum are one lane pair's: no exchange but one half-wave swap per tile.
+// A row's maximum and sum are one lane pair's: no exchange but one half-wave swap per tile.  Operands are read four instructions
+// ahead, and the products of 16 keys with V run beside the probabilities of the next 16.
+// Head size 128: the matrix pipe works 0.54 of the cycles beside 170 plain instructions per tile and wave (1024 matrix cycles), and power
+// holds the clock at 1.7 GHz: 8192 x 16 heads 496 - 515 us, causal 16384 x 16 heads 996 - 1030 us (1060 - 1104 TFLOP/s over two cards; a
+// library product of 8192^3 1229).  Capped scores, 298 plain instructions (an exponential and a reciprocal more per score): causal
+// 1157 - 1212 us (906 - 950 TFLOP/s).  Head size 64, as many exponentials for half the products: 4 x 16 heads x 4096 321 us
+// (856 TFLOP/s), with three waves per SIMD; two 334 us.
 template <int D>
 __device__ __forceinline__ int att_k_slot(int row, int chunk) {   // 16-byte column of the K tile in LDS
     return D == 128 ? chunk ^ (row & 15) : D == 64 ? chunk ^ ((row >> 1) & 7) : chunk ^ ((row >> 2) & 3);
@@ -384,7 +392,7 @@ __global__ __launch_bounds__(256, D <= 64 ? 3 : 2) void attention_kernel(AttArgs
         }
     };
     float off;
-    auto maxima = [&]() {
+    auto maxima = [&](auto safe_) {     // safe_: o may hold infinities
         float top = s[0][0];
         ATT_EACH top = score.larger(top, s[i][r]);
         top = att_half_max(fmaf(top, score.mul, score.add));
@@ -398,7 +406,7 @@ __global__ __launch_bounds__(256, D <= 64 ? 3 : 2) void attention_kernel(AttArgs
 #pragma unroll
             for (int db = 0; db < D / 32; ++db)
 #pragma unroll
-                for (int r = 0; r < 16; ++r) o[db][r] *= f;
+                for (int r = 0; r < 16; ++r) o[db][r] = decltype(safe_)::value ? att_weigh(f, o[db][r]) : o[db][r] * f;
         }
         off = score.add - (m == -INFINITY ? 0.0f : m);
     };
@@ -432,7 +440,7 @@ __global__ __launch_bounds__(256, D <= 64 ? 3 : 2) void attention_kernel(AttArgs
         if (it + 1 < it1) fetch(it + 1, decltype(stage_)::value ^ 1);      // behind the reads of K, which it would hold up
         shape(j0);
         if (j0 < lo_max || j0 + 64 > hi_min) hide(j0);
-        maxima();
+        maxima(std::false_type());
         // the products of 16 keys run beside the probabilities of the next 16, whose values are read meanwhile
         // two waves per SIMD (head sizes from 96): the one that forms probabilities goes first; both pipes have work from it then,
         // and the other's score products fill the matrix pipe meanwhile (causal 16384 x 16 heads of 128: 1053 -> 1030 us, capped
@@ -486,7 +494,7 @@ __global__ __launch_bounds__(256, D <= 64 ? 3 : 2) void attention_kernel(AttArgs
             products(0);
             shape(j0);
             const unsigned seen = hide_all(j0);
-            maxima();
+            maxima(std::true_type());
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
                 const vec8 pf = probabilities(k);
@@ -558,6 +566,8 @@ __global__ __launch_bounds__(256, D <= 64 ? 3 : 2) void attention_kernel(AttArgs
 // the few hundred cycles of its score instructions, 128 KB per CU.  16x16x32 instructions: S^T[key][row], lane (row = lane & 15,
 // quarter = lane >> 4) holds keys 4 quarter + 0..3 of each 16, which are its k-slots in O^T[dim][row] = V^T P^T.  Matrix work is
 // free here, so P goes in as two 16-bit parts (value and remainder): the result is rounded once, at the end.
+// Measured: 48 x 8 pairs over 2048 .. 8192 keys of 128 bf16 219 us (5.0 TB/s), one token of 2 pairs over 131072 keys 34 us, 32 x 16 pairs
+// over 4096 keys of 64 f16 109 us (4.9 TB/s).
 template <int D>
 __device__ __forceinline__ int att_v_slot16(int row, int chunk) {
     return D == 128 ? chunk ^ (((row & 3) << 2) | ((row & 4) >> 1)) : D == 64 ? chunk ^ ((((row >> 1) & 1) << 2) | ((row & 4) >> 1)) : chunk;
@@ -702,7 +712,7 @@ __global__ __launch_bounds__(256, 2) void attention_token_kernel(AttArgs p) {
 #pragma unroll
                 for (int db = 0; db < D / 16; ++db)
 #pragma unroll
-                    for (int r = 0; r < 4; ++r) o[db][r] *= f;
+                    for (int r = 0; r < 4; ++r) o[db][r] = SAFE ? att_weigh(f, o[db][r]) : o[db][r] * f;
             }
             const float off = score.add - (m == -INFINITY ? 0.0f : m);
             uintx4 hi, lo;
@@ -782,11 +792,10 @@ __global__ __launch_bounds__(256, 2) void attention_token_kernel(AttArgs p) {
 #pragma unroll
         for (int w = 0; w < 4; ++w) {
             const float f = sm[w * 16 + r] == -INFINITY ? (sl[w * 16 + r] == 0.0f ? 0.0f : 1.0f) : att_exp2(sm[w * 16 + r] - base);
-            if (f == 0.0f) continue;
             sum = fmaf(f, sl[w * 16 + r], sum);
-            const floatx4 x = *(const floatx4 *)(so + (w * 16 + r) * OLD + d4);
+            const floatx4 x = *(const floatx4 *)(so + (w * 16 + r) * OLD + d4);      // zeros for a wave without keys
 #pragma unroll
-            for (int e = 0; e < 4; ++e) y[e] = fmaf(f, x[e], y[e]);
+            for (int e = 0; e < 4; ++e) y[e] += att_weigh(f, x[e]);
         }
         const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
         const int rt = p.by_group.div(r), rh = kvh * p.group + (r - rt * p.group);
@@ -835,7 +844,7 @@ __global__ __launch_bounds__(256) void attention_join_kernel(AttArgs p) {
             const float w = att_exp2(pl[s] - base);
             sum += w;
 #pragma unroll
-            for (int e = 0; e < 4; ++e) y[e] = w == 0.0f ? y[e] : fmaf(w, x[e], y[e]);   // a part without keys holds zeros
+            for (int e = 0; e < 4; ++e) y[e] += att_weigh(w, x[e]);      // a part without keys holds zeros
         }
         *(floatx4 *)(&red[g][d4]) = y;
         if (d4 == 0) red[g][D] = sum;

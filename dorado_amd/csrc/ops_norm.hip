@@ -3,7 +3,11 @@
 // A few flops per element against 2-8 bytes: bound by HBM.  So a row is read once, stays in f32 registers (TPR threads hold
 // NCH chunks of 8 consecutive columns each) through both reductions (sum of squares, then max |y| where the output has 8 bits)
 // and leaves once.  Rows of up to 2048 columns take one wave (or a quarter of one) and reduce by lane shuffles alone; wider ones
-// take a workgroup and one LDS exchange per reduction.
+// take a workgroup and one LDS exchange per reduction: as few threads as hold the row in six chunks (11320 columns: 256 threads x 6
+// chunks 39 us, 1024 x 2 54), 1024 beyond.
+// Measured: 262144 x 512 f16 with residual 134 us (6.0 TB/s), 16383 x 4096 bf16 with residual, sum and e4m3 codes per 128 columns
+// 89 us (5.3 TB/s), 10000 x 5001 bf16 (unaligned rows) 73 us (4.1 TB/s), 3794 x 11320 e4m3 39 us (3.3 TB/s: the conversion's
+// instructions).
 #include "ops.h"
 
 struct NormArgs {

@@ -281,7 +281,7 @@ def attention(q, k, v, *, scale=None, causal: bool = False, window=(-1, -1), sof
             back, ahead, q_start, d ** -0.5 if scale is None else scale, softcap, 0)
     _, _, run, workspace = _fns or _entry()
     args = _ATTN_ARGS.pack(*head, 0, 0, *tail)
-    need = workspace(args)
+    need = workspace(args) if m >= 512 else 0      # fewer keys are never split
     if need:
         room = torch.empty(need, dtype=torch.uint8, device=q.device)
         args = _ATTN_ARGS.pack(*head, room.data_ptr(), need, *tail)

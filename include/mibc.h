@@ -302,9 +302,11 @@ MIBC_API int mibc_rope_frequencies(int scaling, int rot_dim, double theta, doubl
  * document d is the tokens [doc_offsets[d], doc_offsets[d + 1]); a token sees its own document only, prefix is then [n_docs] and
  * counts from the document's start, tokens in no document see nothing and are seen by none.  A query that sees nothing, or only
  * scores of -infinity, gives zeros and lse = -infinity.  What a query does not see has no influence on its result, whatever it
- * holds (NaN and infinity included).  lse (optional) [batch][heads][q_tokens] f32 contiguous: log of the sum of exp(scores).
+ * holds (NaN and infinity included); a NaN or infinity of v that it does see reaches it, however small its weight.  lse (optional)
+ * [batch][heads][q_tokens] f32 contiguous: log of the sum of exp(scores).
  * Types F16, BF16; head_dim 32, 64, 96 or 128; token and head strides multiples of 8 elements, pointers aligned to 16 bytes.
- * workspace: mibc_attention_workspace(a) bytes on the device (0: may be NULL), the call's own until it has completed. */
+ * workspace: mibc_attention_workspace(a) bytes on the device (0, as for any call with fewer than 512 keys: may be NULL), the
+ * call's own until it has completed. */
 #define MIBC_ATTN_END (-2147483647 - 1)
 typedef struct mibc_attention_args {
     const void *q, *k, *v;

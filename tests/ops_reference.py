@@ -142,12 +142,15 @@ def attention(q, k, v, scale=None, window=(-1, -1), softcap=0.0, slopes=None, k_
             o = p[:, ~strange] @ vv[~strange]
             for j in strange.nonzero()[:, 0].tolist():
                 o = o + torch.where(hidden[:, j, None], zero, p[:, j, None] * vv[j])
-            av = p[:, ~strange] @ vv[~strange].abs()
+            # a column's bound sums over all its finite values, those of keys with a NaN or infinity in another column too: their
+            # rounded probabilities enter this column like any other key's
+            size_v = vv.abs().masked_fill(~vv.isfinite(), 0.0)
+            av = p @ size_v
             e = es.masked_fill(hidden, 0.0).nan_to_num(0.0, 0.0, 0.0).amax(1, keepdim=True) if m else torch.zeros(n, 1, dtype=F64)
             div = torch.where(total == 0, torch.ones_like(total), total)
             out[x, :, y] = torch.where(empty[:, None], zero, o / div)
             # probabilities rounded to t (f16: to 2^-25 below 2^-14), sums of m terms in f32, joins of parts
-            sub = (~hidden[:, ~strange]).to(F64) @ vv[~strange].abs() * (2.0 ** -25 if t is torch.float16 else 0.0)
+            sub = (~hidden).to(F64) @ size_v * (2.0 ** -25 if t is torch.float16 else 0.0)
             tol[x, :, y] = (av * (u(t) + 2 * e + 2.0 ** -19) + sub) / div + u(t) * out[x, :, y].abs() + 2.0 ** -25
             lse[x, y] = torch.where(empty, torch.full_like(base[:, 0], -math.inf), base[:, 0] + torch.log(total[:, 0]))
             ltol[x, y] = e[:, 0] + 2.0 ** -19 + 2.0 ** -21 * lse[x, y].abs().nan_to_num(0.0, 0.0, 0.0)

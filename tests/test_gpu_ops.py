@@ -247,6 +247,16 @@ def test_attention_hidden_values(what, t, d, n):
     check(q, k2, v2, causal=True, k_len=lens)
 
 
+@pytest.mark.parametrize("d", [32, 128])
+@pytest.mark.parametrize("n,m", [(1, 130), (1, 1200), (5, 300), (5, 1200), (40, 300), (40, 1200), (200, 1200)])
+def test_attention_seen_values_of_no_weight(n, m, d):
+    # a slope of 0.5 takes keys that are 210 away to weights below the smallest f32: their NaN and infinities arrive all the same,
+    # in a pass over one part, in the join of waves and in that of parts
+    q, k, v = qkv(2, n, m, 2, 1, d, BF16, 61)
+    v[0, 0, 0, 1], v[0, 2, 0, 2], v[0, 3, 0, 3], v[1, m // 2, 0, 5], v[1, m // 3, 0, 5] = math.nan, math.inf, -math.inf, math.inf, -math.inf
+    check(q, k, v, slopes=torch.tensor([0.5, 0.01]).cuda())
+
+
 def test_attention_extreme_scores():
     q, k, v = qkv(1, 70, 140, 2, 1, 64, F16, 70)
     check(q * 20, k * 20, v)                                   # one key takes all
