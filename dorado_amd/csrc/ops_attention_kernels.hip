@@ -566,7 +566,7 @@ __global__ __launch_bounds__(256, D <= 64 ? 3 : 2) void attention_kernel(AttArgs
 // the few hundred cycles of its score instructions, 128 KB per CU.  16x16x32 instructions: S^T[key][row], lane (row = lane & 15,
 // quarter = lane >> 4) holds keys 4 quarter + 0..3 of each 16, which are its k-slots in O^T[dim][row] = V^T P^T.  Matrix work is
 // free here, so P goes in as two 16-bit parts (value and remainder): the result is rounded once, at the end.
-// Measured: 48 x 8 pairs over 2048 .. 8192 keys of 128 bf16 219 us (5.0 TB/s), one token of 2 pairs over 131072 keys 34 us, 32 x 16 pairs
+// Measured: 48 x 8 pairs over 2048 .. 8192 keys of 128 bf16 219 us (5.0 TB/s), one token of 2 pairs over 131072 keys 32 us, 32 x 16 pairs
 // over 4096 keys of 64 f16 109 us (4.9 TB/s).
 template <int D>
 __device__ __forceinline__ int att_v_slot16(int row, int chunk) {
@@ -814,6 +814,8 @@ __global__ __launch_bounds__(256, 2) void attention_token_kernel(AttArgs p) {
 
 // ------------------------------------------------------------------------------------------------------------------
 // Joins the parts of a row: one workgroup per row, D / 4 threads per part, 256 / (D / 4) parts at a time.
+// Bound by latency (a few KB per row): eight loads per thread in flight, the first ones beside the search for the maximum (16 rows of 116
+// parts 7.0 -> 4.8 us); slots without a part are skipped by the whole wave (1536 rows of 5 parts 4.8 us, 7.1 with idle slots).
 template <typename T, int D>
 __global__ __launch_bounds__(256) void attention_join_kernel(AttArgs p) {
     constexpr int TP = D / 4, G = 256 / TP;     // threads per part, parts at a time (D 96: 24 and 10, the last threads idle)
@@ -827,6 +829,20 @@ __global__ __launch_bounds__(256) void attention_join_kernel(AttArgs p) {
     const int t = p.by_group.div(row), head = kvh * p.group + (row - t * p.group);
     const float *pl = p.part_l + r * p.splits;
     const float *po = p.part_o + r * p.splits * D;
+    const int g = tid / TP, d4 = tid % TP * 4;
+    floatx4 x[8];      // eight parts in flight per thread, the first ones while the maximum is found
+    float w[8];
+    auto fetch = [&](int first) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            if (first + i * G < p.splits) {
+                const int s = first + i * G + g;
+                const bool in = g < G && s < p.splits;
+                x[i] = in ? *(const floatx4 *)(po + (int64_t)s * D + d4) : (floatx4)(0.0f);
+                w[i] = in ? pl[s] : -INFINITY;
+            }
+    };
+    fetch(0);
     float m = -INFINITY;
     for (int s = tid; s < p.splits; s += 256) m = fmaxf(m, pl[s]);
 #pragma unroll
@@ -835,17 +851,22 @@ __global__ __launch_bounds__(256) void attention_join_kernel(AttArgs p) {
     __syncthreads();
     m = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
     const float base = m == -INFINITY ? 0.0f : m;
-    const int g = tid / TP, d4 = tid % TP * 4;
     float sum = 0.0f;
     floatx4 y = (floatx4)(0.0f);
-    if (g < G) {
-        for (int s = g; s < p.splits; s += G) {
-            const floatx4 x = *(const floatx4 *)(po + (int64_t)s * D + d4);
-            const float w = att_exp2(pl[s] - base);
-            sum += w;
+    for (int first = 0;;) {
 #pragma unroll
-            for (int e = 0; e < 4; ++e) y[e] += att_weigh(w, x[e]);      // a part without keys holds zeros
-        }
+        for (int i = 0; i < 8; ++i)
+            if (first + i * G < p.splits) {
+                const float f = att_exp2(w[i] - base);
+                sum += f;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) y[e] += att_weigh(f, x[i][e]);      // a part without keys holds zeros
+            }
+        first += 8 * G;
+        if (first >= p.splits) break;
+        fetch(first);
+    }
+    if (g < G) {
         *(floatx4 *)(&red[g][d4]) = y;
         if (d4 == 0) red[g][D] = sum;
     }
