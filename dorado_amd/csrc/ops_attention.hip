@@ -98,6 +98,8 @@ static uint64_t att_room(const mibc_attention_args &a, const AttPlan &p) {
     return p.splits == 1 ? 0 : (uint64_t)a.batch * a.heads * a.q_tokens * p.splits * (a.head_dim + 1) * 4;
 }
 static int att_check_plan(const mibc_attention_args &a, const AttPlan &p) {
+    // a workgroup writes its rows while others still read keys and values
+    if (a.k_tokens > 0 && (a.out == a.k || a.out == a.v)) return op_refuse(MIBC_ERR_ARG, "attention: out may be q, but not k or v");
     if ((int64_t)a.batch * a.kv_heads * p.tiles * p.splits > 0x7fffffff) return op_refuse(MIBC_NOT_SUPPORTED, "attention: too many row tiles");
     const uint64_t need = att_room(a, p);
     if (need == 0) return MIBC_OK;

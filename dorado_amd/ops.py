@@ -28,6 +28,10 @@ _ATTN_ARGS = struct.Struct("@4PP3PPPQ12q8i3i2fi")
 _fns = None
 
 
+# a number outside its field's range, or none at all
+_BAD_FIELD = (struct.error, OverflowError)
+
+
 def _entry():
     global _fns
     if _fns is None:
@@ -137,10 +141,13 @@ def rms_norm(x, weight=None, *, residual=None, alpha: float = 1.0, eps: float = 
         raise MibcError(f"rms_norm: sum_out must be {list(shape)} {dtype}")
     elif not sum_out.is_contiguous():
         ss = _row_stride("rms_norm", "sum_out", sum_out, cols)
-    args = _NORM_ARGS.pack(
-        x.data_ptr(), 0 if residual is None else residual.data_ptr(), 0 if weight is None else weight.data_ptr(),
-        0 if sum_out is None else sum_out.data_ptr(), out.data_ptr(), 0 if scale is None else scale.data_ptr(), x.numel() // cols,
-        xs, rs, ss, os_, groups, cols, _TYPE[dtype], _TYPE[dtype if weight is None else weight.dtype], _TYPE[out_dtype], group, alpha, eps, 0)
+    try:
+        args = _NORM_ARGS.pack(
+            x.data_ptr(), 0 if residual is None else residual.data_ptr(), 0 if weight is None else weight.data_ptr(),
+            0 if sum_out is None else sum_out.data_ptr(), out.data_ptr(), 0 if scale is None else scale.data_ptr(), x.numel() // cols,
+            xs, rs, ss, os_, groups, cols, _TYPE[dtype], _TYPE[dtype if weight is None else weight.dtype], _TYPE[out_dtype], group, alpha, eps, 0)
+    except _BAD_FIELD as e:
+        raise MibcError(f"rms_norm: {e}") from None
     rc = (_fns or _entry())[0](dev, _stream(dev), args)
     if rc:
         _check(rc, "rms_norm")
@@ -212,9 +219,12 @@ def rope(q, k=None, *, freqs, positions=None, start: int = 0, interleaved: bool 
         plain = plain and ks[3] == 1 and kos[3] == 1
     if not plain and d > 1:
         raise MibcError("rope: head_dim must be contiguous")
-    args = _ROPE_ARGS.pack(q.data_ptr(), kp, qo.data_ptr(), kop, where, freqs.data_ptr(), start, qs[0], qs[1], qs[2], ks[0], ks[1], ks[2],
-                           qos[0], qos[1], qos[2], kos[0], kos[1], kos[2], b, t, h, kh, d, 2 * freqs.shape[0], _TYPE[dtype],
-                           bool(interleaved), where != 0 and positions.dtype is torch.int64, amplitude)
+    try:
+        args = _ROPE_ARGS.pack(q.data_ptr(), kp, qo.data_ptr(), kop, where, freqs.data_ptr(), start, qs[0], qs[1], qs[2], ks[0], ks[1], ks[2],
+                               qos[0], qos[1], qos[2], kos[0], kos[1], kos[2], b, t, h, kh, d, 2 * freqs.shape[0], _TYPE[dtype],
+                               bool(interleaved), where != 0 and positions.dtype is torch.int64, amplitude)
+    except _BAD_FIELD as e:
+        raise MibcError(f"rope: {e}") from None
     rc = (_fns or _entry())[1](dev, _stream(dev), args)
     if rc:
         _check(rc, "rope")
@@ -231,7 +241,7 @@ def attention(q, k, v, *, scale=None, causal: bool = False, window=(-1, -1), sof
     [batch] int32: keys in use; query t stands at position k_len - q_tokens + t, or q_start + t.  prefix [batch] int32: that
     many first keys are seen by all.  doc_offsets [n + 1] int32 (batch 1, self attention): documents packed one after the
     other, each seeing itself only; prefix is then [n] and counts from the document's start.  A query that sees nothing gives
-    zeros.  Returns out like q, or (out, lse f32 [batch, heads, q_tokens])."""
+    zeros.  out: None or the tensor to write, which may be q itself.  Returns out like q, or (out, lse f32 [batch, heads, q_tokens])."""
     dev = _device("attention", q, k, v, slopes, k_len, prefix, doc_offsets, out)
     shape, kshape, dtype = q.shape, k.shape, q.dtype
     if len(shape) != 4 or len(kshape) != 4:
@@ -278,9 +288,12 @@ def attention(q, k, v, *, scale=None, causal: bool = False, window=(-1, -1), sof
     lse = torch.empty((b, h, n), dtype=torch.float32, device=q.device) if return_lse else None
     head = (q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), 0 if lse is None else lse.data_ptr(), lens, pre, offs, slope)
     tail = (qs[0], qs[1], qs[2], ks[0], ks[1], ks[2], vs[0], vs[1], vs[2], os_[0], os_[1], os_[2], b, h, kh, n, m, d, docs, _TYPE[dtype],
-            back, ahead, q_start, d ** -0.5 if scale is None else scale, softcap, 0)
+            back, ahead, q_start, max(d, 1) ** -0.5 if scale is None else scale, softcap, 0)
     _, _, run, workspace = _fns or _entry()
-    args = _ATTN_ARGS.pack(*head, 0, 0, *tail)
+    try:
+        args = _ATTN_ARGS.pack(*head, 0, 0, *tail)
+    except _BAD_FIELD as e:
+        raise MibcError(f"attention: {e}") from None
     need = workspace(args) if m >= 512 else 0      # fewer keys are never split
     if need:
         room = torch.empty(need, dtype=torch.uint8, device=q.device)

@@ -289,6 +289,20 @@ def test_attention_layouts():
     assert ops.attention(q[:, :0], k, v).shape == (b, 0, h, d) and ops.attention(q[:0], k[:0], v[:0]).shape == (0, n, h, d)
 
 
+@pytest.mark.parametrize("n,m", [(1, 1200), (3, 40), (40, 1200), (300, 300)])
+def test_attention_in_place(n, m):
+    # the queries' columns of a packed q | k | v buffer receive the result; the others stay
+    x = rnd((2, max(n, m), 8, 64), F16, 71)
+    q, k, v = x[:, :n, :4], x[:, :m, 4:6], x[:, :m, 6:]
+    before, want = x.clone(), ops.attention(q, k, v)
+    assert ops.attention(q, k, v, out=q) is q and torch.equal(q, want)
+    assert torch.equal(x[:, :, 4:], before[:, :, 4:]) and torch.equal(x[:, n:, :4], before[:, n:, :4])
+    with pytest.raises(capi.MibcError, match="not k or v"):
+        ops.attention(k, k, v, out=v)
+    with pytest.raises((capi.MibcError, capi.MibcNotSupported)):
+        ops.attention(q[..., :0], k[..., :0], v[..., :0])
+
+
 def test_attention_long_axis_is_split_and_joined():
     q, k, v = qkv(1, 1, 20011, 4, 1, 128, BF16, 90)
     a = struct_args(q, k, v)
@@ -303,6 +317,22 @@ def struct_args(q, k, v):
     return ops._ATTN_ARGS.pack(q.data_ptr(), k.data_ptr(), v.data_ptr(), q.data_ptr(), 0, 0, 0, 0, 0, 0, 0, *q.stride()[:3], *k.stride()[:3],
                                *v.stride()[:3], *q.stride()[:3], q.shape[0], q.shape[2], k.shape[2], q.shape[1], k.shape[1], q.shape[3], 0,
                                ops._TYPE[q.dtype], -1, -1, ops.ATTN_END, 0.1, 0.0, 0)
+
+
+def test_numbers_outside_their_fields():
+    x, f = rnd((1, 2, 2, 64), F16, 72), torch.ones(32, dtype=torch.float64).cuda()
+    for bad in (1e39, None):        # infinite in f32, no number
+        for call in (lambda: ops.rope(x, freqs=f, amplitude=bad), lambda: ops.attention(x, x, x, softcap=bad)):
+            with pytest.raises(capi.MibcError):
+                call()
+    with pytest.raises(capi.MibcError, match="rms_norm: "):
+        ops.rms_norm(x, eps=None)
+    with pytest.raises(capi.MibcError, match="rms_norm: "):
+        ops.rms_norm(x, quant="int8", group=1 << 40)
+    with pytest.raises(capi.MibcError, match="rope: "):
+        ops.rope(x, freqs=f, start=1 << 64)
+    with pytest.raises(capi.MibcError, match="attention: "):
+        ops.attention(x, x, x, scale=-1e39)
 
 
 def test_attention_offsets_beyond_32_bits():

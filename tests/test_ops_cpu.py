@@ -82,6 +82,12 @@ def test_attention_refuses(change, code):
     assert rc == code and text.startswith("attention: ")
 
 
+@pytest.mark.parametrize("change", [dict(k=P, v=P + 64), dict(k=P + 64, v=P), dict(k=P, v=P)])
+def test_attention_refuses_to_write_its_keys(change):
+    rc, text = call(2, ATTN, out=P, **change)
+    assert rc == -1 and "not k or v" in text
+
+
 def test_workspace_follows_the_sizes():
     ws = ops._entry()[3]
 
