@@ -24,6 +24,7 @@ struct AttArgs {
     int tiles;        // row tiles per pair
     int splits;       // parts the keys of a tile are split into, joined by the second launch if > 1
     int order;        // workgroup -> (pair, tile, split): 0 pairs innermost, 1 tiles innermost (one pair stays on one XCD)
+    int twin;         // pairs 2 i and 2 i + 1, whose keys share cache lines, run on one XCD at the same time (pairs % 16 == 0)
     float scale2;     // scale * log2(e)
     float cap_in, cap_out;   // scores / cap in, cap out: 2 * scale / cap * log2(e), cap * log2(e); 0: no cap
     float *part_o;    // [pairs * rows][splits][D] f32

@@ -121,6 +121,9 @@ __device__ __forceinline__ const AttArgs &att_args_again() {
     return *(const AttArgs *)at;
 }
 
+// workgroups i and i + 8 of 16 go to one XCD: they get neighbouring pairs
+__device__ __forceinline__ int att_twin(const AttArgs &p, unsigned x) { return p.twin ? (x & ~15u) | (x & 7) << 1 | (x >> 3 & 1) : x; }
+
 // The exponent (base 2) of a score is mul * x + add, x being what the registers hold.  Plain: x = q.k, mul = scale log2(e).
 // Capped: cap tanh(y) = cap - 2 cap / (1 + e^2y), so x = 1 / (1 + e^2y) and the last product is the exponent's own fma; the
 // largest score is the smallest x.  A slope adds slope * |i - j| to x, in x's unit.
@@ -201,15 +204,15 @@ __global__ __launch_bounds__(256, D <= 64 ? 3 : 2) void attention_kernel(AttArgs
     int pair, tile, split;
     if (p.order == 0) {
         const unsigned rest = p.by_pairs.div(id);
-        pair = id - rest * p.pairs;
+        pair = att_twin(p, id - rest * p.pairs);
         const unsigned z = p.by_splits.div(rest);
         split = rest - z * p.splits;
         tile = p.tiles - 1 - (int)z;                    // causal: the long tiles start first
     } else {
-        const unsigned rest = id >> 3, y = p.by_splits.div(rest), z = p.by_tiles.div(y);
+        const unsigned rest = id >> (p.twin ? 4 : 3), y = p.by_splits.div(rest), z = p.by_tiles.div(y);
         split = rest - y * p.splits;
         tile = y - z * p.tiles;
-        pair = z * 8 + (id & 7);
+        pair = p.twin ? att_twin(p, z * 16 + (id & 15)) : z * 8 + (id & 7);
     }
     const int b = p.by_kv.div(pair), kvh = pair - b * a.kv_heads;
 
@@ -587,7 +590,7 @@ __global__ __launch_bounds__(256, 2) void attention_token_kernel(AttArgs p) {
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int l15 = lane & 15, quarter = lane >> 4;
-    const int split = p.by_pairs.div(blockIdx.x), pair = blockIdx.x - split * p.pairs;
+    const int split = p.by_pairs.div(blockIdx.x), pair = att_twin(p, blockIdx.x - split * p.pairs);
     const int b = p.by_kv.div(pair), kvh = pair - b * a.kv_heads;
 
     const int rr = min(l15, p.rows - 1), t = p.by_group.div(rr), head = kvh * p.group + (rr - t * p.group);

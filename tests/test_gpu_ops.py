@@ -289,6 +289,14 @@ def test_attention_layouts():
     assert ops.attention(q[:, :0], k, v).shape == (b, 0, h, d) and ops.attention(q[:0], k[:0], v[:0]).shape == (0, n, h, d)
 
 
+@pytest.mark.parametrize("d", [32, 64, 96])
+@pytest.mark.parametrize("b,kh", [(2, 8), (8, 4), (16, 1), (3, 8), (4, 12)])
+@pytest.mark.parametrize("n,m,kw", [(1, 200, {}), (1, 2100, {}), (12, 700, dict(causal=True)), (150, 150, {}), (150, 150, dict(causal=True)), (70, 1100, dict(window=(30, 5)))])
+def test_attention_neighbouring_heads(b, kh, n, m, kw, d):
+    # pairs of heads whose keys share cache lines are dealt to the same part of the chip; every pair is worked on once
+    check(*qkv(b, n, m, kh, kh, d, F16, 75), **kw)
+
+
 @pytest.mark.parametrize("n,m", [(1, 1200), (3, 40), (40, 1200), (300, 300)])
 def test_attention_in_place(n, m):
     # the queries' columns of a packed q | k | v buffer receive the result; the others stay
