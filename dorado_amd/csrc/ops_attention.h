@@ -23,6 +23,7 @@ struct AttArgs {
     int pairs;        // batch * kv_heads
     int tiles;        // row tiles per pair
     int splits;       // parts the keys of a tile are split into, joined by the second launch if > 1
+    unsigned groups;  // workgroups: pairs * tiles * splits
     int order;        // workgroup -> (pair, tile, split): 0 pairs innermost, 1 tiles innermost (one pair stays on one XCD)
     int twin;         // pairs 2 i and 2 i + 1, whose keys share cache lines, run on one XCD at the same time (pairs % 16 == 0)
     float scale2;     // scale * log2(e)
@@ -32,7 +33,7 @@ struct AttArgs {
 };
 
 // tokens: the kernel for at most 16 rows per pair, else tiles of 128 rows
-#define MIBC_ATT_DECLARE(D) int mibc_att_launch_##D(hipStream_t s, const AttArgs &p, bool tokens, unsigned grid);
+#define MIBC_ATT_DECLARE(D) int mibc_att_launch_##D(hipStream_t s, const AttArgs &p, bool tokens);
 MIBC_ATT_DECLARE(32)
 MIBC_ATT_DECLARE(64)
 MIBC_ATT_DECLARE(96)

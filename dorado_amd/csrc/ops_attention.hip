@@ -145,16 +145,16 @@ int mibc_launch_attention(hipStream_t s, const mibc_attention_args &a, bool whol
         p.part_o = (float *)a.workspace;
         p.part_l = p.part_o + (uint64_t)p.pairs * p.rows * p.splits * a.head_dim;
     }
-    const int64_t grid = (int64_t)p.pairs * p.tiles * p.splits;
+    p.groups = (unsigned)((int64_t)p.pairs * p.tiles * p.splits);
     p.order = (a.window_ahead != 0 && p.pairs % 8 == 0) ? 1 : 0;
     // heads of 64 or 192 bytes share 128-byte lines with their neighbours, which two XCDs would both fetch (32 x 4 pairs over 8192 keys
     // of 32: 45 -> 28 us, 64 x 1024 windows of 256 keys, 8 heads of 32: 72 -> 53, of 96: 149 -> 132; nothing at 64 and 128)
     p.twin = a.head_dim % 64 != 0 && a.kv_heads % 2 == 0 && p.pairs % 16 == 0 && a.k_stride[2] == a.head_dim;
     switch (a.head_dim) {
-        case 32: return mibc_att_launch_32(s, p, plan.tokens, (unsigned)grid);
-        case 64: return mibc_att_launch_64(s, p, plan.tokens, (unsigned)grid);
-        case 96: return mibc_att_launch_96(s, p, plan.tokens, (unsigned)grid);
-        default: return mibc_att_launch_128(s, p, plan.tokens, (unsigned)grid);
+        case 32: return mibc_att_launch_32(s, p, plan.tokens);
+        case 64: return mibc_att_launch_64(s, p, plan.tokens);
+        case 96: return mibc_att_launch_96(s, p, plan.tokens);
+        default: return mibc_att_launch_128(s, p, plan.tokens);
     }
 }
 

@@ -200,7 +200,8 @@ __global__ __launch_bounds__(256, D <= 64 ? 3 : 2) void attention_kernel(AttArgs
     const int half = lane >> 5;
 
     // workgroup -> (split, tile, pair)
-    const unsigned id = blockIdx.x;
+    const unsigned id = (blockIdx.y << 20) + blockIdx.x;
+    if (id >= p.groups) return;
     int pair, tile, split;
     if (p.order == 0) {
         const unsigned rest = p.by_pairs.div(id);
@@ -590,7 +591,9 @@ __global__ __launch_bounds__(256, 2) void attention_token_kernel(AttArgs p) {
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int l15 = lane & 15, quarter = lane >> 4;
-    const int split = p.by_pairs.div(blockIdx.x), pair = att_twin(p, blockIdx.x - split * p.pairs);
+    const unsigned id = (blockIdx.y << 20) + blockIdx.x;
+    if (id >= p.groups) return;
+    const int split = p.by_pairs.div(id), pair = att_twin(p, id - split * p.pairs);
     const int b = p.by_kv.div(pair), kvh = pair - b * a.kv_heads;
 
     const int rr = min(l15, p.rows - 1), t = p.by_group.div(rr), head = kvh * p.group + (rr - t * p.group);
@@ -888,21 +891,24 @@ __global__ __launch_bounds__(256) void attention_join_kernel(AttArgs p) {
 }
 
 template <typename T, bool CAP, bool SLOPES>
-static void att_one(hipStream_t s, const AttArgs &p, bool tokens, unsigned grid) {
+static void att_one(hipStream_t s, const AttArgs &p, bool tokens) {
+    // a launch holds less than 2^32 threads in x
+    const unsigned x = p.groups < 1u << 20 ? p.groups : 1u << 20;
+    const dim3 grid(x, (p.groups + x - 1) / x);
     constexpr int ROWS = 4 * 64 * ATT_D * 2, STEPS = 4 * 2 * 32 * ATT_D * 2, JOIN = 4 * 16 * (ATT_D + 4 + 2) * 4, TOKEN = STEPS > JOIN ? STEPS : JOIN;
 #define ATT_GO(KERNEL, LDS)                                                             \
     do {                                                                                \
         MIBC_LDS_ATTR_ONCE(KERNEL, LDS);                                                \
-        hipLaunchKernelGGL(KERNEL, dim3(grid), dim3(256), LDS, s, p);                   \
+        hipLaunchKernelGGL(KERNEL, grid, dim3(256), LDS, s, p);                         \
     } while (0)
     if (tokens) ATT_GO((attention_token_kernel<T, ATT_D, CAP, SLOPES>), TOKEN);
     else ATT_GO((attention_kernel<T, ATT_D, CAP, SLOPES>), ROWS);
 #undef ATT_GO
 }
 template <typename T>
-static int att_launch(hipStream_t s, const AttArgs &p, bool tokens, unsigned grid) {
-    if (p.cap_out > 0.0f) p.a.slopes ? att_one<T, true, true>(s, p, tokens, grid) : att_one<T, true, false>(s, p, tokens, grid);
-    else p.a.slopes ? att_one<T, false, true>(s, p, tokens, grid) : att_one<T, false, false>(s, p, tokens, grid);
+static int att_launch(hipStream_t s, const AttArgs &p, bool tokens) {
+    if (p.cap_out > 0.0f) p.a.slopes ? att_one<T, true, true>(s, p, tokens) : att_one<T, true, false>(s, p, tokens);
+    else p.a.slopes ? att_one<T, false, true>(s, p, tokens) : att_one<T, false, false>(s, p, tokens);
     int rc = op_hip(hipGetLastError(), "attention");
     if (rc != MIBC_OK || p.splits == 1) return rc;
     hipLaunchKernelGGL((attention_join_kernel<T, ATT_D>), dim3((unsigned)((int64_t)p.pairs * p.rows)), dim3(256), 0, s, p);
@@ -910,6 +916,6 @@ static int att_launch(hipStream_t s, const AttArgs &p, bool tokens, unsigned gri
 }
 #define ATT_CAT2(a, b) a##b
 #define ATT_CAT(a, b) ATT_CAT2(a, b)
-int ATT_CAT(mibc_att_launch_, ATT_D)(hipStream_t s, const AttArgs &p, bool tokens, unsigned grid) {
-    return p.a.type == MIBC_TYPE_F16 ? att_launch<half_t>(s, p, tokens, grid) : att_launch<bf16_t>(s, p, tokens, grid);
+int ATT_CAT(mibc_att_launch_, ATT_D)(hipStream_t s, const AttArgs &p, bool tokens) {
+    return p.a.type == MIBC_TYPE_F16 ? att_launch<half_t>(s, p, tokens) : att_launch<bf16_t>(s, p, tokens);
 }

@@ -2,7 +2,8 @@
 //   h = x + alpha r,   y = h / sqrt(sum h^2 / C + eps) * w,   q = rne(y / s), s = max|y| / 127 | 448
 // A few flops per element against 2-8 bytes: bound by HBM.  So a row is read once, stays in f32 registers (TPR threads hold
 // NCH chunks of 8 consecutive columns each) through both reductions (sum of squares, then max |y| where the output has 8 bits)
-// and leaves once.  Rows of up to 2048 columns take one wave (or a quarter of one) and reduce by lane shuffles alone; wider ones
+// and leaves once.  Rows of up to 2048 columns take one wave, or as few of its lanes as hold them (2M rows of 32 bf16: 4 lanes 6.5 TB/s,
+// 16 lanes 2.6), and reduce by lane shuffles alone; wider ones
 // take a workgroup and one LDS exchange per reduction: as few threads as hold the row in six chunks (11320 columns: 256 threads x 6
 // chunks 39 us, 1024 x 2 54), 1024 beyond.
 // Measured: 262144 x 512 f16 with residual 134 us (6.0 TB/s), 16383 x 4096 bf16 with residual, sum and e4m3 codes per 128 columns
@@ -72,8 +73,8 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void rms_norm_kernel(NormArg
     __shared__ float red[2][NT / 64];
     const mibc_rms_norm_args &a = n.a;
     const int lane = threadIdx.x % TPR;
-    const int64_t row = (int64_t)blockIdx.x * (NT / TPR) + threadIdx.x / TPR;
-    if (TPR <= 64 && row >= a.rows) return;     // whole rows of lanes; TPR >= 256: one row per workgroup, the grid is exact
+    const int64_t row = (((int64_t)blockIdx.y << 20) + blockIdx.x) * (NT / TPR) + threadIdx.x / TPR;
+    if (row >= a.rows) return;     // whole rows of lanes, or a whole workgroup
     const int cols = a.cols;
     const T *x = (const T *)a.x + row * a.x_stride;
     const T *r = (const T *)a.residual + row * a.residual_stride;
@@ -207,9 +208,16 @@ template <typename T, bool VEC>
 static void norm_launch(hipStream_t s, const NormArgs &n) {
     const int chunks = (n.a.cols + 7) / 8;
     const int64_t rows = n.a.rows;
-#define NORM_GO(TPR, NCH, NT) \
-    hipLaunchKernelGGL((rms_norm_kernel<T, TPR, NCH, VEC>), dim3((unsigned)((rows + NT / TPR - 1) / (NT / TPR))), dim3(NT), 0, s, n)
-    if (chunks <= 16) NORM_GO(16, 1, 256);
+    // a launch holds less than 2^32 threads in x
+#define NORM_GO(TPR, NCH, NT)                                                                                        \
+    do {                                                                                                             \
+        const int64_t blocks = (rows + NT / TPR - 1) / (NT / TPR), x = blocks < 1 << 20 ? blocks : 1 << 20;          \
+        hipLaunchKernelGGL((rms_norm_kernel<T, TPR, NCH, VEC>), dim3((unsigned)x, (unsigned)((blocks + x - 1) / x)), \
+                           dim3(NT), 0, s, n);                                                                       \
+    } while (0)
+    if (chunks <= 4) NORM_GO(4, 1, 256);
+    else if (chunks <= 8) NORM_GO(8, 1, 256);
+    else if (chunks <= 16) NORM_GO(16, 1, 256);
     else if (chunks <= 64) NORM_GO(64, 1, 256);
     else if (chunks <= 128) NORM_GO(64, 2, 256);
     else if (chunks <= 256) NORM_GO(64, 4, 256);

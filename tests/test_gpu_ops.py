@@ -144,6 +144,20 @@ def test_rope_in_place_and_back():
     assert torch.equal(ops.rope(wide, freqs=f), ops.rope(wide.contiguous(), freqs=f))
 
 
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("h,kh,d,rot", [(20, 3, 40, 40), (8, 0, 40, 20), (1, 9, 36, 10)])
+def test_rope_in_place_other_sizes(h, kh, d, rot, interleaved):
+    x = rnd((2, 9, h + kh, d), BF16, 24)
+    q, k, f = x[:, :, :h], x[:, :, h:] if kh else None, ops.rope_frequencies(rot)
+    want = ops.rope(q.clone(), None if k is None else k.clone(), freqs=f, start=3, interleaved=interleaved)
+    got = ops.rope(q, k, freqs=f, start=3, interleaved=interleaved, out=q if k is None else (q, k))
+    for a, b in zip((got,) if k is None else got, (want,) if k is None else want):
+        assert torch.equal(a, b)
+    R.close(q, R.rope(rnd((2, 9, h + kh, d), BF16, 24)[:, :, :h], f, torch.arange(3, 12), interleaved),
+            R.rope_tolerance(q.cpu().double(), rnd((2, 9, h + kh, d), BF16, 24)[:, :, :h], f, torch.arange(3, 12), 1.0, BF16, interleaved)
+            + 2.0 ** -8 * R.u(BF16) * q.cpu().double().abs(), "in place")      # the tolerance of the rounded value, not of the exact one
+
+
 # --------------------------------------------------------------------------------------------------------------- attention
 def qkv(b, n, m, h, kh, d, t, seed, mul=1.0):
     return rnd((b, n, h, d), t, seed, mul), rnd((b, m, kh, d), t, seed + 1, mul), rnd((b, m, kh, d), t, seed + 2)
@@ -341,6 +355,46 @@ def test_numbers_outside_their_fields():
         ops.rope(x, freqs=f, start=1 << 64)
     with pytest.raises(capi.MibcError, match="attention: "):
         ops.attention(x, x, x, scale=-1e39)
+
+
+@pytest.mark.parametrize("n", [1, 17])
+def test_attention_many_pairs(n):
+    # more than 2^20 workgroups; any slice of the batch gives the same bits by itself
+    b = (1 << 17) + 3
+    q, k, v = qkv(1, n, 3, 8, 8, 32, F16, 76)
+    scale = (torch.arange(b, device="cuda") % 61 + 1).to(F16)[:, None, None, None] / 32
+    q = q * scale
+    k, v = (x.expand(b, -1, -1, -1) for x in (k, v))
+    out = ops.attention(q, k, v)
+    for x in (0, 70000, b - 40):
+        assert torch.equal(out[x:x + 37], ops.attention(q[x:x + 37], k[:37], v[:37]))
+    assert torch.equal(out[-1], out[(b - 1) % 61])
+
+
+def test_rms_norm_many_rows():
+    rows = (1 << 22) + 5        # four to a workgroup: more than 2^20 of them
+    x = rnd((61, 136), F16, 77)[torch.arange(rows, device="cuda") % 61]
+    y = ops.rms_norm(x)
+    assert torch.equal(y, ops.rms_norm(x[:61])[torch.arange(rows, device="cuda") % 61])
+
+
+@pytest.mark.parametrize("cols", [8, 24, 32, 33, 64, 65])
+@pytest.mark.parametrize("quant", ["int8", "e4m3"])
+def test_rms_norm_narrow_8bit(cols, quant):
+    # 4, 8 and 16 lanes to a row: scales and codes of a row are those of the row alone
+    x, w = rnd((1001, cols), BF16, 78), rnd((cols,), BF16, 79)
+    y = R.rms_norm(x, w)[0]
+    q, s = ops.rms_norm(x, w, quant=quant)
+    most = 127.0 if quant == "int8" else 448.0
+    want = y.abs().amax(1, keepdim=True) / most
+    assert ((s.cpu().to(R.F64) - want).abs() <= 2.0 ** -18 * want).all()
+    # int8: half a code.  e4m3: half a step, 2^-4 of the value (2^-10 of the scale below its normal range), plus the norm's own 2^-18
+    near = 0.5 * want if quant == "int8" else torch.maximum(y.abs() * 2.0 ** -4, want * 2.0 ** -10)
+    off = (q.cpu().to(R.F64) * s.cpu().to(R.F64) - y).abs()
+    assert (off <= near * (1 + 2.0 ** -16) + 2.0 ** -16 * most * want).all()
+    one = [ops.rms_norm(x[r:r + 1], w, quant=quant) for r in (0, 7, 500, 1000)]
+    for r, (q1, s1) in zip((0, 7, 500, 1000), one):
+        assert torch.equal(q[r].view(torch.uint8), q1[0].view(torch.uint8)) and torch.equal(s[r], s1[0])
 
 
 def test_attention_offsets_beyond_32_bits():
