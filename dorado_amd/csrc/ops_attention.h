@@ -14,6 +14,8 @@ struct AttDiv {
     __device__ __forceinline__ unsigned div(unsigned n) const { return m == 0 ? n : __umulhi(n, m) >> (s - 1); }
 };
 
+enum { ATT_NO_CAP, ATT_NEAR, ATT_FAR };     // forms of the cap, see AttScore
+
 struct AttArgs {
     mibc_attention_args a;
     AttDiv by_pairs, by_splits, by_tiles, by_kv, by_group;
@@ -27,7 +29,8 @@ struct AttArgs {
     int order;        // workgroup -> (pair, tile, split): 0 pairs innermost, 1 tiles innermost (one pair stays on one XCD)
     int twin;         // pairs 2 i and 2 i + 1, whose keys share cache lines, run on one XCD at the same time (pairs % 16 == 0)
     float scale2;     // scale * log2(e)
-    float cap_in, cap_out;   // scores / cap in, cap out: 2 * scale / cap * log2(e), cap * log2(e); 0: no cap
+    int cap;          // its form
+    float cap_in, cap_out;   // ATT_NEAR: 2 scale / cap log2(e), cap log2(e); ATT_FAR: scale / cap, cap / scale
     float *part_o;    // [pairs * rows][splits][D] f32
     float *part_l;    // [pairs * rows][splits] log2 of the sum
 };

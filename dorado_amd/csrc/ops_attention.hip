@@ -13,6 +13,7 @@ static int att_check(const mibc_attention_args &a) {
     if (!(a.scale > 0.0f) || !(a.scale <= 1e30f)) return op_refuse(MIBC_ERR_ARG, "attention: scale must be positive and finite");
     if (!(a.softcap >= 0.0f) || !(a.softcap <= 1e30f)) return op_refuse(MIBC_ERR_ARG, "attention: softcap must be 0 (none) or positive and finite");
     if (a.softcap > 0.0f && !(3.0f * a.scale / a.softcap <= 3e38f)) return op_refuse(MIBC_ERR_ARG, "attention: softcap too small for this scale");
+    if (a.softcap > 0.0f && !(a.softcap / a.scale <= 3e37f)) return op_refuse(MIBC_ERR_ARG, "attention: softcap too large for this scale");
     if (a.reserved != 0) return op_refuse(MIBC_ERR_ARG, "attention: reserved must be 0");
     const int64_t big = (int64_t)1 << 28;     // positions, and distances between them, stay far inside 32 bits
     if (a.q_tokens > big || a.k_tokens > big || (int64_t)a.q_tokens * (a.heads / a.kv_heads) > big ||
@@ -137,7 +138,14 @@ int mibc_launch_attention(hipStream_t s, const mibc_attention_args &a, bool whol
     p.back = a.window_back >= 0 && a.window_back < 1 << 30 ? a.window_back : -1;
     p.ahead = a.window_ahead >= 0 && a.window_ahead < 1 << 30 ? a.window_ahead : -1;
     p.scale2 = a.scale * 1.4426950408889634f;
-    if (a.softcap > 0.0f) {
+    // tiles: caps up to 64 take the form of fewer instructions, whose error grows with the cap (causal 16384 x 16 heads of 128: 1210 us,
+    // the other form 1788, no cap 1046).  Single tokens are bound by bytes: 285 us either way and without a cap (48 x 8 pairs x 8192)
+    if (a.softcap > 64.0f || (a.softcap > 0.0f && plan.tokens)) {
+        p.cap = ATT_FAR;
+        p.cap_in = a.scale / a.softcap;
+        p.cap_out = a.softcap / a.scale;
+    } else if (a.softcap > 0.0f) {
+        p.cap = ATT_NEAR;
         p.cap_in = 2.0f * a.scale / a.softcap * 1.4426950408889634f;
         p.cap_out = a.softcap * 1.4426950408889634f;
     }

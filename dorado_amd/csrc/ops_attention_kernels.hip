@@ -124,21 +124,38 @@ __device__ __forceinline__ const AttArgs &att_args_again() {
 // workgroups i and i + 8 of 16 go to one XCD: they get neighbouring pairs
 __device__ __forceinline__ int att_twin(const AttArgs &p, unsigned x) { return p.twin ? (x & ~15u) | (x & 7) << 1 | (x >> 3 & 1) : x; }
 
-// The exponent (base 2) of a score is mul * x + add, x being what the registers hold.  Plain: x = q.k, mul = scale log2(e).
-// Capped: cap tanh(y) = cap - 2 cap / (1 + e^2y), so x = 1 / (1 + e^2y) and the last product is the exponent's own fma; the
-// largest score is the smallest x.  A slope adds slope * |i - j| to x, in x's unit.
-template <bool CAP, bool SLOPES>
+// The exponent (base 2) of a score is mul * x + add, x being what the registers hold.  A slope adds slope * |i - j| to x, in x's unit.
+//   no cap:   x = q.k, mul = scale log2(e)
+//   ATT_NEAR: cap tanh(y) = cap - 2 cap / (1 + e^2y), so x = 1 / (1 + e^2y) and the last product is the exponent's own fma; the
+//             largest score is the smallest x.  Two numbers of the cap's size cancel: off by up to cap 2^-21 whatever the score, so
+//             this form is for caps up to 64 (in tiles of rows, where the other one costs half as much again)
+//   ATT_FAR:  x = q.k tanh(y) / y, mul = scale log2(e): off by 2^-20 of the score.  Below |y| = 1/2 the Taylor series of
+//             tanh(y) / y up to y^12 (the next term is below 2^-23), above it cap / scale (1 - e^-2|y|) / (1 + e^-2|y|)
+template <int CAP, bool SLOPES>
 struct AttScore {
-    float mul, add, slope, in;
-    static constexpr float HIDDEN = CAP ? INFINITY : -INFINITY;
+    float mul, add, slope, in, most;
+    static constexpr float HIDDEN = CAP == ATT_NEAR ? INFINITY : -INFINITY;
     __device__ __forceinline__ AttScore(const AttArgs &p, int head) {
-        mul = CAP ? -2.0f * p.cap_out : p.scale2;
-        add = CAP ? p.cap_out : 0.0f;
+        mul = CAP == ATT_NEAR ? -2.0f * p.cap_out : p.scale2;
+        add = CAP == ATT_NEAR ? p.cap_out : 0.0f;
         in = p.cap_in;
+        most = p.cap_out;
         slope = SLOPES ? -p.a.slopes[head] * 1.4426950408889634f / mul : 0.0f;
     }
-    __device__ __forceinline__ float capped(float x) const { return __builtin_amdgcn_rcpf(1.0f + att_exp2(x * in)); }
-    __device__ __forceinline__ float larger(float a, float b) const { return CAP ? fminf(a, b) : fmaxf(a, b); }
+    __device__ __forceinline__ float capped(float x) const {
+        if (CAP == ATT_NEAR) return __builtin_amdgcn_rcpf(1.0f + att_exp2(x * in));
+        const float y = x * in, z = y * y;
+        float t = fmaf(z, 3.592128036572481e-3f, -8.863235529902197e-3f);      // 21844 / 6081075, -1382 / 155925
+        t = fmaf(z, t, 2.186948853615520e-2f);                                 // 62 / 2835
+        t = fmaf(z, t, -5.396825396825397e-2f);                                // -17 / 315
+        t = fmaf(z, t, 0.1333333333333333f);
+        t = fmaf(z, t, -0.3333333333333333f);
+        t = fmaf(z, t, 1.0f);
+        const float e = att_exp2(fabsf(y) * -2.8853900817779268f);             // 2 log2(e)
+        const float far = copysignf(most * (1.0f - e) * __builtin_amdgcn_rcpf(1.0f + e), x);
+        return fabsf(y) < 0.5f ? x * t : far;                                  // NaN: far, which is NaN
+    }
+    __device__ __forceinline__ float larger(float a, float b) const { return CAP == ATT_NEAR ? fminf(a, b) : fmaxf(a, b); }
 };
 
 // 1 where a value is NaN (kind 0), infinity (1), -infinity (2), else 0
@@ -182,7 +199,7 @@ __device__ __forceinline__ int att_v_slot(int row, int chunk) {
     return D == 128 ? chunk ^ ((row & 3) << 2) : D == 64 ? chunk ^ (((row >> 1) & 1) << 2) : chunk;
 }
 
-template <typename T, int D, bool CAP, bool SLOPES>
+template <typename T, int D, int CAP, bool SLOPES>
 __global__ __launch_bounds__(256, D <= 64 ? 3 : 2) void attention_kernel(AttArgs p) {
     typedef AttType<T> X;
     typedef typename X::vec8 vec8;
@@ -577,7 +594,7 @@ __device__ __forceinline__ int att_v_slot16(int row, int chunk) {
     return D == 128 ? chunk ^ (((row & 3) << 2) | ((row & 4) >> 1)) : D == 64 ? chunk ^ ((((row >> 1) & 1) << 2) | ((row & 4) >> 1)) : chunk;
 }
 
-template <typename T, int D, bool CAP, bool SLOPES>
+template <typename T, int D, int CAP, bool SLOPES>
 __global__ __launch_bounds__(256, 2) void attention_token_kernel(AttArgs p) {
     typedef AttType<T> X;
     typedef typename X::vec8 vec8;
@@ -890,7 +907,7 @@ __global__ __launch_bounds__(256) void attention_join_kernel(AttArgs p) {
     }
 }
 
-template <typename T, bool CAP, bool SLOPES>
+template <typename T, int CAP, bool SLOPES>
 static void att_one(hipStream_t s, const AttArgs &p, bool tokens) {
     // a launch holds less than 2^32 threads in x
     const unsigned x = p.groups < 1u << 20 ? p.groups : 1u << 20;
@@ -901,14 +918,15 @@ static void att_one(hipStream_t s, const AttArgs &p, bool tokens) {
         MIBC_LDS_ATTR_ONCE(KERNEL, LDS);                                                \
         hipLaunchKernelGGL(KERNEL, grid, dim3(256), LDS, s, p);                         \
     } while (0)
-    if (tokens) ATT_GO((attention_token_kernel<T, ATT_D, CAP, SLOPES>), TOKEN);
+    if (tokens) ATT_GO((attention_token_kernel<T, ATT_D, CAP == ATT_NO_CAP ? ATT_NO_CAP : ATT_FAR, SLOPES>), TOKEN);
     else ATT_GO((attention_kernel<T, ATT_D, CAP, SLOPES>), ROWS);
 #undef ATT_GO
 }
 template <typename T>
 static int att_launch(hipStream_t s, const AttArgs &p, bool tokens) {
-    if (p.cap_out > 0.0f) p.a.slopes ? att_one<T, true, true>(s, p, tokens) : att_one<T, true, false>(s, p, tokens);
-    else p.a.slopes ? att_one<T, false, true>(s, p, tokens) : att_one<T, false, false>(s, p, tokens);
+    if (p.cap == ATT_FAR) p.a.slopes ? att_one<T, ATT_FAR, true>(s, p, tokens) : att_one<T, ATT_FAR, false>(s, p, tokens);
+    else if (p.cap == ATT_NEAR) p.a.slopes ? att_one<T, ATT_NEAR, true>(s, p, tokens) : att_one<T, ATT_NEAR, false>(s, p, tokens);
+    else p.a.slopes ? att_one<T, ATT_NO_CAP, true>(s, p, tokens) : att_one<T, ATT_NO_CAP, false>(s, p, tokens);
     int rc = op_hip(hipGetLastError(), "attention");
     if (rc != MIBC_OK || p.splits == 1) return rc;
     hipLaunchKernelGGL((attention_join_kernel<T, ATT_D>), dim3((unsigned)((int64_t)p.pairs * p.rows)), dim3(256), 0, s, p);

@@ -1,0 +1,104 @@
+"""Transformer-layer operators (dorado_amd.ops) at the ends of their ranges, against 64-bit implementations: large caps, weights far below
+the largest, values near the type's end, 8-bit codes that have to be the rounded quotients themselves, pytest -m gpu.  The bounds are
+narrower than those of tests/ops_reference.py: none grows with the cap or with the number of keys."""
+import math
+
+import pytest
+import torch
+
+from dorado_amd import ops
+from tests import ops_reference as R
+
+pytestmark = pytest.mark.gpu
+F16, BF16, F32 = torch.float16, torch.bfloat16, torch.float32
+F64 = torch.float64
+
+
+def rnd(shape, t, seed, mul=1.0):
+    g = torch.Generator().manual_seed(seed)
+    return (torch.randn(shape, generator=g) * mul).to(t).cuda()
+
+
+def reference(q, k, v, softcap=0.0, slopes=None, causal=False):
+    """(out, lse, bound of out, bound of lse) in f64.
+
+    A score is off by (d + 8) 2^-24 of its products' magnitudes (an f32 sum of d of them and the scale), by 2^-20 of itself (the exponent's
+    own roundings and, where it is capped, those of tanh: at most eight of 2^-23) and, caps up to 64, by cap 2^-21 (the cap's form there
+    adds numbers of the cap's size: a reciprocal of 1 ulp near 1/2, twice the cap times; two f32 roundings of the cap).  Probabilities are
+    rounded to the type t before the product with v, by at most u(t) of themselves (f16: by at most 2^-38 of the largest); up to 16 rows
+    per key head by two parts, so u(t)^2.  2^-19: sums of keys in f32, joins.  Then one rounding of the output."""
+    t, (b, n, h, d) = q.dtype, q.shape
+    m, kh = k.shape[1], k.shape[2]
+    q, k, v = (x.cpu().to(F64) for x in (q, k, v))
+    i, j = torch.arange(m - n, m)[:, None], torch.arange(m)[None]
+    hidden = (j > i) if causal else torch.zeros(n, m, dtype=torch.bool)
+    out, tol = torch.zeros(b, n, h, d, dtype=F64), torch.zeros(b, n, h, d, dtype=F64)
+    lse, ltol = torch.zeros(b, h, n, dtype=F64), torch.zeros(b, h, n, dtype=F64)
+    pu = R.u(t) ** 2 if n * (h // kh) <= 16 else R.u(t)
+    for x in range(b):
+        for y in range(h):
+            kk, vv, qq = k[x, :, y * kh // h], v[x, :, y * kh // h], q[x, :, y]
+            s = (qq @ kk.T) * d ** -0.5
+            es = (d + 8) * 2.0 ** -24 * (qq.abs() @ kk.abs().T) * d ** -0.5
+            if softcap > 0:
+                s = softcap * torch.tanh(s / softcap)
+                es = es + (softcap * 2.0 ** -21 if softcap <= 64 else 0.0)
+            if slopes is not None:
+                s = s - float(slopes[y]) * (i - j).abs()
+                es = es + abs(float(slopes[y])) * (i - j).abs() * 2.0 ** -20
+            es = (es + 2.0 ** -20 * s.abs()).nan_to_num(0.0, 0.0, 0.0).masked_fill(hidden, 0.0).amax(1, keepdim=True)
+            s = s.masked_fill(hidden, -math.inf)
+            top = s.amax(1, keepdim=True)
+            p = torch.exp(s - top)
+            total = p.sum(1, keepdim=True)
+            out[x, :, y] = (p @ vv) / total
+            floor = ((~hidden).to(F64) @ vv.abs()) * (2.0 ** -38 if t is F16 else 0.0)
+            tol[x, :, y] = ((p @ vv.abs()) * (pu + 2 * es + 2.0 ** -19) + floor) / total + R.u(t) * out[x, :, y].abs() + R.least(t)
+            lse[x, y] = (top + torch.log(total))[:, 0]
+            ltol[x, y] = es[:, 0] + 2.0 ** -19 + 2.0 ** -21 * lse[x, y].abs()
+    return out, lse, tol, ltol
+
+
+def check(q, k, v, **kw):
+    out, lse = ops.attention(q, k, v, return_lse=True, **{x: (y.cuda() if isinstance(y, torch.Tensor) else y) for x, y in kw.items()})
+    want, wlse, tol, ltol = reference(q, k, v, **kw)
+    R.close(out, want, tol, "out")
+    R.close(lse, wlse, ltol, "lse")
+    return out, lse
+
+
+# rows per key head and keys: single tokens, a few, one tile, several tiles, each whole and in parts
+PATHS = [(1, 300), (3, 2100), (40, 300), (40, 2100), (200, 260)]
+
+
+# ------------------------------------------------------------------------------------------------------------------- caps
+@pytest.mark.parametrize("n,m", PATHS)
+@pytest.mark.parametrize("t,d", [(F16, 64), (BF16, 128)])
+@pytest.mark.parametrize("cap,mul", [(5.0, 1.5), (64.0, 1.5), (65.0, 1.5), (65.0, 60.0), (300.0, 1.5), (300.0, 150.0), (1e4, 1.5), (1e4, 3000.0),
+                                     (1e6, 1.5), (1e8, 30.0), (1e30, 1.5)])
+def test_caps(cap, mul, t, d, n, m):
+    q, k, v = rnd((2, n, 2, d), t, 1, mul), rnd((2, m, 1, d), t, 2), rnd((2, m, 1, d), t, 3)
+    check(q, k, v, softcap=cap, causal=True)
+
+
+@pytest.mark.parametrize("n,m", PATHS)
+def test_caps_with_slopes(n, m):
+    q, k, v = rnd((1, n, 2, 96), BF16, 4, 2.0), rnd((1, m, 1, 96), BF16, 5), rnd((1, m, 1, 96), BF16, 6)
+    for cap in (20.0, 1e3, 1e7):
+        check(q, k, v, softcap=cap, slopes=torch.tensor([0.25, -0.001]))
+
+
+@pytest.mark.parametrize("n,m", PATHS)
+@pytest.mark.parametrize("t,d", [(F16, 32), (BF16, 128)])
+def test_a_cap_far_above_the_scores_changes_nothing(t, d, n, m):
+    q, k, v = rnd((2, n, 2, d), t, 7, 2.0), rnd((2, m, 2, d), t, 8), rnd((2, m, 2, d), t, 9)
+    plain, capped = (ops.attention(q, k, v, softcap=c, return_lse=True) for c in (0.0, 1e30))
+    assert torch.equal(plain[0], capped[0]) and torch.equal(plain[1], capped[1])
+
+
+@pytest.mark.parametrize("n,m", PATHS)
+@pytest.mark.parametrize("cap", [30.0, 1e3])
+def test_infinite_scores_are_capped(cap, n, m):
+    q, k, v = rnd((1, n, 2, 64), BF16, 10).abs() + 0.1, rnd((1, m, 1, 64), BF16, 11), rnd((1, m, 1, 64), BF16, 12)
+    k[0, 5], k[0, 6] = math.inf, -math.inf
+    check(q, k, v, softcap=cap)

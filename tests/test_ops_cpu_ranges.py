@@ -1,0 +1,10 @@
+"""Transformer-layer operators without a GPU: refusals at the ends of their ranges, decided from the arguments alone."""
+import pytest
+
+from tests.test_ops_cpu import ATTN, call
+
+
+@pytest.mark.parametrize("change", [dict(softcap=1e30, scale=1e-10), dict(softcap=1.0, scale=1e-38), dict(softcap=1e-35, scale=1e5)])
+def test_attention_refuses_caps_beyond_f32(change):
+    rc, text = call(2, {**ATTN, "out": 1 << 21}, **change)
+    assert rc == -1 and "for this scale" in text
