@@ -11,12 +11,17 @@ typedef short short4_att __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) void *att_lds_vptr;
 typedef const __attribute__((address_space(1))) char *att_gptr;
 
+// The matrix instructions take weights in the type of v: 2^LIFT times exp(score - the running maximum), which is only moved when it grew
+// by more than 2^GROW, so that most tiles rescale nothing.  f16 ends at 2^16 and drops what is below 2^-25: with 2^11 and 2^4 a weight is
+// off by at most 2^-36 of the largest (2^17 such keys by 2^-19), whereas 2^0 and 2^8 lost 0.2 % of the mass of 131072 keys 18 below a
+// single one.  2^13 and 2^2 rescale more often (4 x 16 heads x 4096 of 64 with scores of spread 4: 345 us against 342).  bf16 has f32's range.
 template <typename T>
 struct AttType;
 template <>
 struct AttType<half_t> {
     typedef half8_t vec8;
     static constexpr unsigned EXPONENT = 0x7c00, MANTISSA = 0x03ff, ONE = 0x3c00;
+    static constexpr float LIFT = 11.0f, GROW = 4.0f;
     static __device__ __forceinline__ float16_t mfma32(vec8 a, vec8 b, float16_t c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
     static __device__ __forceinline__ float4_t mfma16(vec8 a, vec8 b, float4_t c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
 };
@@ -24,6 +29,7 @@ template <>
 struct AttType<bf16_t> {
     typedef bf16x8_t vec8;
     static constexpr unsigned EXPONENT = 0x7f80, MANTISSA = 0x007f, ONE = 0x3f80;
+    static constexpr float LIFT = 0.0f, GROW = 8.0f;
     static __device__ __forceinline__ float16_t mfma32(vec8 a, vec8 b, float16_t c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
     static __device__ __forceinline__ float4_t mfma16(vec8 a, vec8 b, float4_t c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
 };
@@ -417,9 +423,7 @@ __global__ __launch_bounds__(256, D <= 64 ? 3 : 2) void attention_kernel(AttArgs
         float top = s[0][0];
         ATT_EACH top = score.larger(top, s[i][r]);
         top = att_half_max(fmaf(top, score.mul, score.add));
-        // the maximum is only moved when it grew by more than 2^8: probabilities stay below 256, which 16 bits and f32 sums
-        // hold as well as values below 1
-        if (__any(top > m + 8.0f)) {
+        if (__any(top > m + X::GROW)) {
             const float mn = fmaxf(m, top);
             const float f = m == -INFINITY ? 0.0f : att_exp2(m - mn);
             m = mn;
@@ -429,7 +433,7 @@ __global__ __launch_bounds__(256, D <= 64 ? 3 : 2) void attention_kernel(AttArgs
 #pragma unroll
                 for (int r = 0; r < 16; ++r) o[db][r] = decltype(safe_)::value ? att_weigh(f, o[db][r]) : o[db][r] * f;
         }
-        off = score.add - (m == -INFINITY ? 0.0f : m);
+        off = score.add + X::LIFT - (m == -INFINITY ? 0.0f : m);
     };
     auto probabilities = [&](int k) {       // of 16 keys
         uintx4 w;
@@ -548,8 +552,10 @@ __global__ __launch_bounds__(256, D <= 64 ? 3 : 2) void attention_kernel(AttArgs
     }
 
     l = att_half_add(l);
+    constexpr float DOWN = 1.0f / (float)(1 << (int)X::LIFT);
     const float base = m == -INFINITY ? 0.0f : m;
     const float inv = l == 0.0f ? 0.0f : __builtin_amdgcn_rcpf(l);
+    l *= DOWN;
     {   // row, token and head are worked out again rather than kept in registers over the loop
         const AttArgs &p = att_args_again();
         const mibc_attention_args &a = p.a;
@@ -725,7 +731,7 @@ __global__ __launch_bounds__(256, 2) void attention_token_kernel(AttArgs p) {
 #pragma unroll
                 for (int r = 0; r < 4; ++r) top = score.larger(top, s[i][r]);
             top = fmaf(top, score.mul, score.add);
-            if (__any(top > m + 8.0f)) {     // m is the row's, the same in its four lanes
+            if (__any(top > m + X::GROW)) {     // m is the row's, the same in its four lanes
                 top = fmaxf(top, __shfl_xor(top, 16, 64));
                 top = fmaxf(top, __shfl_xor(top, 32, 64));
                 const float mn = fmaxf(m, top);
@@ -737,7 +743,7 @@ __global__ __launch_bounds__(256, 2) void attention_token_kernel(AttArgs p) {
 #pragma unroll
                     for (int r = 0; r < 4; ++r) o[db][r] = SAFE ? att_weigh(f, o[db][r]) : o[db][r] * f;
             }
-            const float off = score.add - (m == -INFINITY ? 0.0f : m);
+            const float off = score.add + X::LIFT - (m == -INFINITY ? 0.0f : m);
             uintx4 hi, lo;
 #pragma unroll
             for (int i = 0; i < 2; ++i)
@@ -821,6 +827,7 @@ __global__ __launch_bounds__(256, 2) void attention_token_kernel(AttArgs p) {
             for (int e = 0; e < 4; ++e) y[e] += att_weigh(f, x[e]);
         }
         const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+        sum *= 1.0f / (float)(1 << (int)X::LIFT);
         const int rt = p.by_group.div(r), rh = kvh * p.group + (r - rt * p.group);
         if (p.splits > 1) {
             const int64_t at = ((int64_t)pair * p.rows + r) * p.splits + split;

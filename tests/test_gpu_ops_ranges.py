@@ -25,7 +25,8 @@ def reference(q, k, v, softcap=0.0, slopes=None, causal=False):
     A score is off by (d + 8) 2^-24 of its products' magnitudes (an f32 sum of d of them and the scale), by 2^-20 of itself (the exponent's
     own roundings and, where it is capped, those of tanh: at most eight of 2^-23) and, caps up to 64, by cap 2^-21 (the cap's form there
     adds numbers of the cap's size: a reciprocal of 1 ulp near 1/2, twice the cap times; two f32 roundings of the cap).  Probabilities are
-    rounded to the type t before the product with v, by at most u(t) of themselves (f16: by at most 2^-38 of the largest); up to 16 rows
+    rounded to the type t before the product with v, by at most u(t) of themselves (f16: by at most 2^-36 of the largest: half a step of
+    2^-24, with 2^11 in front); up to 16 rows
     per key head by two parts, so u(t)^2.  2^-19: sums of keys in f32, joins.  Then one rounding of the output."""
     t, (b, n, h, d) = q.dtype, q.shape
     m, kh = k.shape[1], k.shape[2]
@@ -52,7 +53,7 @@ def reference(q, k, v, softcap=0.0, slopes=None, causal=False):
             p = torch.exp(s - top)
             total = p.sum(1, keepdim=True)
             out[x, :, y] = (p @ vv) / total
-            floor = ((~hidden).to(F64) @ vv.abs()) * (2.0 ** -38 if t is F16 else 0.0)
+            floor = ((~hidden).to(F64) @ vv.abs()) * (2.0 ** -36 if t is F16 else 0.0)
             tol[x, :, y] = ((p @ vv.abs()) * (pu + 2 * es + 2.0 ** -19) + floor) / total + R.u(t) * out[x, :, y].abs() + R.least(t)
             lse[x, y] = (top + torch.log(total))[:, 0]
             ltol[x, y] = es[:, 0] + 2.0 ** -19 + 2.0 ** -21 * lse[x, y].abs()
@@ -102,3 +103,23 @@ def test_infinite_scores_are_capped(cap, n, m):
     q, k, v = rnd((1, n, 2, 64), BF16, 10).abs() + 0.1, rnd((1, m, 1, 64), BF16, 11), rnd((1, m, 1, 64), BF16, 12)
     k[0, 5], k[0, 6] = math.inf, -math.inf
     check(q, k, v, softcap=cap)
+
+
+# ------------------------------------------------------------------------------------------- weights far below the largest
+@pytest.mark.parametrize("away", [12.0, 17.0, 18.0, 21.0])
+@pytest.mark.parametrize("t,d", [(F16, 64), (F16, 128), (BF16, 64)])
+@pytest.mark.parametrize("n,m", [(1, 131072), (4, 20000), (40, 20000), (130, 3000)])
+def test_many_keys_far_below_a_sink(n, m, t, d, away):
+    # one key without a value of its own stands `away` above all others, whose weights then make up the whole result
+    q, k, v = torch.zeros((1, n, 1, d), dtype=t), torch.zeros((1, m, 1, d), dtype=t), rnd((1, m, 1, d), t, 13).abs().cpu() + 0.5
+    q[..., 0], k[0, m // 3, 0, 0], v[0, m // 3] = 1.0, away * d ** 0.5, 0.0
+    check(q.cuda(), k.cuda(), v.cuda())
+
+
+@pytest.mark.parametrize("n,m", PATHS)
+@pytest.mark.parametrize("away", [8.0, 16.0])
+def test_weights_far_below_a_sink_of_all_sizes(away, n, m):
+    q, k, v = rnd((2, n, 2, 64), F16, 14), rnd((2, m, 1, 64), F16, 15), rnd((2, m, 1, 64), F16, 16).abs()
+    q[..., 0], k[..., 0] = 1.0, 0.0
+    k[:, 1, :, 0], v[:, 1] = away * 8, 0.0
+    check(q, k, v, causal=n > 1 and m > n)
