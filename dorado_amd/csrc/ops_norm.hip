@@ -171,13 +171,26 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void rms_norm_kernel(NormArg
         const bool fine = top[i] < 0x7f800000u;
         float s = fine ? __uint_as_float(top[i]) / most : NAN;
         if (s == 0.0f) s = 1.0f;     // nothing but zeros, or values whose scale is below f32
-        // the reciprocal of a scale below 2^-126 overflows: both sides are lifted by 2^64 first
-        const float lift = s < 1e-30f ? 0x1p64f : 1.0f, inv = 1.0f / (s * lift);
         unsigned lo = 0, hi = 0;
         if (fine) {
-            float v[8];              // at most 127 or 448 times 1 + 2^-22: rounds to the largest code
+            // y / s, rounded once: the product with the rounded reciprocal is off by a step or two, its remainder is exact, and one
+            // more product with the reciprocal sets it right
+            float v[8];              // at most 127 or 448 times 1 + 2^-23: rounds to the largest code
+            const auto divide = [&](float by) {
+                const float inv = 1.0f / by;
 #pragma unroll
-            for (int e = 0; e < 8; ++e) v[e] = h[i][e] * lift * inv;
+                for (int e = 0; e < 8; ++e) {
+                    const float q = h[i][e] * inv;
+                    v[e] = fmaf(fmaf(-q, by, h[i][e]), inv, q);
+                }
+            };
+            if (s >= 1e-20f) {
+                divide(s);
+            } else {                 // remainders and reciprocals beyond f32: both sides are lifted by 2^64 first
+#pragma unroll
+                for (int e = 0; e < 8; ++e) h[i][e] *= 0x1p64f;
+                divide(s * 0x1p64f);
+            }
             if (a.out_type == MIBC_TYPE_I8) {
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {

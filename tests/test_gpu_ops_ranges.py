@@ -123,3 +123,27 @@ def test_weights_far_below_a_sink_of_all_sizes(away, n, m):
     q[..., 0], k[..., 0] = 1.0, 0.0
     k[:, 1, :, 0], v[:, 1] = away * 8, 0.0
     check(q, k, v, causal=n > 1 and m > n)
+
+
+# ------------------------------------------------------------------------------------------------------------ 8-bit codes
+def codes_of(y, s, quant):
+    """round(y / s) in f32 as a whole number or e4m3 (nearest, ties to even), where s is a rounded quotient of the group's largest |y|."""
+    v = (y.view(*s.shape, -1) / s[..., None]).view(y.shape)
+    most = 127.0 if quant == "int8" else 448.0
+    v = v.clamp(-most, most)
+    return v.round().to(torch.int8) if quant == "int8" else v.to(torch.float8_e4m3fn)
+
+
+@pytest.mark.parametrize("quant", ["int8", "e4m3"])
+@pytest.mark.parametrize("cols,group,rows", [(4096, 0, 4096), (4096, 128, 4096), (1000, 0, 8000), (64, 32, 60000), (11320, 0, 999), (20000, 0, 300)])
+def test_codes_are_rounded_quotients(cols, group, rows, quant):
+    x, w = rnd((rows, cols), F32, 17), rnd((cols,), F32, 18) + 1
+    y = ops.rms_norm(x, w).cpu()
+    q, s = ops.rms_norm(x, w, quant=quant, group=group)
+    q, s = q.cpu(), s.cpu()
+    most = 127.0 if quant == "int8" else 448.0
+    largest = y.view(rows, -1, group or cols).abs().amax(-1)
+    assert torch.equal(s, largest / torch.tensor(most))
+    want = codes_of(y, s, quant)
+    assert torch.equal(q.view(torch.uint8), want.view(torch.uint8)), int((q.view(torch.uint8) != want.view(torch.uint8)).sum())
+    assert (q.float().view(rows, -1, group or cols).abs().amax(-1) == most).all()      # the group's largest value gets the largest code
