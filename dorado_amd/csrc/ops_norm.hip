@@ -190,6 +190,9 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void rms_norm_kernel(NormArg
 #pragma unroll
                 for (int e = 0; e < 8; ++e) h[i][e] *= 0x1p64f;
                 divide(s * 0x1p64f);
+                // a scale of few bits is off by up to a third
+#pragma unroll
+                for (int e = 0; e < 8; ++e) v[e] = fminf(fmaxf(v[e], -most), most);
             }
             if (a.out_type == MIBC_TYPE_I8) {
 #pragma unroll

@@ -254,7 +254,7 @@ MIBC_API int mibc_svb16_decode(mibc_engine *e, const uint8_t *streams_dev, const
  * in between.  sum_out (optional) receives h, out receives y, both in `type`; or, out_type I8 / E4M3, out receives
  * round(y / s) (the f32 quotient, then the code, nearest with ties to even), s = max|y| / 127 (I8) or / 448 (E4M3) over the row
  * (group 0) or over each group of 32, 64 or 128 columns, and scale_out [rows][cols / group] receives s.  Where max|y| is 0, s = 1; where a value of the group is not finite, s = NaN
- * and the group's codes are 0.  weight: f32 or `type`, NULL = ones; residual NULL = none.  1 <= cols <= 32768. */
+ * and the group's codes are 0; codes end at 127 and 448 (a scale of some 2^-149 steps is off by up to a third; below half a step s = 1).  weight: f32 or `type`, NULL = ones; residual NULL = none.  1 <= cols <= 32768. */
 typedef struct mibc_rms_norm_args {
     const void *x, *residual, *weight;
     void *sum_out, *out;

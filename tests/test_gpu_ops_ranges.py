@@ -147,3 +147,21 @@ def test_codes_are_rounded_quotients(cols, group, rows, quant):
     want = codes_of(y, s, quant)
     assert torch.equal(q.view(torch.uint8), want.view(torch.uint8)), int((q.view(torch.uint8) != want.view(torch.uint8)).sum())
     assert (q.float().view(rows, -1, group or cols).abs().amax(-1) == most).all()      # the group's largest value gets the largest code
+
+
+@pytest.mark.parametrize("quant,most", [("int8", 127), ("e4m3", 448)])
+def test_scales_of_few_bits(quant, most):
+    # values of some hundred of f32's smallest steps: the scale is a step or two, off by up to a third, and codes end at the largest one
+    step = 2.0 ** -149
+    for top in (0.4, 0.6, 1.0, 1.4, 1.49, 2.4, 3.5, 100.0, 1e4):
+        w = (torch.linspace(-1.0, 1.0, 64, dtype=F64) * (top * most)).round() * step
+        x = torch.ones((3, 64), device="cuda")
+        y = ops.rms_norm(x, w.float().cuda(), eps=0.0).cpu()
+        assert torch.equal(y[0], w.float())                 # 1 / sqrt(1) and the product are exact
+        q, s = ops.rms_norm(x, w.float().cuda(), eps=0.0, quant=quant)
+        want = (y.abs().amax(1, keepdim=True).double() / step / most).round() * step
+        want = torch.where(want == 0, torch.ones_like(want), want)
+        assert torch.equal(s.cpu().double(), want), (float(s[0]), float(want[0]))
+        ratio = (y.double() / want).float().clamp(-most, most)      # exact: both are whole numbers of steps below 2^24
+        code = ratio.round().to(torch.int8) if quant == "int8" else ratio.to(torch.float8_e4m3fn)
+        assert torch.equal(q.cpu().view(torch.uint8), code.view(torch.uint8)), top
