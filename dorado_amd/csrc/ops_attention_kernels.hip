@@ -14,14 +14,16 @@ typedef const __attribute__((address_space(1))) char *att_gptr;
 // The matrix instructions take weights in the type of v: 2^LIFT times exp(score - the running maximum), which is only moved when it grew
 // by more than 2^GROW, so that most tiles rescale nothing.  f16 ends at 2^16 and drops what is below 2^-25: with 2^11 and 2^4 a weight is
 // off by at most 2^-36 of the largest (2^17 such keys by 2^-19), whereas 2^0 and 2^8 lost 0.2 % of the mass of 131072 keys 18 below a
-// single one.  2^13 and 2^2 rescale more often (4 x 16 heads x 4096 of 64 with scores of spread 4: 345 us against 342).  bf16 has f32's range.
+// single one.  2^13 and 2^2 rescale more often (4 x 16 heads x 4096 of 64 with scores of spread 4: 345 us against 342).  bf16 has f32's range,
+// so sums of its values may end beyond f32: where one did, the pass for values that are not finite runs at 2^-40 (2^28 keys of weight 2^8 stay
+// below 2^-4 of the largest value; values below 2^-86 lose bits beside such sums).
 template <typename T>
 struct AttType;
 template <>
 struct AttType<half_t> {
     typedef half8_t vec8;
     static constexpr unsigned EXPONENT = 0x7c00, MANTISSA = 0x03ff, ONE = 0x3c00;
-    static constexpr float LIFT = 11.0f, GROW = 4.0f;
+    static constexpr float LIFT = 11.0f, LIFT_AGAIN = 11.0f, GROW = 4.0f;
     static __device__ __forceinline__ float16_t mfma32(vec8 a, vec8 b, float16_t c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
     static __device__ __forceinline__ float4_t mfma16(vec8 a, vec8 b, float4_t c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
 };
@@ -29,7 +31,7 @@ template <>
 struct AttType<bf16_t> {
     typedef bf16x8_t vec8;
     static constexpr unsigned EXPONENT = 0x7f80, MANTISSA = 0x007f, ONE = 0x3f80;
-    static constexpr float LIFT = 0.0f, GROW = 8.0f;
+    static constexpr float LIFT = 0.0f, LIFT_AGAIN = -40.0f, GROW = 8.0f;
     static __device__ __forceinline__ float16_t mfma32(vec8 a, vec8 b, float16_t c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
     static __device__ __forceinline__ float4_t mfma16(vec8 a, vec8 b, float4_t c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
 };
@@ -433,7 +435,7 @@ __global__ __launch_bounds__(256, D <= 64 ? 3 : 2) void attention_kernel(AttArgs
 #pragma unroll
                 for (int r = 0; r < 16; ++r) o[db][r] = decltype(safe_)::value ? att_weigh(f, o[db][r]) : o[db][r] * f;
         }
-        off = score.add + X::LIFT - (m == -INFINITY ? 0.0f : m);
+        off = score.add + (decltype(safe_)::value ? X::LIFT_AGAIN : X::LIFT) - (m == -INFINITY ? 0.0f : m);
     };
     auto probabilities = [&](int k) {       // of 16 keys
         uintx4 w;
@@ -505,7 +507,7 @@ __global__ __launch_bounds__(256, D <= 64 ? 3 : 2) void attention_kernel(AttArgs
     if (__any(odd) && lane == 0) flag = 1;
     __syncthreads();
     if (flag) {
-        // something is not finite: from a value or key that the row sees, or 0 * (a value that it does not see).  Once more, tile by tile: values
+        // something is not finite: from a value or key that the row sees, 0 * (a value that it does not see), or a sum beyond f32.  Once more, tile by tile: values
         // that are not finite stay out of the products, and the places of NaN (kind 0), infinity (1) and -infinity (2) are
         // multiplied with the mask instead, so that they reach the rows that see their key and no other
         start();
@@ -552,10 +554,9 @@ __global__ __launch_bounds__(256, D <= 64 ? 3 : 2) void attention_kernel(AttArgs
     }
 
     l = att_half_add(l);
-    constexpr float DOWN = 1.0f / (float)(1 << (int)X::LIFT);
     const float base = m == -INFINITY ? 0.0f : m;
     const float inv = l == 0.0f ? 0.0f : __builtin_amdgcn_rcpf(l);
-    l *= DOWN;
+    l *= att_exp2(flag ? -X::LIFT_AGAIN : -X::LIFT);
     {   // row, token and head are worked out again rather than kept in registers over the loop
         const AttArgs &p = att_args_again();
         const mibc_attention_args &a = p.a;
@@ -743,7 +744,7 @@ __global__ __launch_bounds__(256, 2) void attention_token_kernel(AttArgs p) {
 #pragma unroll
                     for (int r = 0; r < 4; ++r) o[db][r] = SAFE ? att_weigh(f, o[db][r]) : o[db][r] * f;
             }
-            const float off = score.add + X::LIFT - (m == -INFINITY ? 0.0f : m);
+            const float off = score.add + (SAFE ? X::LIFT_AGAIN : X::LIFT) - (m == -INFINITY ? 0.0f : m);
             uintx4 hi, lo;
 #pragma unroll
             for (int i = 0; i < 2; ++i)
@@ -790,14 +791,18 @@ __global__ __launch_bounds__(256, 2) void attention_token_kernel(AttArgs p) {
         }
     };
     pass(std::false_type());
-    bool odd = false;
+    float zero = 0.0f;
 #pragma unroll
     for (int db = 0; db < D / 16; ++db)
 #pragma unroll
-        for (int r = 0; r < 4; ++r) odd = odd || o[db][r] != o[db][r];
-    if (__any(odd)) pass(std::true_type());
+        for (int r = 0; r < 4; ++r) zero = fmaf(o[db][r], 0.0f, zero);
+    if (__any(zero != 0.0f)) {
+        pass(std::true_type());
+        m += X::LIFT - X::LIFT_AGAIN;     // the other waves' unit
+    }
 
-    // the four waves' parts, through LDS: [wave][16 rows][D] sums, [wave][16] maxima and sums of a row
+    // the four waves' parts, through LDS: [wave][16 rows][D] sums, [wave][16] maxima and sums of a row; a quarter of each, so that four
+    // finite ones end inside f32
     l += __shfl_xor(l, 16, 64);
     l += __shfl_xor(l, 32, 64);
     __syncthreads();
@@ -820,14 +825,14 @@ __global__ __launch_bounds__(256, 2) void attention_token_kernel(AttArgs p) {
         floatx4 y = (floatx4)(0.0f);
 #pragma unroll
         for (int w = 0; w < 4; ++w) {
-            const float f = sm[w * 16 + r] == -INFINITY ? (sl[w * 16 + r] == 0.0f ? 0.0f : 1.0f) : att_exp2(sm[w * 16 + r] - base);
+            const float f = sm[w * 16 + r] == -INFINITY ? (sl[w * 16 + r] == 0.0f ? 0.0f : 0.25f) : 0.25f * att_exp2(sm[w * 16 + r] - base);
             sum = fmaf(f, sl[w * 16 + r], sum);
             const floatx4 x = *(const floatx4 *)(so + (w * 16 + r) * OLD + d4);      // zeros for a wave without keys
 #pragma unroll
             for (int e = 0; e < 4; ++e) y[e] += att_weigh(f, x[e]);
         }
         const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-        sum *= 1.0f / (float)(1 << (int)X::LIFT);
+        sum *= 4.0f / (float)(1 << (int)X::LIFT);
         const int rt = p.by_group.div(r), rh = kvh * p.group + (r - rt * p.group);
         if (p.splits > 1) {
             const int64_t at = ((int64_t)pair * p.rows + r) * p.splits + split;
@@ -887,7 +892,7 @@ __global__ __launch_bounds__(256) void attention_join_kernel(AttArgs p) {
 #pragma unroll
         for (int i = 0; i < 8; ++i)
             if (first + i * G < p.splits) {
-                const float f = att_exp2(w[i] - base);
+                const float f = att_exp2(w[i] - base) * 0x1p-8f;      // 255 finite parts end inside f32
                 sum += f;
 #pragma unroll
                 for (int e = 0; e < 4; ++e) y[e] += att_weigh(f, x[i][e]);      // a part without keys holds zeros
@@ -910,7 +915,7 @@ __global__ __launch_bounds__(256) void attention_join_kernel(AttArgs p) {
         const float inv = n == 0.0f ? 0.0f : 1.0f / n;
         ((T *)a.out + b * a.out_stride[0] + t * a.out_stride[1] + head * a.out_stride[2])[d] = (T)(v * inv);
         if (a.lse != nullptr && d == 0)
-            a.lse[((int64_t)b * a.heads + head) * a.q_tokens + t] = n == 0.0f ? -INFINITY : base * 0.6931471805599453f + logf(n);
+            a.lse[((int64_t)b * a.heads + head) * a.q_tokens + t] = n == 0.0f ? -INFINITY : base * 0.6931471805599453f + logf(n * 0x1p8f);
     }
 }
 

@@ -165,3 +165,29 @@ def test_scales_of_few_bits(quant, most):
         ratio = (y.double() / want).float().clamp(-most, most)      # exact: both are whole numbers of steps below 2^24
         code = ratio.round().to(torch.int8) if quant == "int8" else ratio.to(torch.float8_e4m3fn)
         assert torch.equal(q.cpu().view(torch.uint8), code.view(torch.uint8)), top
+
+
+# ------------------------------------------------------------------------------------------------ values near the type's end
+@pytest.mark.parametrize("n,m", PATHS + [(1, 9000), (16, 20), (40, 9000)])
+@pytest.mark.parametrize("d", [32, 128])
+@pytest.mark.parametrize("size", [1e31, 1e36, 3.3e38])
+def test_sums_of_values_near_the_end_of_bf16(size, d, n, m):
+    # a mean of finite values is finite, however many of them there are
+    q, k = rnd((2, n, 2, d), BF16, 19), rnd((2, m, 1, d), BF16, 20)
+    v = (torch.rand((2, m, 1, d), generator=torch.Generator().manual_seed(21)) * 0.5 + 0.5) * size
+    v[1, :, :, ::2] *= -1
+    v[0, :, :, 1] = 1.0                            # an ordinary column beside them
+    out, _ = check(q, k, v.to(BF16).cuda(), causal=n > 1)
+    assert out.isfinite().all()
+
+
+@pytest.mark.parametrize("n,m", PATHS)
+def test_infinities_beside_values_near_the_end(n, m):
+    q, k = rnd((1, n, 1, 64), BF16, 22), rnd((1, m, 1, 64), BF16, 23)
+    v = torch.full((1, m, 1, 64), 3.3e38, dtype=BF16)
+    v[0, 3, 0, 5], v[0, 4, 0, 6], v[0, 5, 0, 7] = math.inf, -math.inf, math.nan
+    out = ops.attention(q, k, v.cuda())
+    assert (out[..., 5] == math.inf).all() and (out[..., 6] == -math.inf).all() and out[..., 7].isnan().all()
+    want = reference(q, k, torch.full_like(v, 3.3e38))
+    rest = [c for c in range(64) if c not in (5, 6, 7)]
+    R.close(out[..., rest], want[0][..., rest], want[2][..., rest], "other columns")
