@@ -14,6 +14,9 @@ static int att_check(const mibc_attention_args &a) {
     if (!(a.softcap >= 0.0f) || !(a.softcap <= 1e30f)) return op_refuse(MIBC_ERR_ARG, "attention: softcap must be 0 (none) or positive and finite");
     if (a.softcap > 0.0f && !(3.0f * a.scale / a.softcap <= 3e38f)) return op_refuse(MIBC_ERR_ARG, "attention: softcap too small for this scale");
     if (a.softcap > 0.0f && !(a.softcap / a.scale <= 3e37f)) return op_refuse(MIBC_ERR_ARG, "attention: softcap too large for this scale");
+    // a slope is held in the scores' unit: slope / scale, or slope / (2 softcap)
+    if (a.slopes != nullptr && (a.scale < 1e-18f || (a.softcap > 0.0f && a.softcap < 1e-18f)))
+        return op_refuse(MIBC_ERR_ARG, "attention: slopes need a scale and a softcap of at least 1e-18");
     if (a.reserved != 0) return op_refuse(MIBC_ERR_ARG, "attention: reserved must be 0");
     const int64_t big = (int64_t)1 << 28;     // positions, and distances between them, stay far inside 32 bits
     if (a.q_tokens > big || a.k_tokens > big || (int64_t)a.q_tokens * (a.heads / a.kv_heads) > big ||

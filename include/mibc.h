@@ -306,7 +306,7 @@ MIBC_API int mibc_rope_frequencies(int scaling, int rot_dim, double theta, doubl
  * holds (NaN and infinity included); a NaN or infinity of v that it does see reaches it, however small its weight.  lse (optional)
  * [batch][heads][q_tokens] f32 contiguous: log of the sum of exp(scores).
  * Scores are off by a few 2^-22 of their own size and, for a softcap of up to 64, of the cap's.  softcap / scale may be at most
- * 3e37 and scale / softcap at most 1e38.
+ * 3e37 and scale / softcap at most 1e38; with slopes, both are at least 1e-18, and slopes / scale must stay inside f32.
  * Types F16, BF16; head_dim 32, 64, 96 or 128; token and head strides multiples of 8 elements, pointers aligned to 16 bytes.
  * workspace: mibc_attention_workspace(a) bytes on the device (0, as for any call with fewer than 512 keys: may be NULL), the
  * call's own until it has completed. */

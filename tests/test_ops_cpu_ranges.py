@@ -8,3 +8,10 @@ from tests.test_ops_cpu import ATTN, call
 def test_attention_refuses_caps_beyond_f32(change):
     rc, text = call(2, {**ATTN, "out": 1 << 21}, **change)
     assert rc == -1 and "for this scale" in text
+
+
+@pytest.mark.parametrize("change", [dict(scale=1e-20), dict(softcap=1e-20, scale=1e-10), dict(scale=1e-40, softcap=1e-30)])
+def test_attention_refuses_slopes_beyond_f32(change):
+    # slope / scale is infinite there, and infinity times a distance of 0 is NaN
+    rc, text = call(2, {**ATTN, "out": 1 << 21}, slopes=1 << 22, **change)
+    assert rc == -1 and ("slopes need" in text or "for this scale" in text)
