@@ -41,7 +41,7 @@ int tx_create(mibc_engine *e, const mibc_model_desc &d, const float *const *weig
     tx.D = C;
     tx.H = d.tx_nhead;
     tx.hd = hd;
-    tx.by_ops = hd != 64 || 64 + d.tx_win_upper + d.tx_win_lower > 320;
+    tx.by_ops = hd != 64 || (int64_t)d.tx_win_upper + d.tx_win_lower > 256;
     tx.FF = d.tx_dim_ff;
     tx.depth = d.tx_depth;
     tx.sf = d.up_scale_factor;
