@@ -337,6 +337,12 @@ static int tx_attention_by_ops(mibc_engine *e, int N, int T) {
     return MIBC_OK;
 }
 
+// what an operator's launch returned, as the engine's error: a HIP error or a wrong argument keeps its code and text
+static int tx_op_status(mibc_engine *e, int rc, const char *what) {
+    if (rc == MIBC_OK) return MIBC_OK;
+    return rc < 0 ? fail(e, rc, std::string(mibc_gerr())) : fail(e, MIBC_NOT_SUPPORTED, what);
+}
+
 // x <- RMSNorm(in + alpha * x) * w: the fixed-width kernel where there is one, the operator elsewhere
 static int tx_residual_norm(mibc_engine *e, const half_t *in, half_t *x, const float *w, long rows, int C, float alpha) {
     if (mibc_launch_residual_rmsnorm(e->stream, in, x, w, rows, C, alpha) == 0) return MIBC_OK;
@@ -409,17 +415,17 @@ int tx_run_network(mibc_engine *e, const half_t *in_dev, int N, int T_in) {
         else
             arc = mibc_launch_window_attention(e->stream, tx.qkv, tx.attn, N, T, C, tx.H, d.tx_win_upper,
                                                d.tx_win_lower);
-        if (arc != 0) return fail(e, MIBC_NOT_SUPPORTED, "tx attention shape");
+        if (const int rc = tx_op_status(e, arc, "tx attention shape")) return rc;
         // everything behind the attention in ONE launch (txlayer.hip) when the model has the sup@v5 width
         if (L.wimg != nullptr && tx.fused &&
             mibc_launch_tx_layer(e->stream, tx.attn, tx.x, L.wimg, L.bo, L.n1, L.n2, d.tx_deepnorm_alpha, R, tx.FF, 3) == 0)
             continue;
         if (gemm(e, tx.attn, L.wo, L.bo, tx.tmp, R, C, C, -1) != 0) return fail(e, MIBC_NOT_SUPPORTED, "tx out_proj");
-        if (tx_residual_norm(e, tx.tmp, tx.x, L.n1, R, C, d.tx_deepnorm_alpha) != 0) return fail(e, MIBC_NOT_SUPPORTED, "tx rmsnorm");
+        if (const int rc = tx_op_status(e, tx_residual_norm(e, tx.tmp, tx.x, L.n1, R, C, d.tx_deepnorm_alpha), "tx rmsnorm")) return rc;
         if (gemm(e, tx.x, L.wfc1, nullptr, tx.ff, R, 2 * tx.FF, C, -1, /*swiglu*/ 2, 0, tx.FF) != 0)
             return fail(e, MIBC_NOT_SUPPORTED, "tx fc1");
         if (gemm(e, tx.ff, L.wfc2, nullptr, tx.tmp, R, C, tx.FF, -1) != 0) return fail(e, MIBC_NOT_SUPPORTED, "tx fc2");
-        if (tx_residual_norm(e, tx.tmp, tx.x, L.n2, R, C, d.tx_deepnorm_alpha) != 0) return fail(e, MIBC_NOT_SUPPORTED, "tx rmsnorm");
+        if (const int rc = tx_op_status(e, tx_residual_norm(e, tx.tmp, tx.x, L.n2, R, C, d.tx_deepnorm_alpha), "tx rmsnorm")) return rc;
     }
     // upsample: [R][C] -> [R][sf*C] == [N][sf*T][C]
     if (gemm(e, tx.x, tx.wup, tx.bup, tx.up, R, tx.sf * C, C, -1) != 0) return fail(e, MIBC_NOT_SUPPORTED, "tx upsample");
@@ -441,6 +447,12 @@ int tx_run_head(mibc_engine *e, int N, int n0, int ns, half_t *scores_out) {
 }
 
 #ifdef MIBC_DEBUG_KERNELS
+// Test entry (debug library only): what a caller of the engine sees of an operator's launch that returned `rc` with `text`
+MIBC_HOOK int mibc_debug_tx_op_status(int rc, const char *text) {
+    mibc_gerr() = text;
+    return tx_op_status(nullptr, rc, "tx attention shape");
+}
+
 // Test entry (debug library only): the fused layer tail (txlayer.hip) against the five-launch path it replaces
 // (gemm256 out-proj -> residual_rmsnorm -> gemm256 FC1 + SwiGLU -> gemm256 FC2 -> residual_rmsnorm) on the same
 // pseudo-random attn / x / weights.  mode 3 = whole tail, 1 = out-proj + norm 1 only (contract: bit-identical), 2 = MLP +
