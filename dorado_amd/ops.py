@@ -4,13 +4,15 @@
 Tensors live on one HIP device; the work goes to torch's current stream of that device and nothing is synchronised.  New
 outputs and the workspace of a split attention come from torch's caching allocator, so a call can be captured into a graph.
 There is no CPU form: a tensor elsewhere raises.  Forward only; no autograd graph is recorded, so inputs that require a
-gradient are refused while gradients are being recorded."""
+gradient are refused while gradients are being recorded, and so are forward-mode tangents, tracing (torch.jit.trace, make_fx) and
+tensors without memory of their own (fake, functional, symbolic zeros): all of these would pass the work by."""
 from __future__ import annotations
 
 import ctypes as C
 import struct
 
 import torch
+from torch.autograd import forward_ad
 
 from .capi import MIBC_OK, MibcError, MibcNotSupported, lib
 
@@ -50,8 +52,21 @@ def _check(rc: int, what: str) -> None:
         raise (MibcNotSupported if rc > 0 else MibcError)(f"{what}: {lib().mibc_last_error(None).decode()}")
 
 
+_is_tracing, _modes = torch._C._is_tracing, torch._C._len_torch_dispatch_stack
+
+
+def _infra(mode) -> bool:
+    return getattr(mode, "_mode_key", None) is not None      # proxies, fake and functional tensors; counters and loggers have none
+
+
 def _device(what: str, first: torch.Tensor, *others) -> int:
-    """The device index all tensors share; refuses tensors elsewhere and gradients."""
+    """The device index all tensors share; refuses tensors elsewhere, gradients and transformations."""
+    if _is_tracing() or (_modes() and any(map(_infra, torch.utils._python_dispatch._get_current_dispatch_mode_stack()))):
+        raise MibcNotSupported(f"{what}: cannot be traced")
+    if forward_ad._current_level >= 0:
+        for t in (first, *others):
+            if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+                raise MibcNotSupported(f"{what}: forward only; tangents are not carried along")
     dev = first.device
     if dev.type != "cuda":
         raise MibcError(f"{what}: tensors must be on a HIP device (got {dev}); there is no CPU form")
@@ -68,6 +83,16 @@ def _device(what: str, first: torch.Tensor, *others) -> int:
 
 # the current stream's handle, without a Stream object around it where this torch offers that
 _stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda device: torch.cuda.current_stream(device).cuda_stream)
+
+
+def _ptr(what: str, t) -> int:
+    """Address of an operand that may be left out (0)."""
+    if t is None:
+        return 0
+    p = t.data_ptr()
+    if p == 0 and t.numel():
+        raise MibcNotSupported(f"{what}: a tensor without memory of its own")
+    return p
 
 
 def _row_stride(what: str, name: str, t: torch.Tensor, cols: int) -> int:
@@ -94,7 +119,7 @@ def _index32(what: str, name: str, t, n: int) -> int:
     """Pointer of a contiguous int32 tensor of n elements."""
     if t.dtype is not torch.int32 or t.shape != (n,) or not t.is_contiguous():
         raise MibcError(f"{what}: {name} must be a contiguous int32 tensor of {n} elements")
-    return t.data_ptr()
+    return _ptr(what, t)
 
 
 def rms_norm(x, weight=None, *, residual=None, alpha: float = 1.0, eps: float = 1e-5, quant=None, group: int = 0,
@@ -111,6 +136,10 @@ def rms_norm(x, weight=None, *, residual=None, alpha: float = 1.0, eps: float = 
     if not shape or shape[-1] == 0:
         raise MibcError("rms_norm: x needs a last dimension")
     cols = shape[-1]
+    if cols == 1:      # the only width at which an imaginary part's view counts as contiguous
+        for t in (x, residual, weight, out, sum_out):
+            if t is not None and t.is_neg():
+                raise MibcNotSupported("rms_norm: a tensor with its negation pending; resolve_neg() it")
     if weight is not None and (weight.shape != (cols,) or not (weight.dtype is torch.float32 or weight.dtype is dtype)
                                or not weight.is_contiguous()):
         raise MibcError(f"rms_norm: weight must be a contiguous [{cols}] tensor, f32 or {dtype}")
@@ -143,8 +172,9 @@ def rms_norm(x, weight=None, *, residual=None, alpha: float = 1.0, eps: float = 
         ss = _row_stride("rms_norm", "sum_out", sum_out, cols)
     try:
         args = _NORM_ARGS.pack(
-            x.data_ptr(), 0 if residual is None else residual.data_ptr(), 0 if weight is None else weight.data_ptr(),
-            0 if sum_out is None else sum_out.data_ptr(), out.data_ptr(), 0 if scale is None else scale.data_ptr(), x.numel() // cols,
+            x.data_ptr(), 0 if residual is None else residual.data_ptr() or _ptr("rms_norm", residual),
+            0 if weight is None else weight.data_ptr() or _ptr("rms_norm", weight),
+            0 if sum_out is None else sum_out.data_ptr() or _ptr("rms_norm", sum_out), out.data_ptr(), 0 if scale is None else scale.data_ptr(), x.numel() // cols,
             xs, rs, ss, os_, groups, cols, _TYPE[dtype], _TYPE[dtype if weight is None else weight.dtype], _TYPE[out_dtype], group, alpha, eps, 0)
     except _BAD_FIELD as e:
         raise MibcError(f"rms_norm: {e}") from None
@@ -195,7 +225,7 @@ def rope(q, k=None, *, freqs, positions=None, start: int = 0, interleaved: bool 
                 raise MibcError(f"rope: positions must be [{b}, {t}] or [{t}]")
             positions = positions.expand(b, t)
         positions = positions.contiguous()
-        where = positions.data_ptr()
+        where = _ptr("rope", positions)
     if out is None:
         qo, ko = _new(q), None if k is None else _new(k)
     else:
@@ -271,7 +301,7 @@ def attention(q, k, v, *, scale=None, causal: bool = False, window=(-1, -1), sof
     if slopes is not None:
         if slopes.dtype is not torch.float32 or slopes.shape != (h,) or not slopes.is_contiguous():
             raise MibcError(f"attention: slopes must be a contiguous f32 tensor [{h}]")
-        slope = slopes.data_ptr()
+        slope = _ptr("attention", slopes)
     if doc_offsets is not None:
         docs = doc_offsets.shape[0] - 1 if doc_offsets.dim() == 1 else -1
         if docs < 0:

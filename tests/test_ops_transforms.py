@@ -1,0 +1,94 @@
+"""Transformer-layer operators under torch's transformations: what would pass the work by is refused, what does not concern it is not."""
+import pytest
+import torch
+import torch.autograd.forward_ad as fwd
+from torch.fx.experimental.proxy_tensor import make_fx
+
+from dorado_amd import capi, ops
+
+FREQS = torch.ones(32, dtype=torch.float64)
+
+
+def calls(device):
+    """(name, f): f of one [1, 4, 2, 64] tensor, each operand in turn."""
+    def x():
+        return torch.ones((1, 4, 2, 64), dtype=torch.float16, device=device)
+    f = FREQS.to(device)
+    return [("x", lambda t: ops.rms_norm(t)), ("residual", lambda t: ops.rms_norm(x(), residual=t)),
+            ("weight", lambda t: ops.rms_norm(x(), t[0, 0, 0])), ("q", lambda t: ops.rope(t, freqs=f)), ("k", lambda t: ops.rope(x(), t, freqs=f)[1]),
+            ("query", lambda t: ops.attention(t, x(), x())), ("key", lambda t: ops.attention(x(), t, x())), ("value", lambda t: ops.attention(x(), x(), t))]
+
+
+NAMES = [n for n, _ in calls("cpu")]
+
+
+@pytest.mark.parametrize("name", NAMES)
+def test_tangents_are_refused(name):
+    f, x = dict(calls("cpu"))[name], torch.ones((1, 4, 2, 64), dtype=torch.float16)
+    with fwd.dual_level(), pytest.raises(capi.MibcNotSupported, match="tangents"):
+        f(fwd.make_dual(x, x))
+    with fwd.dual_level(), pytest.raises(capi.MibcError, match="no CPU form"):       # a tensor without one is as any other
+        f(x)
+
+
+@pytest.mark.parametrize("name", NAMES)
+def test_tracing_is_refused(name):
+    f, x = dict(calls("cpu"))[name], torch.ones((1, 4, 2, 64), dtype=torch.float16)
+    with pytest.raises(capi.MibcNotSupported, match="traced"):
+        torch.jit.trace(f, (x,))
+    for mode in ("real", "fake", "symbolic"):
+        with pytest.raises(capi.MibcNotSupported, match="traced"):
+            make_fx(f, tracing_mode=mode)(x)
+
+
+def test_counters_may_watch():
+    from torch.utils.flop_counter import FlopCounterMode
+    with FlopCounterMode(display=False), pytest.raises(capi.MibcError, match="no CPU form"):
+        ops.rms_norm(torch.ones((2, 64), dtype=torch.float16))
+
+
+gpu = pytest.mark.gpu
+
+
+@gpu
+@pytest.mark.parametrize("name", NAMES)
+def test_transformations_of_device_tensors_are_refused(name):
+    f, x = dict(calls("cuda"))[name], torch.ones((1, 4, 2, 64), dtype=torch.float16, device="cuda")
+    refused = (capi.MibcError, capi.MibcNotSupported, RuntimeError)
+    with fwd.dual_level(), pytest.raises(capi.MibcNotSupported, match="tangents"):
+        f(fwd.make_dual(x, x))
+    with pytest.raises(capi.MibcNotSupported, match="traced"):
+        torch.jit.trace(f, (x,))
+    with pytest.raises(capi.MibcNotSupported, match="traced"):
+        make_fx(f)(x)
+    for transform in (lambda: torch.func.functionalize(f)(x), lambda: torch.vmap(f)(x[None]), lambda: torch.func.jvp(f, (x,), (x,)),
+                      lambda: torch.func.grad(lambda y: f(y).float().sum())(x)):
+        with pytest.raises(refused):
+            transform()
+    if name in ("residual", "value"):
+        with pytest.raises(refused):
+            f(torch._efficientzerotensor((1, 4, 2, 64), dtype=torch.float16, device="cuda"))
+
+
+@gpu
+def test_a_pending_negation_is_refused():
+    z = torch.complex(torch.ones(3, 1), torch.full((3, 1), 2.0)).cuda()
+    im = z.conj().imag
+    assert im.is_neg()
+    with pytest.raises(capi.MibcNotSupported, match="negation"):
+        ops.rms_norm(im)
+    y = ops.rms_norm(im.resolve_neg().clone(), eps=0.0)
+    assert (y == -1).all()
+
+
+@gpu
+@pytest.mark.filterwarnings("ignore")
+def test_compiled_callers_get_the_same_results():
+    x, f = torch.rand((1, 4, 2, 64), device="cuda").half(), FREQS.cuda()
+
+    def layer(t):
+        y = ops.rms_norm(t * 2)
+        q, k = ops.rope(y, y + 1, freqs=f)
+        return ops.attention(q, k, y) + 1
+
+    assert torch.equal(torch.compile(layer, backend="eager")(x), layer(x))
