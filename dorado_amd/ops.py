@@ -5,7 +5,8 @@ Tensors live on one HIP device; the work goes to torch's current stream of that 
 outputs and the workspace of a split attention come from torch's caching allocator, so a call can be captured into a graph.
 There is no CPU form: a tensor elsewhere raises.  Forward only; no autograd graph is recorded, so inputs that require a
 gradient are refused while gradients are being recorded, and so are forward-mode tangents, tracing (torch.jit.trace, make_fx) and
-tensors without memory of their own (fake, functional, symbolic zeros): all of these would pass the work by."""
+tensors without memory of their own (fake, functional, symbolic zeros): all of these would pass the work by.  A tensor given as
+out= has its version raised, as by any operation in place."""
 from __future__ import annotations
 
 import ctypes as C
@@ -95,6 +96,12 @@ def _ptr(what: str, t) -> int:
     return p
 
 
+def _written(t) -> None:
+    """Raises the version of a tensor that the caller handed in to be written."""
+    if not t.is_inference():
+        torch.autograd.graph.increment_version(t)
+
+
 def _row_stride(what: str, name: str, t: torch.Tensor, cols: int) -> int:
     """Elements from row to row of `t` seen as rows of `cols`."""
     st = t.stride()
@@ -155,6 +162,7 @@ def rms_norm(x, weight=None, *, residual=None, alpha: float = 1.0, eps: float = 
         scale = torch.empty(shape[:-1] + (groups,), dtype=torch.float32, device=x.device)
     xs = cols if x.is_contiguous() else _row_stride("rms_norm", "x", x, cols)
     rs = ss = os_ = cols
+    out_given, sum_given = out is not None, sum_out is not None
     if residual is not None and not residual.is_contiguous():
         rs = _row_stride("rms_norm", "residual", residual, cols)
     if out is None:
@@ -181,6 +189,10 @@ def rms_norm(x, weight=None, *, residual=None, alpha: float = 1.0, eps: float = 
     rc = (_fns or _entry())[0](dev, _stream(dev), args)
     if rc:
         _check(rc, "rms_norm")
+    if out_given:
+        _written(out)
+    if sum_given:
+        _written(sum_out)
     if scale is None:
         return out if sum_out is None else (out, sum_out)
     return (out, scale) if sum_out is None else (out, scale, sum_out)
@@ -258,6 +270,10 @@ def rope(q, k=None, *, freqs, positions=None, start: int = 0, interleaved: bool 
     rc = (_fns or _entry())[1](dev, _stream(dev), args)
     if rc:
         _check(rc, "rope")
+    if out is not None:
+        _written(qo)
+        if k is not None:
+            _written(ko)
     return qo if k is None else (qo, ko)
 
 
@@ -290,6 +306,7 @@ def attention(q, k, v, *, scale=None, causal: bool = False, window=(-1, -1), sof
             raise MibcError("attention: causal is window (-1, 0); give one of the two")
         ahead = 0
     back, ahead = max(-1, min(int(back), 0x7fffffff)), max(-1, min(int(ahead), 0x7fffffff))
+    out_given = out is not None
     if out is None:
         out = _new(q)
     elif out.shape != shape or out.dtype is not dtype:
@@ -331,4 +348,6 @@ def attention(q, k, v, *, scale=None, causal: bool = False, window=(-1, -1), sof
     rc = run(dev, _stream(dev), args)
     if rc:
         _check(rc, "attention")
+    if out_given:
+        _written(out)
     return out if lse is None else (out, lse)

@@ -82,6 +82,25 @@ def test_a_pending_negation_is_refused():
 
 
 @gpu
+@pytest.mark.parametrize("which", ["norm", "sum", "rope", "keys", "attention"])
+def test_written_tensors_get_a_new_version(which):
+    # a tensor that a backward pass still needs is overwritten: autograd has to notice
+    x, f = torch.rand((1, 4, 2, 64), device="cuda").half() + 0.5, FREQS.cuda()
+    a = torch.rand_like(x).requires_grad_()
+    y = (a * x).sum()                     # keeps x
+    before = x._version
+    with torch.no_grad():
+        {"norm": lambda: ops.rms_norm(x, out=x), "sum": lambda: ops.rms_norm(x.clone(), sum_out=x), "rope": lambda: ops.rope(x, freqs=f, out=x),
+         "keys": lambda: ops.rope(x.clone(), x, freqs=f, out=(torch.empty_like(x), x)), "attention": lambda: ops.attention(x, x.clone(), x.clone(), out=x)}[which]()
+    assert x._version > before
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.backward()
+    with torch.inference_mode():          # tensors without versions stay usable
+        z = torch.ones((2, 64), dtype=torch.float16, device="cuda")
+        ops.rms_norm(z, out=z)
+
+
+@gpu
 @pytest.mark.filterwarnings("ignore")
 def test_compiled_callers_get_the_same_results():
     x, f = torch.rand((1, 4, 2, 64), device="cuda").half(), FREQS.cuda()
