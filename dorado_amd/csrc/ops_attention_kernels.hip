@@ -38,7 +38,8 @@ struct AttType<bf16_t> {
 
 // 16 bytes per lane from base + offset straight to LDS at `lds_addr` + 16 * lane (one wait state between M0 and its use).  Written
 // as assembly, because the compiler waits for every LDS load of its own before any LDS read, and the next tile's are meant to
-// stay in flight: the kernels wait for them by vmcnt.  The load writes no register.
+// stay in flight: the kernels wait for them by vmcnt.  The load writes no register.  M0 is one the compiler never allocates (it takes no
+// clobber of it either) and needs for nothing else here: a test looks at the assembly for that.
 __device__ __forceinline__ void att_dma16(att_gptr base, unsigned offset, unsigned lds_addr) {
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(lds_addr), "v"(offset), "s"(base) : "memory");
 }
