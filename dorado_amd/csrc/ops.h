@@ -38,6 +38,55 @@ static inline int op_hip(hipError_t rc, const char *what) {
     return MIBC_ERR_HIP;
 }
 
+// The memory of an operand: runs of bytes at base + sum i_d stride_d, i_d < size_d.  A stride of 0 is a broadcast dimension.
+struct OpSpan {
+    uintptr_t base, end;      // equal where there is nothing
+    int64_t run, size[3], stride[3];
+};
+static inline OpSpan op_span(const void *base, int64_t run, int64_t n0 = 1, int64_t s0 = 0, int64_t n1 = 1, int64_t s1 = 0, int64_t n2 = 1, int64_t s2 = 0) {
+    OpSpan s = {(uintptr_t)base, (uintptr_t)base, run, {n0, n1, n2}, {s0, s1, s2}};
+    if (base == nullptr || n0 == 0 || n1 == 0 || n2 == 0) return s;
+    // no operand reaches beyond 2^63 bytes
+    s.end += run + (n0 > 1 ? (n0 - 1) * s0 : 0) + (n1 > 1 ? (n1 - 1) * s1 : 0) + (n2 > 1 ? (n2 - 1) * s2 : 0);
+    return s;
+}
+static inline bool op_same(const OpSpan &a, const OpSpan &b) {
+    bool same = a.base == b.base && a.run == b.run;
+    for (int d = 0; d < 3; ++d) same = same && a.size[d] == b.size[d] && (a.size[d] <= 1 || a.stride[d] == b.stride[d]);
+    return same;
+}
+// Whether two operands share no byte.  Either their ends show it, or the strides from some size on are all multiples of an M, and what
+// the smaller strides reach of each lies apart within M (columns of one packed buffer, heads or rows dealt to two tensors).  False for
+// what neither shows
+static inline bool op_apart(const OpSpan &a, const OpSpan &b) {
+    if (a.end <= b.base || b.end <= a.base || a.end == a.base || b.end == b.base) return true;
+    const OpSpan *const both[2] = {&a, &b};
+    auto reach = [](const OpSpan &s, int64_t below) {     // bytes from the base to the end, strides below that limit only
+        int64_t n = s.run;
+        for (int d = 0; d < 3; ++d)
+            if (s.stride[d] < below && s.size[d] > 1) n += (s.size[d] - 1) * s.stride[d];
+        return n;
+    };
+    const int64_t from = (int64_t)(b.base - a.base);
+    for (const OpSpan *s : both)
+        for (int d = 0; d < 3; ++d) {
+            const int64_t least = s->stride[d];
+            if (s->size[d] <= 1 || least == 0) continue;
+            int64_t m = 0;
+            for (const OpSpan *t : both)
+                for (int e = 0; e < 3; ++e)
+                    if (t->size[e] > 1 && t->stride[e] >= least)
+                        for (int64_t x = t->stride[e]; x != 0;) {
+                            const int64_t rest = m % x;
+                            m = x;
+                            x = rest;
+                        }
+            const int64_t off = (from % m + m) % m;
+            if (off >= reach(a, least) && off <= m - reach(b, least)) return true;
+        }
+    return false;
+}
+
 static inline int op_type_bytes(int type) { return type == MIBC_TYPE_F32 ? 4 : (type == MIBC_TYPE_I8 || type == MIBC_TYPE_E4M3) ? 1 : 2; }
 static inline bool op_aligned(const void *p, unsigned bytes) { return ((uintptr_t)p & (bytes - 1)) == 0; }
 

@@ -102,14 +102,26 @@ static uint64_t att_room(const mibc_attention_args &a, const AttPlan &p) {
     return p.splits == 1 ? 0 : (uint64_t)a.batch * a.heads * a.q_tokens * p.splits * (a.head_dim + 1) * 4;
 }
 static int att_check_plan(const mibc_attention_args &a, const AttPlan &p) {
-    // a workgroup writes its rows while others still read keys and values
-    if (a.k_tokens > 0 && (a.out == a.k || a.out == a.v)) return op_refuse(MIBC_ERR_ARG, "attention: out may be q, but not k or v");
     if ((int64_t)a.batch * a.kv_heads * p.tiles * p.splits > 0x7fffffff) return op_refuse(MIBC_NOT_SUPPORTED, "attention: too many row tiles");
     const uint64_t need = att_room(a, p);
-    if (need == 0) return MIBC_OK;
-    if (a.workspace == nullptr || a.workspace_bytes < need)
+    if (need != 0 && (a.workspace == nullptr || a.workspace_bytes < need))
         return op_refuse(MIBC_ERR_ARG, "attention: workspace smaller than mibc_attention_workspace says");
-    if (!op_aligned(a.workspace, 16)) return op_refuse(MIBC_ERR_ARG, "attention: workspace must be aligned to 16 bytes");
+    if (need != 0 && !op_aligned(a.workspace, 16)) return op_refuse(MIBC_ERR_ARG, "attention: workspace must be aligned to 16 bytes");
+    // a workgroup writes its rows while others still read
+    auto span = [&](const void *x, int64_t tokens, int64_t heads, const int64_t *s) {
+        return op_span(x, a.head_dim * 2, a.batch, s[0] * 2, tokens, s[1] * 2, heads, s[2] * 2);
+    };
+    const OpSpan q = span(a.q, a.q_tokens, a.heads, a.q_stride), k = span(a.k, a.k_tokens, a.kv_heads, a.k_stride),
+                 v = span(a.v, a.k_tokens, a.kv_heads, a.v_stride), out = span(a.out, a.q_tokens, a.heads, a.out_stride);
+    if (!op_apart(out, k) || !op_apart(out, v) || (!op_same(out, q) && !op_apart(out, q)))
+        return op_refuse(MIBC_ERR_ARG, "attention: out may be q, but not k or v, nor overlap any of them otherwise");
+    const OpSpan lse = op_span(a.lse, (int64_t)a.batch * a.heads * a.q_tokens * 4), room = op_span(need ? a.workspace : nullptr, (int64_t)need);
+    const OpSpan small[4] = {op_span(a.k_len, (int64_t)a.batch * 4), op_span(a.prefix, (int64_t)(a.doc_offsets ? a.n_docs : a.batch) * 4),
+                             op_span(a.doc_offsets, ((int64_t)a.n_docs + 1) * 4), op_span(a.slopes, (int64_t)a.heads * 4)};
+    bool fine = op_apart(out, lse) && op_apart(out, room) && op_apart(lse, room);
+    for (const OpSpan *x : {&q, &k, &v, &small[0], &small[1], &small[2], &small[3]}) fine = fine && op_apart(lse, *x) && op_apart(room, *x);
+    for (const OpSpan &x : small) fine = fine && op_apart(out, x);
+    if (!fine) return op_refuse(MIBC_ERR_ARG, "attention: out, lse and workspace may not overlap another operand");
     return MIBC_OK;
 }
 
@@ -118,14 +130,7 @@ extern "C" uint64_t mibc_attention_workspace(const mibc_attention_args *a) {
     return att_room(*a, att_plan(*a));
 }
 
-// launch on a stream of the current device (the engine's own path); checks included.  whole: the keys are not split, so there is
-// no workspace (the engine's batches fill the device)
-int mibc_launch_attention(hipStream_t s, const mibc_attention_args &a, bool whole) {
-    if (const int rc = att_check(a)) return rc;
-    if (a.batch == 0 || a.q_tokens == 0) return MIBC_OK;
-    AttPlan plan = att_plan(a);
-    if (whole) plan.splits = 1;
-    if (const int rc = att_check_plan(a, plan)) return rc;
+static int att_run(hipStream_t s, const mibc_attention_args &a, const AttPlan &plan) {
     AttArgs p{};
     p.a = a;
     p.group = a.heads / a.kv_heads;
@@ -169,12 +174,24 @@ int mibc_launch_attention(hipStream_t s, const mibc_attention_args &a, bool whol
     }
 }
 
+// launch on a stream of the current device (the engine's own path); checks included.  whole: the keys are not split, so there is
+// no workspace (the engine's batches fill the device)
+int mibc_launch_attention(hipStream_t s, const mibc_attention_args &a, bool whole) {
+    if (const int rc = att_check(a)) return rc;
+    if (a.batch == 0 || a.q_tokens == 0) return MIBC_OK;
+    AttPlan plan = att_plan(a);
+    if (whole) plan.splits = 1;
+    if (const int rc = att_check_plan(a, plan)) return rc;
+    return att_run(s, a, plan);
+}
+
 extern "C" int mibc_attention(int device, void *stream, const mibc_attention_args *a) {
     if (a == nullptr) return op_refuse(MIBC_ERR_ARG, "attention: null arguments");
     if (const int rc = att_check(*a)) return rc;
     if (a->batch == 0 || a->q_tokens == 0) return MIBC_OK;
-    if (const int rc = att_check_plan(*a, att_plan(*a))) return rc;
+    const AttPlan plan = att_plan(*a);
+    if (const int rc = att_check_plan(*a, plan)) return rc;
     OpDevice d(device);
     if (d.rc != hipSuccess) return op_hip(d.rc, "attention: device");
-    return mibc_launch_attention((hipStream_t)stream, *a, false);
+    return att_run((hipStream_t)stream, *a, plan);
 }

@@ -274,6 +274,14 @@ static int norm_check(const mibc_rms_norm_args &a, bool *vec) {
     if (!op_aligned(a.x, eb) || !op_aligned(a.residual, eb) || !op_aligned(a.sum_out, eb) || !op_aligned(a.weight, (unsigned)op_type_bytes(a.weight_type)) ||
         !op_aligned(a.out, (unsigned)op_type_bytes(a.out_type)) || !op_aligned(a.scale_out, 4))
         return op_refuse(MIBC_ERR_ARG, "rms_norm: pointer not aligned to its type");
+    const int64_t wide = (int64_t)a.cols * eb, ob = op_type_bytes(a.out_type);
+    const OpSpan x = op_span(a.x, wide, a.rows, a.x_stride * eb), r = op_span(a.residual, wide, a.rows, a.residual_stride * eb),
+                 w = op_span(a.weight, (int64_t)a.cols * op_type_bytes(a.weight_type)), sum = op_span(a.sum_out, wide, a.rows, a.sum_stride * eb),
+                 out = op_span(a.out, a.cols * ob, a.rows, a.out_stride * ob), sc = op_span(a.scale_out, ngroups * 4, quant ? a.rows : 0, a.scale_stride * 4);
+    auto in_place = [&](const OpSpan &o) { return (op_same(o, x) || op_apart(o, x)) && (op_same(o, r) || op_apart(o, r)) && op_apart(o, w); };
+    if (!in_place(sum) || !in_place(out) || !op_apart(sum, out) || !op_apart(sc, x) || !op_apart(sc, r) || !op_apart(sc, w) || !op_apart(sc, sum) ||
+        !op_apart(sc, out))
+        return op_refuse(MIBC_ERR_ARG, "rms_norm: an output may be x or residual, but not overlap them, the weight or another output otherwise");
     // aligned 16-byte accesses where every row of every tensor allows them, unaligned ones and single elements at a row's end elsewhere
     *vec = a.cols % 8 == 0 && op_aligned(a.x, 16) && a.x_stride % 8 == 0 && op_aligned(a.weight, 16) &&
            (a.residual == nullptr || (op_aligned(a.residual, 16) && a.residual_stride % 8 == 0)) &&
@@ -282,11 +290,7 @@ static int norm_check(const mibc_rms_norm_args &a, bool *vec) {
     return MIBC_OK;
 }
 
-// launch on a stream of the current device (the engine's own path); checks included
-int mibc_launch_rms_norm(hipStream_t s, const mibc_rms_norm_args &a) {
-    bool vec = false;
-    if (const int rc = norm_check(a, &vec)) return rc;
-    if (a.rows == 0) return MIBC_OK;
+static int norm_run(hipStream_t s, const mibc_rms_norm_args &a, bool vec) {
     const NormArgs n{a};
 #define NORM_T(T)                              \
     do {                                       \
@@ -300,12 +304,19 @@ int mibc_launch_rms_norm(hipStream_t s, const mibc_rms_norm_args &a) {
     return op_hip(hipGetLastError(), "rms_norm");
 }
 
+// launch on a stream of the current device (the engine's own path); checks included
+int mibc_launch_rms_norm(hipStream_t s, const mibc_rms_norm_args &a) {
+    bool vec = false;
+    if (const int rc = norm_check(a, &vec)) return rc;
+    return a.rows == 0 ? MIBC_OK : norm_run(s, a, vec);
+}
+
 extern "C" int mibc_rms_norm(int device, void *stream, const mibc_rms_norm_args *a) {
     if (a == nullptr) return op_refuse(MIBC_ERR_ARG, "rms_norm: null arguments");
-    bool vec;
+    bool vec = false;
     if (const int rc = norm_check(*a, &vec)) return rc;
     if (a->rows == 0) return MIBC_OK;
     OpDevice d(device);
     if (d.rc != hipSuccess) return op_hip(d.rc, "rms_norm: device");
-    return mibc_launch_rms_norm((hipStream_t)stream, *a);
+    return norm_run((hipStream_t)stream, *a, vec);
 }

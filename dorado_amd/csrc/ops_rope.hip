@@ -181,6 +181,16 @@ static int rope_check(const mibc_rope_args &a, bool *vec) {
         }
         if (!op_aligned(a.x[w], 16) || !op_aligned(a.out[w], 16)) *vec = false;
     }
+    auto span = [&](const void *p, int w, const int64_t *s) {
+        return op_span(p, (int64_t)a.head_dim * eb, a.batch, s[0] * eb, a.tokens, s[1] * eb, a.heads[w], s[2] * eb);
+    };
+    const OpSpan x[2] = {span(a.x[0], 0, a.x_stride[0]), span(a.x[1], 1, a.x_stride[1])};
+    const OpSpan out[2] = {span(a.out[0], 0, a.out_stride[0]), span(a.heads[1] ? a.out[1] : nullptr, 1, a.out_stride[1])};
+    const OpSpan p = op_span(a.positions, a.batch * a.tokens * (a.positions_64 ? 8 : 4)), f = op_span(a.freqs, (int64_t)a.rot_dim * 4);
+    bool fine = op_apart(out[0], out[1]);
+    for (int w = 0; w < 2; ++w)
+        fine = fine && (op_same(out[w], x[w]) || op_apart(out[w], x[w])) && op_apart(out[w], x[1 - w]) && op_apart(out[w], p) && op_apart(out[w], f);
+    if (!fine) return op_refuse(MIBC_ERR_ARG, "rope: an output may be its input, but not overlap it, another operand or the other output otherwise");
     return MIBC_OK;
 }
 
@@ -213,11 +223,7 @@ static void rope_launch(hipStream_t s, RopeArgs &r, bool vec) {
     else hipLaunchKernelGGL((rope_kernel<T, false>), grid, dim3(256), 0, s, r);
 }
 
-// launch on a stream of the current device (the engine's own path); checks included
-int mibc_launch_rope(hipStream_t s, const mibc_rope_args &a) {
-    bool vec = false;
-    if (const int rc = rope_check(a, &vec)) return rc;
-    if (a.batch == 0 || a.tokens == 0) return MIBC_OK;
+static int rope_run(hipStream_t s, const mibc_rope_args &a, bool vec) {
     RopeArgs r{};
     r.a = a;
     r.total = a.batch * a.tokens;
@@ -227,14 +233,21 @@ int mibc_launch_rope(hipStream_t s, const mibc_rope_args &a) {
     return op_hip(hipGetLastError(), "rope");
 }
 
+// launch on a stream of the current device (the engine's own path); checks included
+int mibc_launch_rope(hipStream_t s, const mibc_rope_args &a) {
+    bool vec = false;
+    if (const int rc = rope_check(a, &vec)) return rc;
+    return a.batch == 0 || a.tokens == 0 ? MIBC_OK : rope_run(s, a, vec);
+}
+
 extern "C" int mibc_rope(int device, void *stream, const mibc_rope_args *a) {
     if (a == nullptr) return op_refuse(MIBC_ERR_ARG, "rope: null arguments");
-    bool vec;
+    bool vec = false;
     if (const int rc = rope_check(*a, &vec)) return rc;
     if (a->batch == 0 || a->tokens == 0) return MIBC_OK;
     OpDevice d(device);
     if (d.rc != hipSuccess) return op_hip(d.rc, "rope: device");
-    return mibc_launch_rope((hipStream_t)stream, *a);
+    return rope_run((hipStream_t)stream, *a, vec);
 }
 
 extern "C" int mibc_rope_frequencies(int scaling, int rot_dim, double theta, double factor, double original_length, double turns_low,

@@ -242,8 +242,8 @@ MIBC_API int mibc_svb16_decode(mibc_engine *e, const uint8_t *streams_dev, const
  * synchronises or keeps anything for the next one, so all of them can be captured into a graph; the caller's current device is
  * left as it was.  Refusals are decided from the arguments alone, before anything is launched (text: mibc_last_error(NULL)).
  * Strides count elements; the innermost dimension is contiguous.  A stride may be 0 on inputs (a broadcast dimension), never
- * on outputs.  An output may be x, residual or q where shape and strides are the same (in place), never k or v of an attention;
- * other overlaps are not checked. */
+ * on outputs.  An output may be x, residual or q where type, shape and strides are the same (in place); an output that shares memory with
+ * another operand in any other way is refused. */
 #define MIBC_TYPE_F16 0
 #define MIBC_TYPE_BF16 1
 #define MIBC_TYPE_F32 2
