@@ -191,3 +191,27 @@ def test_infinities_beside_values_near_the_end(n, m):
     want = reference(q, k, torch.full_like(v, 3.3e38))
     rest = [c for c in range(64) if c not in (5, 6, 7)]
     R.close(out[..., rest], want[0][..., rest], want[2][..., rest], "other columns")
+
+
+# ------------------------------------------------------------------------------------------------------- scores of -infinity
+@pytest.mark.parametrize("n,m", PATHS + [(1, 9000), (40, 9000)])
+@pytest.mark.parametrize("slopes", [False, True])
+@pytest.mark.parametrize("t,d", [(F16, 64), (BF16, 128)])
+def test_only_scores_of_minus_infinity(t, d, slopes, n, m):
+    q, k, v = rnd((1, n, 2, d), t, 24).abs() + 0.1, rnd((1, m, 1, d), t, 25), rnd((1, m, 1, d), t, 26)
+    low = torch.full_like(k, -math.inf)
+    kw = dict(slopes=torch.tensor([0.5, 0.01], device="cuda")) if slopes else {}
+    out, lse = ops.attention(q, low, v, return_lse=True, **kw)
+    assert (out == 0).all() and (lse == -math.inf).all()
+    # the first keys only: rows that see no other give zeros, the others what they would without those keys
+    first = m - n // 2 - 1
+    low[:, first:] = k[:, first:]
+    out, lse = ops.attention(q, low, v, causal=True, return_lse=True, **kw)
+    blind = first - (m - n)          # rows 0 .. blind - 1 stand before key `first`
+    assert blind >= 0 and (out[:, :blind] == 0).all() and (lse[:, :, :blind] == -math.inf).all()
+    want, wlse = ops.attention(q[:, blind:], k[:, first:], v[:, first:], causal=True, return_lse=True, **kw)
+    bound = reference(q[:, blind:], k[:, first:], v[:, first:], causal=True, slopes=kw["slopes"].cpu() if slopes else None)
+    R.close(out[:, blind:], bound[0], bound[2], "out")
+    R.close(lse[:, :, blind:], bound[1], bound[3], "lse")
+    R.close(want, bound[0], bound[2], "alone")
+    R.close(wlse, bound[1], bound[3], "lse alone")
