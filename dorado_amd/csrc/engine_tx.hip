@@ -189,7 +189,7 @@ size_t tx_bytes_per_chunk(const mibc_engine *e, int T_in) {
         }
     }
     const size_t R = (size_t)T;
-    b += R * (tx.D /* x */ + 3 * tx.D /* qkv */ + tx.D /* vT */ + tx.D /* attn */ + tx.D /* tmp */ + tx.FF + tx.sf * tx.D) * 2;   // == tx_reserve
+    b += R * (tx.D /* x */ + 3 * tx.D /* qkv */ + (tx.by_ops ? 0 : tx.D) /* vT */ + tx.D /* attn */ + tx.D /* tmp */ + tx.FF + tx.sf * tx.D) * 2;   // == tx_reserve
     b += 3 * R * tx.sf;
     return b;
 }
@@ -219,7 +219,7 @@ int tx_reserve(mibc_engine *e, int N_max, int T_in, size_t *total_out) {
     const size_t R = N * (size_t)T;
     if (alloc(&tx.x, R * tx.D)) return MIBC_ERR_MEM;
     if (alloc(&tx.qkv, R * 3 * tx.D)) return MIBC_ERR_MEM;
-    if (alloc(&tx.vT, R * tx.D)) return MIBC_ERR_MEM;      // used when the call's token count is a multiple of 128
+    if (!tx.by_ops && alloc(&tx.vT, R * tx.D)) return MIBC_ERR_MEM;      // used when the call's token count is a multiple of 128
     if (alloc(&tx.attn, R * tx.D)) return MIBC_ERR_MEM;
     if (alloc(&tx.tmp, R * tx.D)) return MIBC_ERR_MEM;
     if (alloc(&tx.ff, R * tx.FF)) return MIBC_ERR_MEM;

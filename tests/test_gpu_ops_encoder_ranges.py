@@ -62,3 +62,15 @@ def test_wide_encoders_vs_oracle(d_model, nhead, ff, depth, n, t_in):
     for a, b in zip(got, want):
         assert a[0] == b[0] and (a[2] == b[2]).all()
     eng.close()
+
+
+def test_operators_need_no_transposed_values():
+    # the same width with heads of 64 (window kernels, which read V transposed) and of 32 (the operators, which read it as it lies)
+    need = []
+    for nhead in (4, 8):
+        cfg = config.tiny_tx(256, nhead)
+        eng = capi.Engine(cfg, synth.make_weights(cfg, seed=77))
+        need.append(eng.query_memory(1536)[0])
+        tokens = eng.output_steps(1536) // cfg.tx.up_scale_factor
+        eng.close()
+    assert need[0] - need[1] == tokens * 256 * 2
