@@ -55,6 +55,17 @@ static inline bool op_same(const OpSpan &a, const OpSpan &b) {
     for (int d = 0; d < 3; ++d) same = same && a.size[d] == b.size[d] && (a.size[d] <= 1 || a.stride[d] == b.stride[d]);
     return same;
 }
+// Whether no byte of an output is written twice: every stride steps over all that the smaller ones reach, as in any view of a dense buffer.
+static inline bool op_plain(const OpSpan &s) {
+    for (int d = 0; d < 3; ++d) {
+        if (s.size[d] <= 1) continue;
+        int64_t n = s.run;
+        for (int e = 0; e < 3; ++e)
+            if (e != d && s.size[e] > 1 && (s.stride[e] < s.stride[d] || (s.stride[e] == s.stride[d] && e > d))) n += (s.size[e] - 1) * s.stride[e];
+        if (s.stride[d] < n) return false;
+    }
+    return true;
+}
 // Whether two operands share no byte.  Either their ends show it, or the strides from some size on are all multiples of an M, and what
 // the smaller strides reach of each lies apart within M (columns of one packed buffer, heads or rows dealt to two tensors).  False for
 // what neither shows

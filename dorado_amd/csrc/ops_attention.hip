@@ -113,6 +113,7 @@ static int att_check_plan(const mibc_attention_args &a, const AttPlan &p) {
     };
     const OpSpan q = span(a.q, a.q_tokens, a.heads, a.q_stride), k = span(a.k, a.k_tokens, a.kv_heads, a.k_stride),
                  v = span(a.v, a.k_tokens, a.kv_heads, a.v_stride), out = span(a.out, a.q_tokens, a.heads, a.out_stride);
+    if (!op_plain(out)) return op_refuse(MIBC_ERR_ARG, "attention: output heads overlap");
     if (!op_apart(out, k) || !op_apart(out, v) || (!op_same(out, q) && !op_apart(out, q)))
         return op_refuse(MIBC_ERR_ARG, "attention: out may be q, but not k or v, nor overlap any of them otherwise");
     const OpSpan lse = op_span(a.lse, (int64_t)a.batch * a.heads * a.q_tokens * 4), room = op_span(need ? a.workspace : nullptr, (int64_t)need);

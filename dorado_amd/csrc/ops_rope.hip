@@ -187,6 +187,7 @@ static int rope_check(const mibc_rope_args &a, bool *vec) {
     const OpSpan x[2] = {span(a.x[0], 0, a.x_stride[0]), span(a.x[1], 1, a.x_stride[1])};
     const OpSpan out[2] = {span(a.out[0], 0, a.out_stride[0]), span(a.heads[1] ? a.out[1] : nullptr, 1, a.out_stride[1])};
     const OpSpan p = op_span(a.positions, a.batch * a.tokens * (a.positions_64 ? 8 : 4)), f = op_span(a.freqs, (int64_t)a.rot_dim * 4);
+    if (!op_plain(out[0]) || (a.heads[1] && !op_plain(out[1]))) return op_refuse(MIBC_ERR_ARG, "rope: output heads overlap");
     bool fine = op_apart(out[0], out[1]);
     for (int w = 0; w < 2; ++w)
         fine = fine && (op_same(out[w], x[w]) || op_apart(out[w], x[w])) && op_apart(out[w], x[1 - w]) && op_apart(out[w], p) && op_apart(out[w], f);

@@ -139,3 +139,33 @@ def test_attention_overlaps(change, refused):
     wide = (8192, 1024, 64)
     base = {**ATTN, "q": N, "k": N + 512, "v": N + 1024, "out": N, "q_stride": wide, "k_stride": wide, "v_stride": wide, "out_stride": wide}
     assert (on_no_device(2, base, **change) is not None) == refused
+
+
+def test_outputs_that_overlap_themselves_are_refused():
+    # strides of at least a head each, as the sizes allow: refused wherever two of the output's heads share a byte, views of one buffer not
+    r = random.Random(2)
+    bad = good = 0
+    for _ in range(3000):
+        b, n, h, d = r.randint(1, 3), r.randint(1, 4), r.randint(1, 4), 2
+        if r.random() < 0.5:
+            dense = [(r.randint(m, m + 2), i) for i, m in enumerate((b, n, h))]
+            r.shuffle(dense)
+            strides, step = [0, 0, 0], d + 2 * r.randint(0, 1)
+            for m, i in dense:
+                strides[i] = step
+                step *= m
+        else:
+            dense, strides = None, [2 * r.randint(1, 14) for _ in range(3)]
+        x = bytes_of(0, 4 * d, *[(m, 4 * s) for m, s in zip((b, n, h), strides)])
+        touch = x.size < 4 * d * b * n * h
+        said = on_no_device(1, ROPE, x0=1 << 28, out0=1 << 20, freqs=1 << 30, batch=b, tokens=n, h0=h, head_dim=d, rot_dim=d, type=2,
+                            xs=(n * h * d, h * d, d, 0, 0, 0), os=tuple(strides) + (0, 0, 0))
+        if touch:
+            bad += 1
+            assert said is not None, (b, n, h, strides)
+        elif dense is not None:
+            good += 1
+            assert said is None, (b, n, h, strides)
+    assert bad > 300 and good > 500
+    said = on_no_device(2, ATTN, q=1 << 28, k=1 << 29, v=1 << 30, out=1 << 20, out_stride=(1024, 64, 64))
+    assert said == "attention: output heads overlap"
