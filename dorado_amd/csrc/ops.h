@@ -37,6 +37,12 @@ static inline int op_hip(hipError_t rc, const char *what) {
     mibc_gerr() = std::string(what) + ": " + hipGetErrorString(rc);
     return MIBC_ERR_HIP;
 }
+// The launch's own status: the thread's last error may be an older one of the program's
+template <typename A>
+static inline hipError_t op_launch(void (*kernel)(A), dim3 grid, unsigned threads, unsigned lds, hipStream_t s, const A &args) {
+    void *list[1] = {(void *)&args};
+    return hipLaunchKernel((const void *)kernel, grid, dim3(threads), list, lds, s);
+}
 
 // The memory of an operand: runs of bytes at base + sum i_d stride_d, i_d < size_d.  A stride of 0 is a broadcast dimension.
 struct OpSpan {

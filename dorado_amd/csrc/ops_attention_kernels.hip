@@ -921,7 +921,7 @@ __global__ __launch_bounds__(256) void attention_join_kernel(AttArgs p) {
 }
 
 template <typename T, int CAP, bool SLOPES>
-static void att_one(hipStream_t s, const AttArgs &p, bool tokens) {
+static hipError_t att_one(hipStream_t s, const AttArgs &p, bool tokens) {
     // a launch holds less than 2^32 threads in x
     const unsigned x = p.groups < 1u << 20 ? p.groups : 1u << 20;
     const dim3 grid(x, (p.groups + x - 1) / x);
@@ -929,21 +929,20 @@ static void att_one(hipStream_t s, const AttArgs &p, bool tokens) {
 #define ATT_GO(KERNEL, LDS)                                                             \
     do {                                                                                \
         MIBC_LDS_ATTR_ONCE(KERNEL, LDS);                                                \
-        hipLaunchKernelGGL(KERNEL, grid, dim3(256), LDS, s, p);                         \
+        return op_launch(KERNEL, grid, 256, LDS, s, p);                                 \
     } while (0)
     if (tokens) ATT_GO((attention_token_kernel<T, ATT_D, CAP == ATT_NO_CAP ? ATT_NO_CAP : ATT_FAR, SLOPES>), TOKEN);
-    else ATT_GO((attention_kernel<T, ATT_D, CAP, SLOPES>), ROWS);
+    ATT_GO((attention_kernel<T, ATT_D, CAP, SLOPES>), ROWS);
 #undef ATT_GO
 }
 template <typename T>
 static int att_launch(hipStream_t s, const AttArgs &p, bool tokens) {
-    if (p.cap == ATT_FAR) p.a.slopes ? att_one<T, ATT_FAR, true>(s, p, tokens) : att_one<T, ATT_FAR, false>(s, p, tokens);
-    else if (p.cap == ATT_NEAR) p.a.slopes ? att_one<T, ATT_NEAR, true>(s, p, tokens) : att_one<T, ATT_NEAR, false>(s, p, tokens);
-    else p.a.slopes ? att_one<T, ATT_NO_CAP, true>(s, p, tokens) : att_one<T, ATT_NO_CAP, false>(s, p, tokens);
-    int rc = op_hip(hipGetLastError(), "attention");
-    if (rc != MIBC_OK || p.splits == 1) return rc;
-    hipLaunchKernelGGL((attention_join_kernel<T, ATT_D>), dim3((unsigned)((int64_t)p.pairs * p.rows)), dim3(256), 0, s, p);
-    return op_hip(hipGetLastError(), "attention");
+#define ATT_S(CAP) (p.a.slopes ? att_one<T, CAP, true>(s, p, tokens) : att_one<T, CAP, false>(s, p, tokens))
+    hipError_t rc = p.cap == ATT_FAR ? ATT_S(ATT_FAR) : p.cap == ATT_NEAR ? ATT_S(ATT_NEAR) : ATT_S(ATT_NO_CAP);
+#undef ATT_S
+    if (rc == hipSuccess && p.splits > 1)
+        rc = op_launch(attention_join_kernel<T, ATT_D>, dim3((unsigned)((int64_t)p.pairs * p.rows)), 256, 0, s, p);
+    return op_hip(rc, "attention");
 }
 #define ATT_CAT2(a, b) a##b
 #define ATT_CAT(a, b) ATT_CAT2(a, b)

@@ -221,26 +221,25 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void rms_norm_kernel(NormArg
 }
 
 template <typename T, bool VEC>
-static void norm_launch(hipStream_t s, const NormArgs &n) {
+static hipError_t norm_launch(hipStream_t s, const NormArgs &n) {
     const int chunks = (n.a.cols + 7) / 8;
     const int64_t rows = n.a.rows;
     // a launch holds less than 2^32 threads in x
 #define NORM_GO(TPR, NCH, NT)                                                                                        \
     do {                                                                                                             \
         const int64_t blocks = (rows + NT / TPR - 1) / (NT / TPR), x = blocks < 1 << 20 ? blocks : 1 << 20;          \
-        hipLaunchKernelGGL((rms_norm_kernel<T, TPR, NCH, VEC>), dim3((unsigned)x, (unsigned)((blocks + x - 1) / x)), \
-                           dim3(NT), 0, s, n);                                                                       \
+        return op_launch(rms_norm_kernel<T, TPR, NCH, VEC>, dim3((unsigned)x, (unsigned)((blocks + x - 1) / x)), NT, 0, s, n); \
     } while (0)
     if (chunks <= 4) NORM_GO(4, 1, 256);
-    else if (chunks <= 8) NORM_GO(8, 1, 256);
-    else if (chunks <= 16) NORM_GO(16, 1, 256);
-    else if (chunks <= 64) NORM_GO(64, 1, 256);
-    else if (chunks <= 128) NORM_GO(64, 2, 256);
-    else if (chunks <= 256) NORM_GO(64, 4, 256);
-    else if (chunks <= 512) NORM_GO(256, 2, 256);
-    else if (chunks <= 1024) NORM_GO(256, 4, 256);
-    else if (chunks <= 1536) NORM_GO(256, 6, 256);
-    else NORM_GO(1024, 4, 1024);
+    if (chunks <= 8) NORM_GO(8, 1, 256);
+    if (chunks <= 16) NORM_GO(16, 1, 256);
+    if (chunks <= 64) NORM_GO(64, 1, 256);
+    if (chunks <= 128) NORM_GO(64, 2, 256);
+    if (chunks <= 256) NORM_GO(64, 4, 256);
+    if (chunks <= 512) NORM_GO(256, 2, 256);
+    if (chunks <= 1024) NORM_GO(256, 4, 256);
+    if (chunks <= 1536) NORM_GO(256, 6, 256);
+    NORM_GO(1024, 4, 1024);
 #undef NORM_GO
 }
 
@@ -292,16 +291,9 @@ static int norm_check(const mibc_rms_norm_args &a, bool *vec) {
 
 static int norm_run(hipStream_t s, const mibc_rms_norm_args &a, bool vec) {
     const NormArgs n{a};
-#define NORM_T(T)                              \
-    do {                                       \
-        if (vec) norm_launch<T, true>(s, n);   \
-        else norm_launch<T, false>(s, n);      \
-    } while (0)
-    if (a.type == MIBC_TYPE_F16) NORM_T(half_t);
-    else if (a.type == MIBC_TYPE_BF16) NORM_T(bf16_t);
-    else NORM_T(float);
+#define NORM_T(T) (vec ? norm_launch<T, true>(s, n) : norm_launch<T, false>(s, n))
+    return op_hip(a.type == MIBC_TYPE_F16 ? NORM_T(half_t) : a.type == MIBC_TYPE_BF16 ? NORM_T(bf16_t) : NORM_T(float), "rms_norm");
 #undef NORM_T
-    return op_hip(hipGetLastError(), "rms_norm");
 }
 
 // launch on a stream of the current device (the engine's own path); checks included

@@ -196,15 +196,13 @@ static int rope_check(const mibc_rope_args &a, bool *vec) {
 }
 
 template <typename T>
-static void rope_launch(hipStream_t s, RopeArgs &r, bool vec) {
+static hipError_t rope_launch(hipStream_t s, RopeArgs &r, bool vec) {
     const mibc_rope_args &a = r.a;
     const int heads = a.heads[0] + a.heads[1];
     if (!vec) {
         const int64_t all = r.total * (a.rot_dim / 2 + a.head_dim - a.rot_dim);
         const int64_t blocks = (all + 255) / 256;
-        hipLaunchKernelGGL((rope_any_kernel<T>), dim3((unsigned)(blocks < 65536 ? blocks : 65536), (unsigned)((heads + ANY_HEADS - 1) / ANY_HEADS)),
-                           dim3(256), 0, s, r);
-        return;
+        return op_launch(rope_any_kernel<T>, dim3((unsigned)(blocks < 65536 ? blocks : 65536), (unsigned)((heads + ANY_HEADS - 1) / ANY_HEADS)), 256, 0, s, r);
     }
     bool inplace = true;
     for (int w = 0; w < 2; ++w)
@@ -220,18 +218,15 @@ static void rope_launch(hipStream_t s, RopeArgs &r, bool vec) {
     const int64_t blocks = (r.total + per - 1) / per;
     const int64_t most = (int64_t)mibc_ncu() * 32;   // a workgroup walks several tokens: frequencies are read once
     const dim3 grid((unsigned)(blocks < most ? blocks : most));
-    if (a.interleaved) hipLaunchKernelGGL((rope_kernel<T, true>), grid, dim3(256), 0, s, r);
-    else hipLaunchKernelGGL((rope_kernel<T, false>), grid, dim3(256), 0, s, r);
+    return a.interleaved ? op_launch(rope_kernel<T, true>, grid, 256, 0, s, r) : op_launch(rope_kernel<T, false>, grid, 256, 0, s, r);
 }
 
 static int rope_run(hipStream_t s, const mibc_rope_args &a, bool vec) {
     RopeArgs r{};
     r.a = a;
     r.total = a.batch * a.tokens;
-    if (a.type == MIBC_TYPE_F16) rope_launch<half_t>(s, r, vec);
-    else if (a.type == MIBC_TYPE_BF16) rope_launch<bf16_t>(s, r, vec);
-    else rope_launch<float>(s, r, vec);
-    return op_hip(hipGetLastError(), "rope");
+    return op_hip(a.type == MIBC_TYPE_F16 ? rope_launch<half_t>(s, r, vec) : a.type == MIBC_TYPE_BF16 ? rope_launch<bf16_t>(s, r, vec) : rope_launch<float>(s, r, vec),
+                  "rope");
 }
 
 // launch on a stream of the current device (the engine's own path); checks included

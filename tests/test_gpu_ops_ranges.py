@@ -1,6 +1,7 @@
 """Transformer-layer operators (dorado_amd.ops) at the ends of their ranges, against 64-bit implementations: large caps, weights far below
 the largest, values near the type's end, 8-bit codes that have to be the rounded quotients themselves, pytest -m gpu.  The bounds are
 narrower than those of tests/ops_reference.py: none grows with the cap or with the number of keys."""
+import ctypes
 import math
 
 import pytest
@@ -215,3 +216,25 @@ def test_only_scores_of_minus_infinity(t, d, slopes, n, m):
     R.close(lse[:, :, blind:], bound[1], bound[3], "lse")
     R.close(want, bound[0], bound[2], "alone")
     R.close(wlse, bound[1], bound[3], "lse alone")
+
+
+# ----------------------------------------------------------------------------------------------------- errors of other calls
+def hip_runtime():
+    path = next(line.split()[-1] for line in open("/proc/self/maps") if "libamdhip64" in line)
+    return ctypes.CDLL(path)
+
+
+@pytest.mark.parametrize("which", ["norm", "rope", "attention", "parts"])
+def test_an_older_error_is_not_taken_for_the_calls_own(which):
+    # a call of the program's own that failed (here: a device that does not exist) leaves its error behind for who asks next
+    x, f, long = rnd((1, 4, 2, 64), F16, 27), ops.rope_frequencies(64), rnd((1, 6000, 2, 64), F16, 28)
+    call = {"norm": lambda: ops.rms_norm(x), "rope": lambda: ops.rope(x, freqs=f), "attention": lambda: ops.attention(x, x, x),
+            "parts": lambda: ops.attention(x, long, long)}[which]
+    want, hip = call(), hip_runtime()
+    torch.cuda.synchronize()
+    assert hip.hipSetDevice(99) != 0
+    try:
+        got = call()
+    finally:
+        left = hip.hipGetLastError()
+    assert left != 0 and torch.equal(got, want)      # nor is it taken away from the program
