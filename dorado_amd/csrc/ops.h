@@ -34,6 +34,7 @@ struct OpDevice {
 };
 static inline int op_hip(hipError_t rc, const char *what) {
     if (rc == hipSuccess) return MIBC_OK;
+    (void)hipGetLastError();      // reported here, not by the caller's next call as well
     mibc_gerr() = std::string(what) + ": " + hipGetErrorString(rc);
     return MIBC_ERR_HIP;
 }

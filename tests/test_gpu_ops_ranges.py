@@ -7,7 +7,7 @@ import math
 import pytest
 import torch
 
-from dorado_amd import ops
+from dorado_amd import capi, ops
 from tests import ops_reference as R
 
 pytestmark = pytest.mark.gpu
@@ -238,3 +238,11 @@ def test_an_older_error_is_not_taken_for_the_calls_own(which):
     finally:
         left = hip.hipGetLastError()
     assert left != 0 and torch.equal(got, want)      # nor is it taken away from the program
+
+
+def test_a_failed_call_leaves_no_error_behind():
+    x, hip = rnd((4, 64), F16, 29), hip_runtime()
+    args = ops._NORM_ARGS.pack(x.data_ptr(), 0, 0, 0, x.data_ptr(), 0, 4, 64, 64, 64, 64, 0, 64, 0, 0, 0, 0, 1.0, 1e-5, 0)
+    hip.hipGetLastError()
+    assert ops._entry()[0](99, 0, args) == -2 and capi.lib().mibc_last_error(None).decode().startswith("rms_norm: device: ")
+    assert hip.hipGetLastError() == 0
