@@ -15,8 +15,8 @@ typedef const __attribute__((address_space(1))) char *att_gptr;
 // by more than 2^GROW, so that most tiles rescale nothing.  f16 ends at 2^16 and drops what is below 2^-25: with 2^11 and 2^4 a weight is
 // off by at most 2^-36 of the largest (2^17 such keys by 2^-19), whereas 2^0 and 2^8 lost 0.2 % of the mass of 131072 keys 18 below a
 // single one.  2^13 and 2^2 rescale more often (4 x 16 heads x 4096 of 64 with scores of spread 4: 345 us against 342).  bf16 has f32's range,
-// so sums of its values may end beyond f32: where one did, the pass for values that are not finite runs at 2^-40 (2^28 keys of weight 2^8 stay
-// below 2^-4 of the largest value; values below 2^-86 lose bits beside such sums).
+// so sums of its values may end beyond f32: where one did, the pass for values that are not finite runs at 2^-40 (2^28 keys of weight 2^8
+// stay below 2^-4 of the largest value; values below 2^-86 lose bits beside such sums).
 template <typename T>
 struct AttType;
 template <>
@@ -192,6 +192,9 @@ __device__ __forceinline__ uintx4 att_places(uintx4 v, int kind) {
 //   S^T[key][row] = K Q^T   on 32x32x16: lane (row = lane & 31, half = lane >> 5) holds keys 8 g + 4 half + 0..3 of each 32
 //   O^T[dim][row] = V^T P^T  takes P^T from those very registers: the 16 k-slots of a step are enumerated as the keys a lane holds,
 //   and V^T comes out of the row-major V tile through transposing LDS reads (ds_read_b64_tr_b16).
+// P is rounded to the type of v for that product, which takes one type for both operands; the sums l are of the unrounded values.  Two
+// parts of P would be exact to f32 for half as many matrix instructions again, which is what bounds this kernel: the rounding makes the
+// result's error against 64 bits 1.2 - 1.4 times that of the output's own rounding (f16 2.1e-4 -> 2.5 - 2.9e-4, bf16 1.5e-3 -> 1.9e-3).
 // A row's maximum and sum are one lane pair's: no exchange but one half-wave swap per tile.  Operands are read four instructions
 // ahead, and the products of 16 keys with V run beside the probabilities of the next 16.
 // Head size 128: the matrix pipe works 0.54 of the cycles beside 170 plain instructions per tile and wave (1024 matrix cycles), and power
@@ -508,9 +511,9 @@ __global__ __launch_bounds__(256, D <= 64 ? 3 : 2) void attention_kernel(AttArgs
     if (__any(odd) && lane == 0) flag = 1;
     __syncthreads();
     if (flag) {
-        // something is not finite: from a value or key that the row sees, 0 * (a value that it does not see), or a sum beyond f32.  Once more, tile by tile: values
-        // that are not finite stay out of the products, and the places of NaN (kind 0), infinity (1) and -infinity (2) are
-        // multiplied with the mask instead, so that they reach the rows that see their key and no other
+        // something is not finite: from a value or key that the row sees, 0 * (a value that it does not see), or a sum beyond f32.  Once
+        // more, tile by tile: values that are not finite stay out of the products, and the places of NaN (kind 0), infinity (1) and
+        // -infinity (2) are multiplied with the mask instead, so that they reach the rows that see their key and no other
         start();
 #pragma unroll 1
         for (int it = it0; it < it1; ++it) {

@@ -7,8 +7,8 @@
 // take a workgroup and one LDS exchange per reduction: as few threads as hold the row in six chunks (11320 columns: 256 threads x 6
 // chunks 39 us, 1024 x 2 54), 1024 beyond.
 // Measured: 262144 x 512 f16 with residual 134 us (6.0 TB/s), 16383 x 4096 bf16 with residual, sum and e4m3 codes per 128 columns
-// 89 us (5.3 TB/s), 10000 x 5001 bf16 (unaligned rows) 73 us (4.1 TB/s), 3794 x 11320 e4m3 39 us (3.3 TB/s: the conversion's
-// instructions).
+// 90 us (5.3 TB/s), 10000 x 5001 bf16 with residual (unaligned rows) 73 us (4.1 TB/s), 3794 x 11320 e4m3 38 us (3.4 TB/s: the
+// conversion's instructions, of which the quotients' last step is 1 us).
 #include "ops.h"
 
 struct NormArgs {

@@ -202,7 +202,8 @@ static hipError_t rope_launch(hipStream_t s, RopeArgs &r, bool vec) {
     if (!vec) {
         const int64_t all = r.total * (a.rot_dim / 2 + a.head_dim - a.rot_dim);
         const int64_t blocks = (all + 255) / 256;
-        return op_launch(rope_any_kernel<T>, dim3((unsigned)(blocks < 65536 ? blocks : 65536), (unsigned)((heads + ANY_HEADS - 1) / ANY_HEADS)), 256, 0, s, r);
+        const dim3 grid((unsigned)(blocks < 65536 ? blocks : 65536), (unsigned)((heads + ANY_HEADS - 1) / ANY_HEADS));
+        return op_launch(rope_any_kernel<T>, grid, 256, 0, s, r);
     }
     bool inplace = true;
     for (int w = 0; w < 2; ++w)
@@ -225,8 +226,9 @@ static int rope_run(hipStream_t s, const mibc_rope_args &a, bool vec) {
     RopeArgs r{};
     r.a = a;
     r.total = a.batch * a.tokens;
-    return op_hip(a.type == MIBC_TYPE_F16 ? rope_launch<half_t>(s, r, vec) : a.type == MIBC_TYPE_BF16 ? rope_launch<bf16_t>(s, r, vec) : rope_launch<float>(s, r, vec),
-                  "rope");
+#define ROPE_T(T) rope_launch<T>(s, r, vec)
+    return op_hip(a.type == MIBC_TYPE_F16 ? ROPE_T(half_t) : a.type == MIBC_TYPE_BF16 ? ROPE_T(bf16_t) : ROPE_T(float), "rope");
+#undef ROPE_T
 }
 
 // launch on a stream of the current device (the engine's own path); checks included

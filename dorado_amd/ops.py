@@ -134,6 +134,7 @@ def rms_norm(x, weight=None, *, residual=None, alpha: float = 1.0, eps: float = 
     """h = x + alpha * residual; y = h / sqrt(mean(h^2) + eps) * weight over the last dimension.
 
     x: f16, bf16 or f32, any shape with a contiguous last dimension; residual like x; weight [cols] f32 or of x's type.
+    out and sum_out may be x or residual themselves; any other overlap of an output with an operand is refused, here and below.
     quant "int8" / "e4m3": the codes round(y / s) and the f32 scales s [..., groups], one per row (group 0) or per `group`
     (32, 64, 128) columns.  Returns y or (codes, scales), followed by h (x's type) if return_sum or sum_out is given."""
     dev = _device("rms_norm", x, weight, residual, out, sum_out)
@@ -182,7 +183,8 @@ def rms_norm(x, weight=None, *, residual=None, alpha: float = 1.0, eps: float = 
         args = _NORM_ARGS.pack(
             x.data_ptr(), 0 if residual is None else residual.data_ptr() or _ptr("rms_norm", residual),
             0 if weight is None else weight.data_ptr() or _ptr("rms_norm", weight),
-            0 if sum_out is None else sum_out.data_ptr() or _ptr("rms_norm", sum_out), out.data_ptr(), 0 if scale is None else scale.data_ptr(), x.numel() // cols,
+            0 if sum_out is None else sum_out.data_ptr() or _ptr("rms_norm", sum_out), out.data_ptr(),
+            0 if scale is None else scale.data_ptr(), x.numel() // cols,
             xs, rs, ss, os_, groups, cols, _TYPE[dtype], _TYPE[dtype if weight is None else weight.dtype], _TYPE[out_dtype], group, alpha, eps, 0)
     except _BAD_FIELD as e:
         raise MibcError(f"rms_norm: {e}") from None
@@ -287,7 +289,8 @@ def attention(q, k, v, *, scale=None, causal: bool = False, window=(-1, -1), sof
     [batch] int32: keys in use; query t stands at position k_len - q_tokens + t, or q_start + t.  prefix [batch] int32: that
     many first keys are seen by all.  doc_offsets [n + 1] int32 (batch 1, self attention): documents packed one after the
     other, each seeing itself only; prefix is then [n] and counts from the document's start.  A query that sees nothing gives
-    zeros.  out: None or the tensor to write, which may be q itself.  Returns out like q, or (out, lse f32 [batch, heads, q_tokens])."""
+    zeros.  out: None or the tensor to write, which may be q itself.  f32 arithmetic; probabilities are rounded to the tensors' type
+    before the product with v where a key head has more than 16 query rows.  Returns out like q, or (out, lse f32 [batch, heads, q_tokens])."""
     dev = _device("attention", q, k, v, slopes, k_len, prefix, doc_offsets, out)
     shape, kshape, dtype = q.shape, k.shape, q.dtype
     if len(shape) != 4 or len(kshape) != 4:

@@ -253,8 +253,10 @@ MIBC_API int mibc_svb16_decode(mibc_engine *e, const uint8_t *streams_dev, const
 /* h = x + alpha * residual;  y = h / sqrt(mean(h^2) + eps) * weight  over the last dimension, computed in f32, h not rounded
  * in between.  sum_out (optional) receives h, out receives y, both in `type`; or, out_type I8 / E4M3, out receives
  * round(y / s) (the f32 quotient, then the code, nearest with ties to even), s = max|y| / 127 (I8) or / 448 (E4M3) over the row
- * (group 0) or over each group of 32, 64 or 128 columns, and scale_out [rows][cols / group] receives s.  Where max|y| is 0, s = 1; where a value of the group is not finite, s = NaN
- * and the group's codes are 0; codes end at 127 and 448 (a scale of some 2^-149 steps is off by up to a third; below half a step s = 1).  weight: f32 or `type`, NULL = ones; residual NULL = none.  1 <= cols <= 32768. */
+ * (group 0) or over each group of 32, 64 or 128 columns, and scale_out [rows][cols / group] receives s.
+ * Where max|y| is 0, s = 1; where a value of the group is not finite, s = NaN and the group's codes are 0; codes end at 127 and 448 (a
+ * scale of some 2^-149 steps is off by up to a third; below half a step s = 1).  weight: f32 or `type`, NULL = ones; residual NULL = none.
+ * 1 <= cols <= 32768. */
 typedef struct mibc_rms_norm_args {
     const void *x, *residual, *weight;
     void *sum_out, *out;
@@ -302,11 +304,14 @@ MIBC_API int mibc_rope_frequencies(int scaling, int rot_dim, double theta, doubl
  * j < prefix[n].  doc_offsets [n_docs + 1] (needs batch 1, q_tokens == k_tokens, no k_len, q_start MIBC_ATTN_END; ascending):
  * document d is the tokens [doc_offsets[d], doc_offsets[d + 1]); a token sees its own document only, prefix is then [n_docs] and
  * counts from the document's start, tokens in no document see nothing and are seen by none.  A query that sees nothing, or only
- * scores of -infinity, gives zeros and lse = -infinity.  What a query does not see has no influence on its result, whatever it
- * holds (NaN and infinity included); a NaN or infinity of v that it does see reaches it, however small its weight.  lse (optional)
- * [batch][heads][q_tokens] f32 contiguous: log of the sum of exp(scores).
- * Scores are off by a few 2^-22 of their own size and, for a softcap of up to 64, of the cap's.  softcap / scale may be at most
- * 3e37 and scale / softcap at most 1e38; with slopes, both are at least 1e-18, and slopes / scale must stay inside f32.
+ * scores of -infinity, gives zeros and lse = -infinity.  What a query does not see has no influence on its result, whatever it holds (NaN
+ * and infinity included); a NaN or infinity of v that it does see reaches it, however small its weight (as NaN where no key has any).
+ * lse (optional) [batch][heads][q_tokens] f32 contiguous: log of the sum of exp(scores).
+ * Scores, statistics and sums are f32.  With more than 16 query rows per key head the probabilities are rounded to `type` before their
+ * product with v: each is off by at most 2^-8 of itself in bf16, by 2^-11 or 2^-36 of the row's largest in f16; what is summed for the
+ * denominator and lse is not rounded.  With at most 16 rows they enter as two such parts (2^-16, 2^-22 or the same 2^-36).  Scores are off
+ * by a few 2^-22 of their own size and, for a softcap of up to 64, of the cap's.  softcap / scale may be at most 3e37 and scale / softcap
+ * at most 1e38; with slopes, scale and softcap are at least 1e-18, and slopes / scale must stay inside f32.
  * Types F16, BF16; head_dim 32, 64, 96 or 128; token and head strides multiples of 8 elements, pointers aligned to 16 bytes.
  * workspace: mibc_attention_workspace(a) bytes on the device (0, as for any call with fewer than 512 keys: may be NULL), the
  * call's own until it has completed. */

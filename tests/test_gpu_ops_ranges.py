@@ -246,3 +246,12 @@ def test_a_failed_call_leaves_no_error_behind():
     hip.hipGetLastError()
     assert ops._entry()[0](99, 0, args) == -2 and capi.lib().mibc_last_error(None).decode().startswith("rms_norm: device: ")
     assert hip.hipGetLastError() == 0
+
+
+@pytest.mark.parametrize("n,m", PATHS + [(1, 9000), (40, 9000)])
+def test_values_beside_scores_of_minus_infinity(n, m):
+    # no key has a weight: zeros, and NaN in the columns where a seen value is not finite
+    q, k, v = rnd((1, n, 1, 64), BF16, 30).abs() + 0.1, torch.full((1, m, 1, 64), -math.inf, dtype=BF16, device="cuda"), rnd((1, m, 1, 64), BF16, 31)
+    v[0, m // 2, 0, 3], v[0, m // 3, 0, 4], v[0, 0, 0, 5] = math.nan, math.inf, -math.inf
+    out, lse = ops.attention(q, k, v, return_lse=True)
+    assert out[..., 3:6].isnan().all() and (out[..., :3] == 0).all() and (out[..., 6:] == 0).all() and (lse == -math.inf).all()
