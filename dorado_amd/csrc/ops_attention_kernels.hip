@@ -17,13 +17,16 @@ typedef const __attribute__((address_space(1))) char *att_gptr;
 // single one.  2^13 and 2^2 rescale more often (4 x 16 heads x 4096 of 64 with scores of spread 4: 345 us against 342).  bf16 has f32's range,
 // so sums of its values may end beyond f32: where one did, the pass for values that are not finite runs at 2^-40 (2^28 keys of weight 2^8
 // stay below 2^-4 of the largest value; values below 2^-86 lose bits beside such sums).
+// The exponent is one fma of the raw score and minus the maximum, which was rounded: all weights of a row are off by one factor, which
+// cancels, but whose own exponent is up to 2^-25 of the maximum.  Rows whose maximum is at FAR or beyond, where it nears what the type
+// holds, take the other pass too; a score is rounded like the maximum there before the two are subtracted.
 template <typename T>
 struct AttType;
 template <>
 struct AttType<half_t> {
     typedef half8_t vec8;
     static constexpr unsigned EXPONENT = 0x7c00, MANTISSA = 0x03ff, ONE = 0x3c00;
-    static constexpr float LIFT = 11.0f, LIFT_AGAIN = 11.0f, GROW = 4.0f;
+    static constexpr float LIFT = 11.0f, LIFT_AGAIN = 11.0f, GROW = 4.0f, FAR = 0x1p22f;
     static __device__ __forceinline__ float16_t mfma32(vec8 a, vec8 b, float16_t c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
     static __device__ __forceinline__ float4_t mfma16(vec8 a, vec8 b, float4_t c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
 };
@@ -31,7 +34,7 @@ template <>
 struct AttType<bf16_t> {
     typedef bf16x8_t vec8;
     static constexpr unsigned EXPONENT = 0x7f80, MANTISSA = 0x007f, ONE = 0x3f80;
-    static constexpr float LIFT = 0.0f, LIFT_AGAIN = -40.0f, GROW = 8.0f;
+    static constexpr float LIFT = 0.0f, LIFT_AGAIN = -40.0f, GROW = 8.0f, FAR = 0x1p28f;
     static __device__ __forceinline__ float16_t mfma32(vec8 a, vec8 b, float16_t c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
     static __device__ __forceinline__ float4_t mfma16(vec8 a, vec8 b, float4_t c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
 };
@@ -164,9 +167,18 @@ struct AttScore {
         const float far = copysignf(most * (1.0f - e) * __builtin_amdgcn_rcpf(1.0f + e), x);
         return fabsf(y) < 0.5f ? x * t : far;                                  // NaN: far, which is NaN
     }
+    // of the raw score x; off: minus the maximum, in the first pass with what else is added to the exponent
+    template <bool SAFE>
+    __device__ __forceinline__ float weight(float x, float off, float lift) const {
+        return SAFE ? att_exp2((fmaf(x, mul, add) + off) + lift) : att_exp2(fmaf(x, mul, off));
+    }
     __device__ __forceinline__ float larger(float a, float b) const { return CAP == ATT_NEAR ? fminf(a, b) : fmaxf(a, b); }
 };
 
+template <typename T>
+__device__ __forceinline__ bool att_far(float m) {     // a row's maximum, which may be -infinity (no key) or not a number
+    return fabsf(m) >= AttType<T>::FAR && !__builtin_isinf(m);
+}
 // 1 where a value is NaN (kind 0), infinity (1), -infinity (2), else 0
 template <typename T>
 __device__ __forceinline__ uintx4 att_places(uintx4 v, int kind) {
@@ -439,15 +451,16 @@ __global__ __launch_bounds__(256, D <= 64 ? 3 : 2) void attention_kernel(AttArgs
 #pragma unroll
                 for (int r = 0; r < 16; ++r) o[db][r] = decltype(safe_)::value ? att_weigh(f, o[db][r]) : o[db][r] * f;
         }
-        off = score.add + (decltype(safe_)::value ? X::LIFT_AGAIN : X::LIFT) - (m == -INFINITY ? 0.0f : m);
+        off = (decltype(safe_)::value ? 0.0f : score.add + X::LIFT) - (m == -INFINITY ? 0.0f : m);
     };
-    auto probabilities = [&](int k) {       // of 16 keys
+    auto probabilities = [&](auto safe_, int k) {       // of 16 keys
+        constexpr bool SAFE = decltype(safe_)::value;
         uintx4 w;
         float sum = 0.0f;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            const float x = att_exp2(fmaf(s[k >> 1][8 * (k & 1) + 2 * i], score.mul, off));
-            const float y = att_exp2(fmaf(s[k >> 1][8 * (k & 1) + 2 * i + 1], score.mul, off));
+            const float x = score.template weight<SAFE>(s[k >> 1][8 * (k & 1) + 2 * i], off, X::LIFT_AGAIN);
+            const float y = score.template weight<SAFE>(s[k >> 1][8 * (k & 1) + 2 * i + 1], off, X::LIFT_AGAIN);
             sum += x + y;                   // before the rounding: the sum is also a result
             w[i] = op_pack2(x, y, T());
         }
@@ -482,14 +495,14 @@ __global__ __launch_bounds__(256, D <= 64 ? 3 : 2) void attention_kernel(AttArgs
 #pragma unroll
         for (int db = 0; db < N; ++db) v[0][db] = values(AT, db, 0);
         vec8 pf[2];
-        pf[0] = probabilities(0);
+        pf[0] = probabilities(std::false_type(), 0);
         ATT_FENCE();
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
             if (k < 3) {
 #pragma unroll
                 for (int db = 0; db < N; ++db) v[(k + 1) & 1][db] = values(AT, db, k + 1);
-                pf[(k + 1) & 1] = probabilities(k + 1);
+                pf[(k + 1) & 1] = probabilities(std::false_type(), k + 1);
             }
 #pragma unroll
             for (int db = 0; db < N; ++db) o[db] = X::mfma32(__builtin_bit_cast(vec8, v[k & 1][db]), pf[k & 1], o[db]);
@@ -507,12 +520,12 @@ __global__ __launch_bounds__(256, D <= 64 ? 3 : 2) void attention_kernel(AttArgs
     for (int db = 0; db < D / 32; ++db)
 #pragma unroll
         for (int r = 0; r < 16; ++r) zero[r & 3] = fmaf(o[db][r], 0.0f, zero[r & 3]);
-    const bool odd = !(zero[0] + zero[1] + zero[2] + zero[3] == 0.0f);
+    const bool odd = !(zero[0] + zero[1] + zero[2] + zero[3] == 0.0f) || att_far<T>(m);
     if (__any(odd) && lane == 0) flag = 1;
     __syncthreads();
     if (flag) {
-        // something is not finite: from a value or key that the row sees, 0 * (a value that it does not see), or a sum beyond f32.  Once
-        // more, tile by tile: values that are not finite stay out of the products, and the places of NaN (kind 0), infinity (1) and
+        // something is not finite: from a value or key that the row sees, 0 * (a value that it does not see), or a sum beyond f32; or a
+        // maximum is too far out.  Once more, tile by tile: values that are not finite stay out of the products, and the places of NaN (kind 0), infinity (1) and
         // -infinity (2) are multiplied with the mask instead, so that they reach the rows that see their key and no other
         start();
 #pragma unroll 1
@@ -528,7 +541,7 @@ __global__ __launch_bounds__(256, D <= 64 ? 3 : 2) void attention_kernel(AttArgs
             maxima(std::true_type());
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
-                const vec8 pf = probabilities(k);
+                const vec8 pf = probabilities(std::true_type(), k);
                 uintx4 w;
 #pragma unroll
                 for (int e = 0; e < 4; ++e)
@@ -748,13 +761,13 @@ __global__ __launch_bounds__(256, 2) void attention_token_kernel(AttArgs p) {
 #pragma unroll
                     for (int r = 0; r < 4; ++r) o[db][r] = SAFE ? att_weigh(f, o[db][r]) : o[db][r] * f;
             }
-            const float off = score.add + (SAFE ? X::LIFT_AGAIN : X::LIFT) - (m == -INFINITY ? 0.0f : m);
+            const float off = (SAFE ? 0.0f : score.add + X::LIFT) - (m == -INFINITY ? 0.0f : m);
             uintx4 hi, lo;
 #pragma unroll
             for (int i = 0; i < 2; ++i)
 #pragma unroll
                 for (int r = 0; r < 4; r += 2) {
-                    const float x = att_exp2(fmaf(s[i][r], score.mul, off)), y = att_exp2(fmaf(s[i][r + 1], score.mul, off));
+                    const float x = score.template weight<SAFE>(s[i][r], off, X::LIFT_AGAIN), y = score.template weight<SAFE>(s[i][r + 1], off, X::LIFT_AGAIN);
                     l += x + y;
                     const unsigned h = op_pack2(x, y, T());
                     hi[2 * i + (r >> 1)] = h;
@@ -800,7 +813,7 @@ __global__ __launch_bounds__(256, 2) void attention_token_kernel(AttArgs p) {
     for (int db = 0; db < D / 16; ++db)
 #pragma unroll
         for (int r = 0; r < 4; ++r) zero = fmaf(o[db][r], 0.0f, zero);
-    if (__any(zero != 0.0f)) {
+    if (__any(zero != 0.0f || att_far<T>(m))) {
         pass(std::true_type());
         m += X::LIFT - X::LIFT_AGAIN;     // the other waves' unit
     }

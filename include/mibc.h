@@ -250,8 +250,8 @@ MIBC_API int mibc_svb16_decode(mibc_engine *e, const uint8_t *streams_dev, const
 #define MIBC_TYPE_I8 3
 #define MIBC_TYPE_E4M3 4 /* OCP e4m3 (no infinity, largest value 448) */
 
-/* h = x + alpha * residual;  y = h / sqrt(mean(h^2) + eps) * weight  over the last dimension, computed in f32, h not rounded
- * in between.  sum_out (optional) receives h, out receives y, both in `type`; or, out_type I8 / E4M3, out receives
+/* h = x + alpha * residual;  y = h / sqrt(mean(h^2) + eps) * weight  over the last dimension, computed in f32 (squares beyond it: y = 0), h
+ * not rounded in between.  sum_out (optional) receives h, out receives y, both in `type`; or, out_type I8 / E4M3, out receives
  * round(y / s) (the f32 quotient, then the code, nearest with ties to even), s = max|y| / 127 (I8) or / 448 (E4M3) over the row
  * (group 0) or over each group of 32, 64 or 128 columns, and scale_out [rows][cols / group] receives s.
  * Where max|y| is 0, s = 1; where a value of the group is not finite, s = NaN and the group's codes are 0; codes end at 127 and 448 (a

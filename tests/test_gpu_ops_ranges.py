@@ -255,3 +255,48 @@ def test_values_beside_scores_of_minus_infinity(n, m):
     v[0, m // 2, 0, 3], v[0, m // 3, 0, 4], v[0, 0, 0, 5] = math.nan, math.inf, -math.inf
     out, lse = ops.attention(q, k, v, return_lse=True)
     assert out[..., 3:6].isnan().all() and (out[..., :3] == 0).all() and (out[..., 6:] == 0).all() and (lse == -math.inf).all()
+
+
+# ----------------------------------------------------------------------------------------------------------- scores of any size
+@pytest.mark.parametrize("n,m", PATHS + [(1, 9000), (40, 9000)])
+@pytest.mark.parametrize("t,size", [(F16, 3.0), (F16, 1000.0), (F16, 8000.0), (F16, 60000.0), (BF16, 1e4), (BF16, 1e8), (BF16, 1e13), (BF16, 1e17)])
+@pytest.mark.parametrize("cap", [0.0, 1e25])
+def test_one_key_takes_all(cap, t, size, n, m):
+    # one key along the queries, the others against them: its value and nothing else, at scores from 1e2 to 1e36
+    q, v = torch.full((2, n, 2, 64), size, dtype=t), rnd((2, m, 1, 64), t, 32)
+    q[1] *= 0.7
+    k = torch.full((2, m, 1, 64), -size, dtype=t)
+    at = (m - n) // 2                                  # seen by every row
+    k[:, at] *= -0.9
+    out, lse = ops.attention(q.cuda(), k.cuda(), v, causal=True, return_lse=True, softcap=cap)
+    assert torch.equal(out, v[:, at:at + 1].expand(2, n, 2, 64))
+    s = (q.double() * k[:, at:at + 1].double()).sum(-1).transpose(1, 2) * 64 ** -0.5
+    if cap:
+        s = cap * torch.tanh(s / cap)
+    assert ((lse.cpu().double() - s).abs() <= 2.0 ** -18 * s).all()
+
+
+@pytest.mark.parametrize("n,m", PATHS)
+@pytest.mark.parametrize("t,low,size", [(F16, -65504.0, 1.0), (F16, -65504.0, 300.0), (BF16, torch.finfo(BF16).min, 1e-3), (BF16, -1e30, 1e-3), (BF16, 1e20, 1e10)])
+def test_equal_scores_of_any_size_give_the_mean(t, low, size, n, m):
+    # every key at the type's lowest value (or far up): finite scores, all the same
+    q, k, v = torch.full((1, n, 1, 128), size, dtype=t, device="cuda"), torch.full((1, m, 1, 128), low, dtype=t, device="cuda"), rnd((1, m, 1, 128), t, 33)
+    out, lse = ops.attention(q, k, v, return_lse=True)
+    want = v.double().mean(1, keepdim=True).expand(1, n, 1, 128).cpu()
+    # in parts, weights of parts whose lengths differ by a tile of at most 64 keys in at least 256 are equal to within the score's rounding
+    parts = v.double().abs().mean().cpu() * 0.5 if m >= 512 else 0.0
+    R.close(out, want, R.u(t) * want.abs() + v.double().abs().mean(1, keepdim=True).cpu() * (R.u(t) + 2.0 ** -19) + parts, "mean")
+    s = float(q[0, 0, 0, 0]) * float(k[0, 0, 0, 0]) * 128 ** 0.5 + math.log(m)
+    assert ((lse.cpu().double() - s).abs() <= 2.0 ** -18 * abs(s)).all()
+
+
+@pytest.mark.parametrize("n,m", PATHS)
+def test_large_scores_behind_ordinary_ones(n, m):
+    # keys at the lowest value first, ordinary ones behind them: as if the first were not there
+    q, k, v = rnd((1, n, 2, 64), BF16, 34).abs() + 0.1, rnd((1, m, 1, 64), BF16, 35), rnd((1, m, 1, 64), BF16, 36)
+    low = k.clone()
+    low[:, :m - n - 20] = -1e37
+    want = reference(q, k[:, m - n - 20:], v[:, m - n - 20:], causal=True)
+    out, lse = ops.attention(q, low, v, causal=True, return_lse=True)
+    R.close(out, want[0], want[2], "out")
+    R.close(lse, want[1], want[3], "lse")
