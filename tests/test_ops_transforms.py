@@ -111,3 +111,17 @@ def test_compiled_callers_get_the_same_results():
         return ops.attention(q, k, y) + 1
 
     assert torch.equal(torch.compile(layer, backend="eager")(x), layer(x))
+
+
+@gpu
+def test_operators_work_beside_tangents():
+    # a dual level that concerns none of the operands: whole numbers, codes and tensors without versions among them
+    x, f, p = torch.ones((1, 4, 2, 64), dtype=torch.float16, device="cuda"), FREQS.cuda(), torch.arange(4, device="cuda", dtype=torch.int32)
+    want = ops.rms_norm(x, quant="int8")[0], ops.rope(x, freqs=f, positions=p), ops.attention(x, x, x, k_len=p[3:])
+    with fwd.dual_level():
+        codes = torch.empty(x.shape, dtype=torch.int8, device="cuda")
+        got = ops.rms_norm(x, quant="int8", out=codes)[0], ops.rope(x, freqs=f, positions=p), ops.attention(x, x, x, k_len=p[3:])
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    with torch.inference_mode(), fwd.dual_level():
+        y = torch.ones_like(x)
+        assert torch.equal(ops.rope(y, freqs=f, positions=p, out=y), want[1])
